@@ -1,0 +1,235 @@
+// Rules for the next token, applied to the logits of a step's rows in one pass: penalties for tokens that were seen, biases of single
+// tokens, grammar masks of one bit per token.
+//
+//   z = logit;  count c > 0:  z = (z > 0 ? z / repetition : z * repetition) - presence - frequency * c
+//   z += sum of the row's biases for the token (a sum of minus infinity forbids the token, whatever z is)
+//   z = minus infinity where the row's mask has no bit (whatever z is)
+//
+// What bounds it is traffic: two or four bytes in, four out, four of counts where a row has penalties. A row is cut into slices of
+// 4096 values, a CTA each, and a thread asks for all it needs of two groups of eight values before it uses any of it. Groups
+// that the mask forbids entirely are written without being read (of a grammar's states most allow a few tokens). Biases are few: a CTA
+// looks through its row's list once, and drops what falls into its slice into shared memory behind a bit per value.
+#include "common.cuh"
+
+namespace edl {
+namespace {
+
+constexpr int RULE_THREADS = 256, RULE_GROUPS = 2, RULE_SLICE = RULE_THREADS * RULE_GROUPS * 8;
+
+struct RuleArgs {
+  const void* logits;
+  void* out;
+  long long ld, ldo;
+  int V, slices;
+  const int* counts;
+  long long ld_counts;
+  const int* count_rows;
+  int slots;
+  const float *presence, *frequency, *repetition;
+  const int* bias_ptr;
+  const int* bias_ids;
+  const float* bias_values;
+  int bias_n;
+  const uint32_t* bits;
+  long long ld_bits;
+  const int* mask_rows;
+  int masks;
+  int* status;
+};
+
+template <typename T>
+__device__ __forceinline__ float to_float(T v) {
+  if constexpr (sizeof(T) == 2) return __bfloat162float(v);
+  else return v;
+}
+
+// WIDE: a thread's eight values are neighbours; else they lie 256 apart, so that rows of any alignment are read in whole lines.
+template <typename T, typename TO, bool WIDE>
+__global__ void __launch_bounds__(RULE_THREADS) rules_kernel(const RuleArgs a) {
+  extern __shared__ __align__(16) float s_add[];                                       // [RULE_SLICE], set where the bit is
+  uint32_t* s_bit = reinterpret_cast<uint32_t*>(s_add + RULE_SLICE);                   // [RULE_SLICE / 32]
+  const int row = blockIdx.x / a.slices, tid = threadIdx.x;
+  const int v0 = (blockIdx.x % a.slices) * RULE_SLICE;
+  const T* src = reinterpret_cast<const T*>(a.logits) + row * a.ld;
+  TO* dst = reinterpret_cast<TO*>(a.out) + row * a.ldo;
+
+  int mrow = a.mask_rows ? a.mask_rows[row] : a.bits ? row : -1;
+  int slot = !a.counts ? -1 : a.count_rows ? a.count_rows[row] : row;
+  if (mrow >= a.masks || slot >= a.slots) {
+    if (a.status && tid == 0) atomicCAS(a.status, 0, EDL_BAD_INDEX);
+    if (mrow >= a.masks) mrow = -1;
+    if (slot >= a.slots) slot = -1;
+  }
+  const float pres = a.presence ? a.presence[row] : 0.f, freq = a.frequency ? a.frequency[row] : 0.f;
+  const float rep = a.repetition ? a.repetition[row] : 1.f;
+  const int* cnt = slot >= 0 && (pres != 0.f || freq != 0.f || rep != 1.f) ? a.counts + (long long)slot * a.ld_counts : nullptr;
+  const uint32_t* bits = mrow >= 0 ? a.bits + (long long)mrow * a.ld_bits : nullptr;
+
+  auto index = [&](int grp, int j) { return WIDE ? v0 + (grp * RULE_THREADS + tid) * 8 + j : v0 + (grp * 8 + j) * RULE_THREADS + tid; };
+  uint32_t allow[RULE_GROUPS];
+#pragma unroll
+  for (int q = 0; q < RULE_GROUPS; ++q) {
+    allow[q] = 0;
+    if constexpr (WIDE) {
+      if (index(q, 0) < a.V) allow[q] = bits ? reinterpret_cast<const uint8_t*>(bits)[index(q, 0) >> 3] : 0xff;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int v = index(q, j);
+        if (v < a.V) allow[q] |= (bits ? (bits[v >> 5] >> (v & 31)) & 1u : 1u) << j;
+      }
+    }
+  }
+  float z[RULE_GROUPS][8];
+  int seen[RULE_GROUPS][8];
+#pragma unroll
+  for (int q = 0; q < RULE_GROUPS; ++q) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      z[q][j] = 0.f;
+      seen[q][j] = 0;
+    }
+    if constexpr (WIDE) {
+      if (allow[q]) {
+        const int v = index(q, 0);
+        if constexpr (sizeof(T) == 2) {
+          const uint4 x = *reinterpret_cast<const uint4*>(src + v);
+          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = unpack_bf16x2(w[j]);
+            z[q][2 * j] = f.x;
+            z[q][2 * j + 1] = f.y;
+          }
+        } else {
+          const float4 x = *reinterpret_cast<const float4*>(src + v), y = *reinterpret_cast<const float4*>(src + v + 4);
+          z[q][0] = x.x; z[q][1] = x.y; z[q][2] = x.z; z[q][3] = x.w;
+          z[q][4] = y.x; z[q][5] = y.y; z[q][6] = y.z; z[q][7] = y.w;
+        }
+        if (cnt) {
+          const int4 x = *reinterpret_cast<const int4*>(cnt + v), y = *reinterpret_cast<const int4*>(cnt + v + 4);
+          seen[q][0] = x.x; seen[q][1] = x.y; seen[q][2] = x.z; seen[q][3] = x.w;
+          seen[q][4] = y.x; seen[q][5] = y.y; seen[q][6] = y.z; seen[q][7] = y.w;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (allow[q] >> j & 1) {
+          z[q][j] = to_float(src[index(q, j)]);
+          if (cnt) seen[q][j] = cnt[index(q, j)];
+        }
+    }
+  }
+
+  if (a.bias_ptr) {
+    for (int i = tid; i < RULE_SLICE / 32; i += RULE_THREADS) s_bit[i] = 0;
+    __syncthreads();
+    int lo = a.bias_ptr[row], hi = a.bias_ptr[row + 1];
+    if (lo < 0 || hi > a.bias_n || lo > hi) {
+      if (a.status && tid == 0) atomicCAS(a.status, 0, EDL_BAD_INDEX);
+      lo = hi = 0;
+    }
+    for (int e = lo + tid; e < hi; e += RULE_THREADS) {
+      const int id = a.bias_ids[e];
+      if (id < 0 || id >= a.V) {
+        if (a.status) atomicCAS(a.status, 0, EDL_BAD_INDEX);
+        continue;
+      }
+      if (id < v0 || id >= v0 + RULE_SLICE || (e > lo && a.bias_ids[e - 1] == id)) continue;
+      float sum = a.bias_values[e];                                       // the first of a token's entries adds up the rest, in order
+      for (int f = e + 1; f < hi && a.bias_ids[f] == id; ++f) sum += a.bias_values[f];
+      s_add[id - v0] = sum;
+      atomicOr(&s_bit[(id - v0) >> 5], 1u << ((id - v0) & 31));
+    }
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int q = 0; q < RULE_GROUPS; ++q) {
+    if (cnt) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (seen[q][j] > 0) {
+          float x = z[q][j];
+          if (rep != 1.f) x = x > 0.f ? x / rep : x * rep;
+          z[q][j] = x - (pres + freq * (float)seen[q][j]);
+        }
+    }
+    if (a.bias_ptr) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int at = index(q, j) - v0;
+        if (s_bit[at >> 5] >> (at & 31) & 1) {
+          const float add = s_add[at];
+          z[q][j] = add == -INFINITY ? add : z[q][j] + add;
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (!(allow[q] >> j & 1)) z[q][j] = -INFINITY;
+    if constexpr (WIDE) {
+      const int v = index(q, 0);
+      if (v < a.V) {
+        if constexpr (sizeof(TO) == 2) {
+          *reinterpret_cast<uint4*>(dst + v) = make_uint4(pack_bf16x2(z[q][0], z[q][1]), pack_bf16x2(z[q][2], z[q][3]),
+                                                          pack_bf16x2(z[q][4], z[q][5]), pack_bf16x2(z[q][6], z[q][7]));
+        } else {
+          *reinterpret_cast<float4*>(dst + v) = make_float4(z[q][0], z[q][1], z[q][2], z[q][3]);
+          *reinterpret_cast<float4*>(dst + v + 4) = make_float4(z[q][4], z[q][5], z[q][6], z[q][7]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (index(q, j) < a.V) {
+          if constexpr (sizeof(TO) == 2) dst[index(q, j)] = __float2bfloat16_rn(z[q][j]);
+          else dst[index(q, j)] = z[q][j];
+        }
+    }
+  }
+}
+
+}  // namespace
+}  // namespace edl
+
+using namespace edl;
+
+// logits, out: [R, V] (bf16 or fp32 each; the same memory for in place). counts [slots, *] int32 with a row per entry of count_rows (negative:
+// no penalties; null: row r), presence / frequency / repetition fp32 [R] or null. bias_ptr [R + 1], ids (sorted within a row) and values
+// of bias_n entries, or null. bits: [masks, ld_bits] words, mask_rows [R] (negative: no mask; null: row r).
+EDL_HOST_API int edl_adjust_logits(const void* logits, int in_f32, long long ld, void* out, int out_f32, long long ldo, int R, int V,
+                                   const int* counts, long long ld_counts, int slots, const int* count_rows, const float* presence,
+                                   const float* frequency, const float* repetition, const int* bias_ptr, const int* bias_ids,
+                                   const float* bias_values, int bias_n, const void* bits, long long ld_bits, int masks,
+                                   const int* mask_rows, int* status, void* stream) {
+  if (R <= 0 || V <= 0) return 0;
+  if (logits == out && (in_f32 != out_f32 || ld != ldo)) {
+    set_last_error("edl_adjust_logits: in place needs one type and one stride");
+    return -1;
+  }
+  RuleArgs a{logits, out, ld, ldo, V, (V + RULE_SLICE - 1) / RULE_SLICE, counts, ld_counts, count_rows, slots, presence, frequency, repetition,
+             bias_ptr, bias_ids, bias_values, bias_n, (const uint32_t*)bits, ld_bits, bits ? mask_rows : nullptr, masks, status};
+  auto odd = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; };
+  const bool wide = V % 8 == 0 && ld % (in_f32 ? 4 : 8) == 0 && ldo % (out_f32 ? 4 : 8) == 0 && !odd(logits) && !odd(out) &&
+                    (!counts || (ld_counts % 4 == 0 && !odd(counts)));
+  const long long ctas = (long long)R * a.slices;
+  if (ctas > 0x7fffffffLL) {
+    set_last_error("edl_adjust_logits: too many values for one launch");
+    return -1;
+  }
+  const int smem = bias_ptr ? RULE_SLICE * 4 + RULE_SLICE / 8 : 0;
+  cudaStream_t st = (cudaStream_t)stream;
+#define EDL_RULES(TI, TO)                                                                         \
+  {                                                                                               \
+    if (wide) rules_kernel<TI, TO, true><<<(unsigned)ctas, RULE_THREADS, smem, st>>>(a);          \
+    else rules_kernel<TI, TO, false><<<(unsigned)ctas, RULE_THREADS, smem, st>>>(a);              \
+  }
+  if (in_f32 && out_f32) EDL_RULES(float, float)
+  else if (in_f32) EDL_RULES(float, __nv_bfloat16)
+  else if (out_f32) EDL_RULES(__nv_bfloat16, float)
+  else EDL_RULES(__nv_bfloat16, __nv_bfloat16)
+#undef EDL_RULES
+  return check_cuda(cudaGetLastError(), "adjust_logits launch");
+}

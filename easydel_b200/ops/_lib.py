@@ -9,6 +9,7 @@ callers use the fp32 reference math in :mod:`easydel_b200.ops.reference`.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 import threading
@@ -134,6 +135,13 @@ def stream_ptr() -> int:
     if _raw_stream is None or _device_index is None:
         return torch.cuda.current_stream().cuda_stream
     return _raw_stream(_device_index())
+
+
+def on_device(device: torch.device):
+    """Launches go to a stream of the current device: makes ``device`` the current one where it is not."""
+    if device.index in (None, torch.cuda.current_device()):
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

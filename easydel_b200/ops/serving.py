@@ -19,6 +19,8 @@ _lib.register("edl_attn_paged_sigmoid", i32, [vp, vp, vp, vp, i64, i64, i64, i64
                                               i32, i32, f32, i32, i32, vp, vp, i64, f32, vp, vp])
 _lib.register("edl_paged_kv_append", i32, [vp, vp, vp, vp, vp, i32, i32, i64, i64, i64, i64, vp, vp])
 _lib.register("edl_sample", i32, [vp, i32, i64, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, i64, vp, vp, vp, vp, vp])
+_lib.register("edl_adjust_logits", i32, [vp, i32, i64, vp, i32, i64, i32, i32, vp, i64, i32, vp, vp, vp, vp, vp, vp, vp, i32, vp, i64, i32,
+                                         vp, vp, vp])
 _lib.register("edl_count_update", i32, [vp, i64, vp, vp, i32, i32, vp])
 _lib.register("edl_gather_rows", i32, [vp, vp, vp, i32, i32, i64, vp])
 _lib.register("edl_attn_decode", i32, [vp, vp, vp, vp, vp, i64, i64, i64, i64, vp, vp, i32, i32, i64, i32, i32, i32, i32,
@@ -410,6 +412,104 @@ def sample_reference(logits, *, temperature=None, top_k=None, top_p=None, min_p=
         out[r] = int(idx[j])
         lps[r] = torch.log_softmax(z[r] / t, -1)[idx[j]]
     return out, (lps if want_logprob else None)
+
+
+def adjust_logits(logits: torch.Tensor, *, counts: torch.Tensor | None = None, count_rows: torch.Tensor | None = None, presence=None,
+                  frequency=None, repetition=None, bias: tuple | None = None, mask: tuple | None = None,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rules for the next token on ``[R, V]`` logits (bfloat16 or float32), in one pass and in this order: penalties, biases, masks.
+
+    ``counts [slots, V]`` int32: how often a token was seen, row ``count_rows[r]`` (int32; negative: no penalties; None: row r) for
+    row r, with ``presence`` / ``frequency`` / ``repetition`` (float32 ``[R]``) as in :func:`sample`. ``bias``: ``(ptr, ids, values)``: entries
+    ``ptr[r]:ptr[r + 1]`` (int32 ``[R + 1]``) of ``ids`` (int32, sorted within a row; a repeated id adds up) and ``values`` (float32) belong to
+    row r; minus infinity forbids a token whatever its logit. ``mask``: ``(bits, rows)``: int32 words ``[masks, >= ceil(V / 32)]``, bit
+    ``t % 32`` of word ``t // 32`` allows token t, and the mask of each row (int32; negative: none; ``rows`` None: mask r). What a mask
+    forbids becomes minus infinity, whatever it was. ``out``: bfloat16 or float32 ``[R, V]`` (``logits`` itself for in place); None:
+    a new float32 tensor. Rows, tokens or masks out of range count as absent and set the status word that ``_lib.check_status`` reads.
+    """
+    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"logits are [rows, vocabulary] of bfloat16 or float32, got {tuple(logits.shape)} of {logits.dtype}")
+    R_, V = logits.shape
+    ptr, ids, values = bias if bias is not None else (None, None, None)
+    bits, mask_rows = mask if mask is not None else (None, None)
+    for name, t, dtype, shape in (("count_rows", count_rows, torch.int32, (R_,)), ("presence", presence, torch.float32, (R_,)),
+                                  ("frequency", frequency, torch.float32, (R_,)), ("repetition", repetition, torch.float32, (R_,)),
+                                  ("bias ptr", ptr, torch.int32, (R_ + 1,)), ("bias ids", ids, torch.int32, None),
+                                  ("bias values", values, torch.float32, None if ids is None else tuple(ids.shape)),
+                                  ("mask rows", mask_rows, torch.int32, (R_,))):
+        if t is None:
+            if name.startswith("bias") and bias is not None:
+                raise ValueError("bias is (ptr, ids, values)")
+            continue
+        if t.dtype != dtype or t.dim() != 1 or not t.is_contiguous() or (shape is not None and tuple(t.shape) != shape):
+            raise ValueError(f"{name} is a contiguous {dtype} tensor of shape {shape or '[entries]'}, got {tuple(t.shape)} of {t.dtype}")
+    if counts is None:
+        if count_rows is not None:
+            raise ValueError("count_rows without counts")
+    elif counts.dim() != 2 or counts.dtype != torch.int32 or counts.shape[1] < V or (V > 1 and counts.stride(1) != 1) or \
+            (count_rows is None and counts.shape[0] < R_):
+        raise ValueError(f"counts are int32 rows of at least {V} tokens, one for each row without count_rows, got {tuple(counts.shape)} "
+                         f"of {counts.dtype}")
+    if mask is not None and (bits.dim() != 2 or bits.dtype != torch.int32 or bits.shape[1] < (V + 31) // 32 or
+                             (bits.shape[1] > 1 and bits.stride(1) != 1) or (mask_rows is None and bits.shape[0] < R_)):
+        raise ValueError(f"masks are int32 rows of at least {(V + 31) // 32} words, got {tuple(bits.shape)} of {bits.dtype}")
+    if out is not None and (out.shape != logits.shape or out.dtype not in (torch.bfloat16, torch.float32)):
+        raise ValueError(f"out is {tuple(out.shape)} of {out.dtype}, logits {tuple(logits.shape)}")
+    for t in (counts, count_rows, presence, frequency, repetition, ptr, ids, values, bits, mask_rows, out):
+        if t is not None and t.device != logits.device:
+            raise ValueError(f"tensors on {logits.device} and {t.device}")
+    if not logits.is_cuda:
+        z = adjust_logits_reference(logits, counts, count_rows, presence, frequency, repetition, bias, mask)
+        return z if out is None else out.copy_(z)
+    if V > 1 and logits.stride(1) != 1:
+        if out is logits:
+            return out.copy_(adjust_logits(logits.contiguous(), counts=counts, count_rows=count_rows, presence=presence,
+                                           frequency=frequency, repetition=repetition, bias=bias, mask=mask))
+        logits = logits.contiguous()
+    if out is None:
+        out = torch.empty((R_, V), dtype=torch.float32, device=logits.device)
+    elif V > 1 and out.stride(1) != 1:
+        return out.copy_(adjust_logits(logits, counts=counts, count_rows=count_rows, presence=presence, frequency=frequency,
+                                       repetition=repetition, bias=bias, mask=mask))
+    with _lib.on_device(logits.device):
+        _lib.call("edl_adjust_logits", logits.data_ptr(), int(logits.dtype == torch.float32), logits.stride(0), out.data_ptr(),
+                  int(out.dtype == torch.float32), out.stride(0), R_, V, _lib.ptr(counts), 0 if counts is None else counts.stride(0),
+                  0 if counts is None else counts.shape[0], _lib.ptr(count_rows), _lib.ptr(presence), _lib.ptr(frequency),
+                  _lib.ptr(repetition), _lib.ptr(ptr), _lib.ptr(ids), _lib.ptr(values), 0 if ids is None else ids.numel(),
+                  _lib.ptr(bits), 0 if bits is None else bits.stride(0), 0 if bits is None else bits.shape[0], _lib.ptr(mask_rows),
+                  _lib.status_word(logits.device).data_ptr(), _lib.stream_ptr())
+    return out
+
+
+def adjust_logits_reference(logits, counts=None, count_rows=None, presence=None, frequency=None, repetition=None, bias=None,
+                            mask=None) -> torch.Tensor:
+    """Plain form of :func:`adjust_logits`, float32 (float64 for float64 logits). Entries out of range are left out."""
+    z = logits.to(torch.promote_types(logits.dtype, torch.float32)).clone()
+    R_, V = z.shape
+    rows = torch.arange(R_, device=z.device)
+    if counts is not None:
+        at = rows if count_rows is None else count_rows.long()
+        ok = (at >= 0) & (at < counts.shape[0])
+        c = torch.where(ok[:, None], counts[at.clamp(0, counts.shape[0] - 1), :V], 0) if counts.shape[0] else torch.zeros_like(z)
+        x = z if repetition is None else torch.where(z > 0, z / repetition[:, None], z * repetition[:, None])
+        less = (0 if presence is None else presence[:, None].to(z.dtype)) + \
+            (0 if frequency is None else frequency[:, None].to(z.dtype) * c.to(z.dtype))
+        z = torch.where(c > 0, x - less, z)
+    if bias is not None:
+        ptr, ids, values = bias
+        for r, (lo, hi) in enumerate(zip(ptr.tolist()[:-1], ptr.tolist()[1:])):
+            if 0 <= lo <= hi <= ids.numel():
+                i, v = ids[lo:hi].long(), values[lo:hi].to(z.dtype)
+                i, v = i[(i >= 0) & (i < V)], v[(i >= 0) & (i < V)]
+                add = torch.zeros_like(z[r]).index_put_((i,), v, accumulate=True)
+                z[r] = torch.where(add == -math.inf, add, torch.where(torch.zeros_like(add).index_fill_(0, i, 1) > 0, z[r] + add, z[r]))
+    if mask is not None:
+        bits, at = mask[0], rows if mask[1] is None else mask[1].long()
+        ok = (at >= 0) & (at < bits.shape[0])
+        if bits.shape[0]:
+            allow = (bits[at.clamp(0, bits.shape[0] - 1), :, None] >> torch.arange(32, dtype=torch.int32, device=z.device)) & 1
+            z = torch.where((allow.reshape(R_, -1)[:, :V] == 1) | ~ok[:, None], z, -math.inf)
+    return z
 
 
 def count_update(counts: torch.Tensor, tokens: torch.Tensor, row_slots: torch.Tensor | None = None) -> None:
