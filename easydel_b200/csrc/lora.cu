@@ -2,18 +2,18 @@
 //
 //   out[t, c] = y[t, c] + s * (x[t] A[i, p]^T) B[i, c]^T      i = index[t] (negative: no adapter), p the part of the output that c is in
 //
-// Mathematics of both kernels: two products with a small inner size r, one after the other, so what bounds them is the traffic of x, y
+// Mathematics: two products with a small inner size r, one after the other, so what bounds them is the traffic of x, y
 // and out (or, with a token or two per adapter, of A and B), not arithmetic: at r = 16 a byte of x or y brings 16 products.
-// That is why they issue warp-level `mma.sync` on registers filled straight from global memory and leave tensor memory alone: nothing is
-// reused often enough to be worth a trip through it.
+// That is why they use warp-level `mma.sync` and leave tensor memory alone.
 //
-// Operand layout: the contraction index of a product may be permuted as long as both operands agree, so a lane takes
-// eight neighbouring elements with one 16-byte load and calls them the four register pairs of two m16n8k16 products. The same holds for
-// output columns: a lane ends up with eight neighbouring columns. Weights that are needed across their rows (the backward pass) are loaded
-// along their rows and turned in registers (`movmatrix`).
+// Three forms. Few rows (or rows that no 16-byte access fits, or fp32): one launch, a cluster of CTAs per adapter and chunk of rows, which
+// keeps u = x A^T in shared memory. Many rows: a launch that reduces x to u and one that expands u onto y, each of which only
+// streams, with copies in flight that no register waits for. Gradients of A and B: a launch that contracts over rows.
+// Which rows go together is found by each CTA from the indexes of its rows, so a captured graph follows the indexes of the step and nothing
+// is sorted, counted or copied by the host.
 //
-// Precision: sums are fp32. The intermediate x A^T enters the second product as two bf16 parts (three where the result is fp32), so it
-// keeps 16 (24) bits; fp32 operands enter as three bf16 parts each.
+// Precision: sums are fp32. u enters the second product (and the gradients) as two bf16 parts, three where the result is fp32, so
+// it keeps 16 (24) bits; fp32 operands enter as three bf16 parts each.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -26,7 +26,6 @@ namespace {
 constexpr int LORA_THREADS = 256, LORA_WARPS = 8;
 constexpr int LORA_ROWS = 256;       // rows whose adapters a cluster looks through
 constexpr int LORA_SEGS = 8;
-constexpr int LORA_MAX_CHUNK = 64;
 
 // ---------------------------------------------------------------------------------------------------------- registers
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -111,6 +110,48 @@ __device__ __forceinline__ void load_pairs(const T* p, int valid, uint32_t (&q)[
   }
 }
 
+// Eight neighbouring values of a row as fp32; those from `ok` on are zero (WIDE: all or none).
+template <typename TY>
+__device__ __forceinline__ void unpack_row(const uint4 (&v)[sizeof(TY) / 2], float (&f)[8]) {
+  const uint32_t q[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[sizeof(TY) / 2 - 1].x, v[sizeof(TY) / 2 - 1].y, v[sizeof(TY) / 2 - 1].z, v[sizeof(TY) / 2 - 1].w};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if constexpr (sizeof(TY) == 2) f[e] = __uint_as_float(e & 1 ? q[e >> 1] & 0xffff0000u : q[e >> 1] << 16);
+    else f[e] = __uint_as_float(q[e]);
+  }
+}
+template <typename TY, bool WIDE>
+__device__ __forceinline__ void load_row(const TY* src, int ok, float (&f)[8]) {
+  if constexpr (WIDE) {
+    uint4 v[sizeof(TY) / 2];
+#pragma unroll
+    for (int q = 0; q < (int)sizeof(TY) / 2; ++q) v[q] = ok >= 8 ? reinterpret_cast<const uint4*>(src)[q] : make_uint4(0, 0, 0, 0);
+    unpack_row<TY>(v, f);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = e < ok ? (float)src[e] : 0.f;
+  }
+}
+template <typename TY, bool WIDE>
+__device__ __forceinline__ void store_row(TY* dst, int ok, const float (&f)[8]) {
+  if constexpr (WIDE) {
+    if (ok < 8) return;
+    if constexpr (sizeof(TY) == 2) {
+      *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+    } else {
+      *reinterpret_cast<float4*>(dst) = make_float4(f[0], f[1], f[2], f[3]);
+      *reinterpret_cast<float4*>(dst + 4) = make_float4(f[4], f[5], f[6], f[7]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < ok) {
+        if constexpr (sizeof(TY) == 2) dst[e] = __float2bfloat16_rn(f[e]);
+        else dst[e] = f[e];
+      }
+  }
+}
+
 // d += a b over the parts of both operands whose product is above the rounding of fp32 (part i has the bits from 8 i on).
 template <int PA, int PB>
 __device__ __forceinline__ void mma_parts(float (&d)[4], const uint32_t (&a)[PA][4], const uint32_t (&b)[PB][2]) {
@@ -122,11 +163,42 @@ __device__ __forceinline__ void mma_parts(float (&d)[4], const uint32_t (&a)[PA]
       if (o - i >= 0 && o - i < PB) mma_bf16(d, a[i][0], a[i][1], a[i][2], a[i][3], b[o - i][0], b[o - i][1]);
 }
 
-// ------------------------------------------------------------------------------------------------------------- apply
+// ---------------------------------------------------------------------------------------------------------- which rows
 struct LoraSeg {
   int c0, c1;       // columns of the matrix this side works on
-  int u0, ru;       // ranks: first column in u, count
+  int u0, ru;       // ranks: first one, count
 };
+
+// Weights of the second product for 32 output columns from n0 on and ranks kc .. kc + 15: [column tile][part][register]. A lane's columns are
+// the eight from n0 + 8 * (lane & 3) on, two of each tile. UP_T: they lie [ranks][columns].
+template <typename T, bool UP_T, bool WIDE>
+__device__ __forceinline__ void load_up(const T* wu, long long ld, int n0, const LoraSeg& seg, int kc, uint32_t (&wb)[4][PARTS<T>][2]) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  if constexpr (!UP_T) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = n0 + 8 * (g >> 1) + 2 * j + (g & 1);
+      uint32_t v[PARTS<T>][2];
+      load_pairs<T, 4, WIDE>(wu + (long long)n * ld + kc + 4 * t4, n < seg.c1 ? seg.ru - kc - 4 * t4 : 0, v);
+#pragma unroll
+      for (int s = 0; s < PARTS<T>; ++s) {
+        wb[j][s][0] = v[s][0];
+        wb[j][s][1] = v[s][1];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int rank = kc + 4 * (g >> 1) + (g & 1) + 2 * h, col = n0 + 8 * t4;
+      uint32_t v[PARTS<T>][4];
+      load_pairs<T, 8, WIDE>(wu + (long long)rank * ld + col, rank < seg.ru ? seg.c1 - col : 0, v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int s = 0; s < PARTS<T>; ++s) wb[j][s][h] = turn(v[s][j]);
+    }
+  }
+}
 
 struct LoraArgs {
   const void* x;
@@ -137,94 +209,123 @@ struct LoraArgs {
   long long ldx, ldy, ldo, down_adapter, ld_down, up_adapter, ld_up;
   const int* index;
   const float* scale;
-  float* u_out;
+  unsigned short* u;     // [parts of u][T][ucols] scaled, bf16; may be null in the one-launch form
   int* status;
   float scale_all;
-  int T, n, rtot, groups, down_segs, up_segs, copy;
+  int T, n, rtot, ucols, groups, look, down_segs, up_segs, copy;
   LoraSeg down_seg[LORA_SEGS], up_seg[LORA_SEGS];
 };
 
 __host__ __device__ constexpr int round16(int v) { return (v + 15) & ~15; }
 __host__ __device__ constexpr int u_stride(int cols) { return cols % 32 ? cols : cols + 16; }      // 8-byte reads without conflicts
 
-// One launch, no workspace. A cluster of CTAs takes up to CHUNK rows of one adapter: each CTA contracts its share of the columns of x
-// (spread over its warps), the CTAs add up their parts of u = x A^T through each other's shared memory (in rank order, so results
-// repeat), and each expands its share of the output's columns. Rows are grouped on the device: a cluster looks through
-// the indexes of its 256 rows, lists the (adapter, chunk) pairs among them and takes every `groups`-th pair, so that a captured graph
-// follows the indexes of the step and nothing is sorted, counted or copied by the host.
+// Rows of a block in the order of their adapters, cut into units of at most `chunk` rows of one adapter.
+struct RowUnits {
+  __align__(16) int idx[LORA_ROWS];
+  short place[LORA_ROWS];                                       // of an adapter's rows in `order`, at its first row
+  short order[LORA_ROWS], base[LORA_ROWS], rows[LORA_ROWS];     // row of a place; first place and rows of a unit
+  int ad[LORA_ROWS];
+  int scan[LORA_WARPS];
+  int total;
+};
+
+// Exclusive sum over the CTA's threads; `total` gets the sum of all.
+__device__ __forceinline__ int cta_scan(int v, int* scan, int& total) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int at = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, at, o);
+    if (lane >= o) at += t;
+  }
+  if (lane == 31) scan[w] = at;
+  __syncthreads();
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < LORA_WARPS; ++i) {
+    if (i < w) at += scan[i];
+    total += scan[i];
+  }
+  __syncthreads();
+  return at - v;
+}
+
+// All threads of the CTA. Rows without an adapter form units (adapter -1) where they have to be copied. Most blocks belong to one
+// request: those take no comparisons.
+__device__ __forceinline__ void find_units(RowUnits& u, const LoraArgs& a, long long row0, int rows, int chunk) {
+  const int tid = threadIdx.x, lane = tid & 31, w0 = tid & ~31;
+  int id = -2;
+  if (tid < rows) {
+    id = a.index ? a.index[row0 + tid] : 0;
+    if (id >= a.n && a.status) atomicCAS(a.status, 0, EDL_BAD_INDEX);
+    if (id < 0 || id >= a.n) id = -1;
+  }
+  u.idx[tid] = id;
+  __syncthreads();
+  int before = tid, count = rows, first_row = 0;
+  if (!__syncthreads_and(tid >= rows || id == u.idx[0])) {
+    before = count = 0;
+    for (int j = 0; j < rows; j += 4) {      // indexes behind the last row are -2
+      if (j == w0) before = count;
+      if (!count) first_row = j;
+      const int4 v = *reinterpret_cast<const int4*>(u.idx + j);
+      count += (v.x == id) + (v.y == id) + (v.z == id) + (v.w == id);
+    }
+    while (tid < rows && u.idx[first_row] != id) ++first_row;
+    before += __popc(__match_any_sync(0xffffffffu, id) & ((1u << lane) - 1));
+  }
+  const bool taken = tid < rows && (id >= 0 || a.copy), first = taken && before == 0;
+  int all;
+  const int place = cta_scan(first ? count : 0, u.scan, all), unit = cta_scan(first ? (count + chunk - 1) / chunk : 0, u.scan, all);
+  if (first) {
+    u.place[tid] = (short)place;
+    for (int q = 0; q * chunk < count; ++q) {
+      u.base[unit + q] = (short)(place + q * chunk);
+      u.rows[unit + q] = (short)min(chunk, count - q * chunk);
+      u.ad[unit + q] = id;
+    }
+  }
+  if (tid == 0) u.total = all;
+  __syncthreads();
+  if (taken) u.order[u.place[first_row] + before] = (short)tid;
+  __syncthreads();
+}
+
+// --------------------------------------------------------------------------------------------------- one launch, few rows
+// A cluster of CTAs takes up to 16 rows of one adapter: each CTA contracts its share of the columns of x (spread over its warps), the
+// CTAs add up their parts of u through each other's shared memory (in rank order, so results repeat), and each
+// expands its share of the output's columns. Every `groups`-th unit of a block of 256 rows belongs to a cluster.
+// Operands come straight from global memory: the contraction index of a product may be permuted as long as both operands agree, so a lane
+// takes eight neighbouring elements with one 16-byte load and calls them the four register pairs of two m16n8k16 products; the same
+// holds for output columns. Weights that are needed across their rows (the backward pass) are turned in registers (`movmatrix`).
 // DOWN_T: the weights of the first product lie [columns][ranks] (B in the backward pass) and those of the second [ranks][columns].
-template <typename T, typename TY, int RT, int NT, bool DOWN_T, bool WIDE>
-__global__ void __launch_bounds__(LORA_THREADS, RT == 1 ? 2 : 1) lora_kernel(const LoraArgs a, int tgroups) {
+template <typename T, typename TY, int RT, bool DOWN_T, bool WIDE>
+__global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const __grid_constant__ LoraArgs a) {
+  constexpr int NT = 2, CHUNK = 8 * NT;
   constexpr int P = PARTS<T>;                           // parts of x and of the weights
   constexpr int S = sizeof(TY) == 4 ? 3 : 2;            // parts of u
   constexpr int RSTRIDE = 16 * RT + 4;
-  __shared__ __align__(16) int s_idx[LORA_ROWS];
-  __shared__ short s_count[LORA_ROWS], s_first[LORA_ROWS], s_chunk[LORA_ROWS];
-  __shared__ int s_rows[LORA_MAX_CHUNK];
-  __shared__ int s_scan[LORA_WARPS];
+  __shared__ RowUnits units;
   extern __shared__ __align__(16) uint8_t dyn[];
 
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), c = cluster.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t4 = lane & 3;
-  const int cid = blockIdx.x / C, row0 = (cid / a.groups) * LORA_ROWS;
-  const int chunk = 8 * NT * tgroups, kwarps = LORA_WARPS / tgroups;
-  const int r16 = a.up_segs ? round16(a.up_seg[0].ru) : 0, ucols = a.up_segs * r16, ustride = u_stride(ucols);
+  const int cid = blockIdx.x / C;
+  const long long row0 = (long long)(cid / a.groups) * LORA_ROWS;
+  const int r16 = a.up_segs ? round16(a.up_seg[0].ru) : 0, ucols = a.ucols, ustride = u_stride(ucols);
   const int pstride = a.rtot;
-  float* part = reinterpret_cast<float*>(dyn);                                      // [chunk][rtot]: this CTA's share of u
-  uint8_t* second = dyn + ((chunk * pstride * 4 + 15) & ~15);
-  float* red = reinterpret_cast<float*>(second);                                    // [kwarps][chunk][RSTRIDE], then
-  unsigned short* su = reinterpret_cast<unsigned short*>(second);                   // [S][chunk][ustride]: scaled u in parts
+  float* part = reinterpret_cast<float*>(dyn);                                      // [CHUNK][rtot]: this CTA's share of u
+  uint8_t* second = dyn + ((CHUNK * pstride * 4 + 15) & ~15);
+  float* red = reinterpret_cast<float*>(second);                                    // [warps][CHUNK][RSTRIDE], then
+  unsigned short* su = reinterpret_cast<unsigned short*>(second);                   // [S][CHUNK][ustride]: scaled u in parts
 
-  // ---- which rows go together
-  const int rows = min(LORA_ROWS, a.T - row0);
-  int id = -2, before = 0, count = 0;
-  if (tid < rows) {
-    id = a.index ? a.index[row0 + tid] : 0;
-    if (id >= a.n && a.status && c == 0) atomicCAS(a.status, 0, EDL_BAD_INDEX);
-    if (id < 0 || id >= a.n) id = -1;
-  }
-  s_idx[tid] = id;
-  __syncthreads();
-  if (!a.index) {
-    before = tid;
-    count = rows;
-  } else {
-    for (int j = 0; j < rows; j += 4) {
-      const int4 v = *reinterpret_cast<const int4*>(s_idx + j);      // indexes behind the last row are -2
-      const int e0 = v.x == id, e1 = v.y == id, e2 = v.z == id, e3 = v.w == id;
-      count += e0 + e1 + e2 + e3;
-      before += (j < tid && e0) + (j + 1 < tid && e1) + (j + 2 < tid && e2) + (j + 3 < tid && e3);
-    }
-  }
-  int units = 0;
-  if (tid < rows && before == 0 && (id >= 0 || a.copy)) units = (count + chunk - 1) / chunk;
-  int at = units;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, at, o);
-    if (lane >= o) at += v;
-  }
-  if (lane == 31) s_scan[w] = at;
-  __syncthreads();
-  int total = 0;
-  for (int i = 0; i < LORA_WARPS; ++i) {
-    if (i < w) at += s_scan[i];
-    total += s_scan[i];
-  }
-  for (int q = 0; q < units; ++q) {
-    s_first[at - units + q] = (short)tid;
-    s_chunk[at - units + q] = (short)q;
-  }
-  s_count[tid] = (short)count;
-  __syncthreads();
+  find_units(units, a, row0, (int)min((long long)LORA_ROWS, a.T - row0), CHUNK);
 
-  const int tg = w % tgroups, kw = w / tgroups;
   bool pending = false;
-  for (int unit = cid % a.groups; unit < total; unit += a.groups) {
-    const int first = s_first[unit], q0 = s_chunk[unit] * chunk, ad = s_idx[first], m = min(chunk, s_count[first] - q0);
-    if (id == ad && before >= q0 && before < q0 + chunk) s_rows[before - q0] = row0 + tid;
-    __syncthreads();
+  for (int unit = cid % a.groups; unit < units.total; unit += a.groups) {
+    const int ad = units.ad[unit], m = units.rows[unit];
+    const short* order = units.order + units.base[unit];
 
     if (ad >= 0) {
       // ---- this CTA's share of u: ranks are the rows of the product, tokens its columns
@@ -232,8 +333,8 @@ __global__ void __launch_bounds__(LORA_THREADS, RT == 1 ? 2 : 1) lora_kernel(con
       const T* xr[NT];
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        const int tok = (tg * NT + i) * 8 + g;
-        xr[i] = tok < m ? reinterpret_cast<const T*>(a.x) + (long long)s_rows[tok] * a.ldx : nullptr;
+        const int tok = i * 8 + g;
+        xr[i] = tok < m ? reinterpret_cast<const T*>(a.x) + (row0 + order[tok]) * a.ldx : nullptr;
       }
       if (pending) {
         asm volatile("barrier.cluster.wait.acquire;" ::: "memory");      // every CTA has read the last unit's parts
@@ -249,8 +350,8 @@ __global__ void __launch_bounds__(LORA_THREADS, RT == 1 ? 2 : 1) lora_kernel(con
             for (int j = 0; j < NT; ++j)
 #pragma unroll
               for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
-#pragma unroll(P == 1 ? 2 : 1)
-          for (int k = seg.c0 + 32 * (c * kwarps + kw); k < seg.c1; k += 32 * C * kwarps) {
+#pragma unroll(P == 1 && RT <= 2 ? 2 : 1)
+          for (int k = seg.c0 + 32 * (c * LORA_WARPS + w); k < seg.c1; k += 32 * C * LORA_WARPS) {
             uint32_t wa[RT][2][P][4];      // [rank tile][k16][part][register]
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
@@ -305,9 +406,9 @@ __global__ void __launch_bounds__(LORA_THREADS, RT == 1 ? 2 : 1) lora_kernel(con
           for (int i = 0; i < RT; ++i)
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-              const int tok = (tg * NT + j) * 8 + 2 * t4;
+              const int tok = j * 8 + 2 * t4;
               const int lo = 16 * i + (DOWN_T ? 4 * (g >> 1) + (g & 1) : g), hi = lo + (DOWN_T ? 2 : 8);
-              float* dst = red + (kw * chunk + tok) * RSTRIDE;
+              float* dst = red + (w * CHUNK + tok) * RSTRIDE;
               dst[lo] = acc[i][j][0];
               dst[RSTRIDE + lo] = acc[i][j][1];
               dst[hi] = acc[i][j][2];
@@ -318,7 +419,8 @@ __global__ void __launch_bounds__(LORA_THREADS, RT == 1 ? 2 : 1) lora_kernel(con
             const int tok = e / (16 * RT), rank = e % (16 * RT);
             if (r0 + rank >= seg.ru) continue;
             float sum = 0.f;
-            for (int k = 0; k < kwarps; ++k) sum += red[(k * chunk + tok) * RSTRIDE + rank];
+#pragma unroll
+            for (int k = 0; k < LORA_WARPS; ++k) sum += red[(k * CHUNK + tok) * RSTRIDE + rank];
             part[tok * pstride + seg.u0 + r0 + rank] = sum;
           }
           __syncthreads();
@@ -327,25 +429,21 @@ __global__ void __launch_bounds__(LORA_THREADS, RT == 1 ? 2 : 1) lora_kernel(con
       // ---- u of all CTAs, scaled, as bf16 parts
       cluster_sync_all();
       const float s = a.scale ? a.scale[ad] : a.scale_all;
-      for (int e = tid; e < chunk * ucols; e += LORA_THREADS) {
-        const int tok = e / ucols, col = e - tok * ucols, p = col / r16, rank = col - p * r16;
+      for (int e = tid; e < CHUNK * ucols; e += LORA_THREADS) {
+        const int tok = e / ucols, col = e - tok * ucols;
+        const int p = a.up_segs > 1 ? col / r16 : 0, rank = col - p * r16;
         float v = 0.f;
         if (tok < m && rank < a.up_seg[p].ru) {
           const int pos = tok * pstride + a.up_seg[p].u0 + rank;
           for (int k = 0; k < C; ++k) v += cluster.map_shared_rank(part, k)[pos];
           v *= s;
-          if (a.u_out && c == 0) a.u_out[(long long)s_rows[tok] * a.rtot + a.up_seg[p].u0 + rank] = v;
         }
         uint32_t parts[S];
         split<S>(v, parts);
 #pragma unroll
-        for (int k = 0; k < S; ++k) su[(k * chunk + tok) * ustride + col] = (unsigned short)parts[k];
-      }
-      if (!a.up_segs && c == 0) {      // only u is asked for
-        for (int e = tid; e < m * a.rtot; e += LORA_THREADS) {
-          float v = 0.f;
-          for (int k = 0; k < C; ++k) v += cluster.map_shared_rank(part, k)[e];
-          a.u_out[(long long)s_rows[e / a.rtot] * a.rtot + e % a.rtot] = v * s;
+        for (int k = 0; k < S; ++k) {
+          su[(k * CHUNK + tok) * ustride + col] = (unsigned short)parts[k];
+          if (a.u && c == 0 && tok < m) a.u[((long long)k * a.T + row0 + order[tok]) * ucols + col] = (unsigned short)parts[k];
         }
       }
       asm volatile("barrier.cluster.arrive.release;" ::: "memory");
@@ -355,8 +453,7 @@ __global__ void __launch_bounds__(LORA_THREADS, RT == 1 ? 2 : 1) lora_kernel(con
 
     // ---- out = y + u B^T over this CTA's share of the columns, 32 per warp and turn
     const T* wu = reinterpret_cast<const T*>(a.up) + (long long)(ad < 0 ? 0 : ad) * a.up_adapter;
-    const int kcs = r16 / 16;
-    for (int grp = c * LORA_WARPS + w;; grp += C * LORA_WARPS) {
+    for (int grp = c * LORA_WARPS + w; a.out; grp += C * LORA_WARPS) {
       int p = 0, gi = grp;
       while (p < a.up_segs) {
         const int have = (a.up_seg[p].c1 - a.up_seg[p].c0 + 31) / 32;
@@ -367,142 +464,319 @@ __global__ void __launch_bounds__(LORA_THREADS, RT == 1 ? 2 : 1) lora_kernel(con
       if (p >= a.up_segs) break;
       const LoraSeg seg = a.up_seg[p];
       const int n0 = seg.c0 + 32 * gi, col = n0 + 8 * t4, ok = seg.c1 - col;      // this lane's eight columns
-      uint32_t wb[RT][4][P][2];                                                 // [k16][column tile][part][register]
-      for (int tt = 0; tt < m; tt += 16) {
-        float acc[4][4];
-        float yv[2][8];
-        int row[2];
+      float yv[2][8];
+      long long row[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int tok = tt + 8 * h + g;
-          row[h] = tok < m ? s_rows[tok] : -1;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) yv[h][e] = 0.f;
-          if (a.y && row[h] >= 0) {
-            const TY* src = reinterpret_cast<const TY*>(a.y) + (long long)row[h] * a.ldy + col;
-            if constexpr (WIDE) {
-              if (ok >= 8) {
-                if constexpr (sizeof(TY) == 2) {
-                  const uint4 v = *reinterpret_cast<const uint4*>(src);
-                  const uint32_t q[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) {
-                    const float2 f = unpack_bf16x2(q[e]);
-                    yv[h][2 * e] = f.x;
-                    yv[h][2 * e + 1] = f.y;
-                  }
-                } else {
-                  const float4 v0 = *reinterpret_cast<const float4*>(src), v1 = *reinterpret_cast<const float4*>(src + 4);
-                  yv[h][0] = v0.x; yv[h][1] = v0.y; yv[h][2] = v0.z; yv[h][3] = v0.w;
-                  yv[h][4] = v1.x; yv[h][5] = v1.y; yv[h][6] = v1.z; yv[h][7] = v1.w;
-                }
-              }
-            } else {
-#pragma unroll
-              for (int e = 0; e < 8; ++e)
-                if (e < ok) yv[h][e] = (float)src[e];
-            }
-          }
-        }
-        if (ad >= 0) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
-          for (int k0 = 0; k0 < kcs; k0 += RT) {
-            if (tt == 0 || kcs > RT) {      // up to RT steps of ranks stay in registers for all rows
-#pragma unroll
-              for (int i = 0; i < RT; ++i) {
-                const int kc = 16 * (k0 + i);
-                if constexpr (!DOWN_T) {
-#pragma unroll
-                  for (int j = 0; j < 4; ++j) {
-                    const int n = n0 + 8 * (g >> 1) + 2 * j + (g & 1);
-                    uint32_t v[P][2];
-                    load_pairs<T, 4, WIDE>(wu + (long long)n * a.ld_up + kc + 4 * t4, n < seg.c1 ? seg.ru - kc - 4 * t4 : 0, v);
-#pragma unroll
-                    for (int s = 0; s < P; ++s) {
-                      wb[i][j][s][0] = v[s][0];
-                      wb[i][j][s][1] = v[s][1];
-                    }
-                  }
-                } else {
-#pragma unroll
-                  for (int h = 0; h < 2; ++h) {
-                    const int rank = kc + 4 * (g >> 1) + (g & 1) + 2 * h;
-                    uint32_t v[P][4];
-                    load_pairs<T, 8, WIDE>(wu + (long long)rank * a.ld_up + col, rank < seg.ru ? ok : 0, v);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-#pragma unroll
-                      for (int s = 0; s < P; ++s) wb[i][j][s][h] = turn(v[s][j]);
-                  }
-                }
-              }
-            }
-#pragma unroll
-            for (int i = 0; i < RT; ++i) {
-              if (k0 + i >= kcs) break;
-              uint32_t ua[S][4];
-#pragma unroll
-              for (int s = 0; s < S; ++s)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  // rows behind the chunk (chunks of 8) repeat its first ones: their products go nowhere
-                  const int tok = (tt + 8 * h + g) & (chunk - 1);
-                  const uint2 v = *reinterpret_cast<const uint2*>(su + (s * chunk + tok) * ustride + p * r16 + 16 * (k0 + i) + 4 * t4);
-                  ua[s][h] = v.x;
-                  ua[s][2 + h] = v.y;
-                }
-#pragma unroll
-              for (int j = 0; j < 4; ++j) mma_parts<S, P>(acc[j], ua, wb[i][j]);
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            yv[0][2 * j] += acc[j][0];
-            yv[0][2 * j + 1] += acc[j][1];
-            yv[1][2 * j] += acc[j][2];
-            yv[1][2 * j + 1] += acc[j][3];
-          }
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (row[h] < 0) continue;
-          TY* dst = reinterpret_cast<TY*>(a.out) + (long long)row[h] * a.ldo + col;
-          if constexpr (WIDE) {
-            if (ok >= 8) {
-              if constexpr (sizeof(TY) == 2) {
-                *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(yv[h][0], yv[h][1]), pack_bf16x2(yv[h][2], yv[h][3]),
-                                                            pack_bf16x2(yv[h][4], yv[h][5]), pack_bf16x2(yv[h][6], yv[h][7]));
-              } else {
-                *reinterpret_cast<float4*>(dst) = make_float4(yv[h][0], yv[h][1], yv[h][2], yv[h][3]);
-                *reinterpret_cast<float4*>(dst + 4) = make_float4(yv[h][4], yv[h][5], yv[h][6], yv[h][7]);
-              }
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (e < ok) {
-                if constexpr (sizeof(TY) == 2) dst[e] = __float2bfloat16_rn(yv[h][e]);
-                else dst[e] = yv[h][e];
-              }
-          }
-        }
+      for (int h = 0; h < 2; ++h) {
+        row[h] = 8 * h + g < m ? row0 + order[8 * h + g] : -1;
+        load_row<TY, WIDE>(reinterpret_cast<const TY*>(a.y) + row[h] * a.ldy + col, a.y && row[h] >= 0 ? ok : 0, yv[h]);
       }
+      if (ad >= 0) {
+        float acc[4][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
+        for (int kc = 0; kc < r16; kc += 16) {
+          uint32_t wb[4][P][2], ua[S][4];
+          load_up<T, DOWN_T, WIDE>(wu, a.ld_up, n0, seg, kc, wb);
+#pragma unroll
+          for (int s = 0; s < S; ++s)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint2 v = *reinterpret_cast<const uint2*>(su + (s * CHUNK + 8 * h + g) * ustride + p * r16 + kc + 4 * t4);
+              ua[s][h] = v.x;
+              ua[s][2 + h] = v.y;
+            }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mma_parts<S, P>(acc[j], ua, wb[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) yv[e >> 1][2 * j + (e & 1)] += acc[j][e];
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        store_row<TY, WIDE>(reinterpret_cast<TY*>(a.out) + row[h] * a.ldo + col, row[h] >= 0 ? ok : 0, yv[h]);
     }
-    __syncthreads();      // rows and parts of u make way for the next unit
+    __syncthreads();      // parts of u make way for the next unit
   }
   if (pending) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");      // no CTA leaves while its parts are read
 }
 
-template <typename T, typename TY, int RT, int NT, bool DOWN_T, bool WIDE>
-int launch_lora(const LoraArgs& a, int cluster, int tgroups, int smem, cudaStream_t stream) {
-  auto* k = lora_kernel<T, TY, RT, NT, DOWN_T, WIDE>;
-  if (smem > 48 * 1024 && check_cuda(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "lora shared memory")) return -1;
+// --------------------------------------------------------------------------------------------------- many rows: x to u
+constexpr int DOWN_ROWS = 64, DOWN_K = 64, DOWN_XROW = DOWN_K * 2 + 16;      // 16 bytes behind each row: no conflicts in `ldmatrix`
+template <int RT> constexpr int DOWN_STAGES = RT == 1 ? 6 : 5;
+template <int RT, bool DOWN_T> constexpr int DOWN_WROW = DOWN_T ? 32 * RT + 16 : DOWN_XROW;
+template <int RT, bool DOWN_T>
+constexpr int DOWN_STAGE = DOWN_ROWS * DOWN_XROW + (DOWN_T ? DOWN_K : 16 * RT) * DOWN_WROW<RT, DOWN_T>;
+template <int RT, bool DOWN_T> constexpr int DOWN_SMEM = DOWN_STAGES<RT> * DOWN_STAGE<RT, DOWN_T> + DOWN_ROWS * 16 * RT * 4;
+
+template <int BYTES>
+__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool ok) {      // zeros where not ok
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(ok ? 8 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+template <bool TRANS>
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  if constexpr (TRANS)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+// u of 64 rows of one adapter: columns in steps of 64 through a ring of shared-memory stages (`cp.async`, rows gathered as they are
+// copied), cut over the CTAs of a cluster where there are few rows. Warps 0-3 take 16 rows each and the first half of a step's columns,
+// warps 4-7 the second. Sums of the halves and of the CTAs are added in a fixed order.
+template <int RT, bool DOWN_T>
+__global__ void __launch_bounds__(LORA_THREADS, 2) lora_down_kernel(const __grid_constant__ LoraArgs a, int parts) {
+  constexpr int STAGES = DOWN_STAGES<RT>, STAGE = DOWN_STAGE<RT, DOWN_T>, WROW = DOWN_WROW<RT, DOWN_T>, RSTRIDE = 16 * RT + 4;
+  __shared__ RowUnits units;
+  extern __shared__ __align__(16) uint8_t dyn[];
+  float* part = reinterpret_cast<float*>(dyn + STAGES * STAGE);      // [64][16 RT]
+  float* red = reinterpret_cast<float*>(dyn);                        // [64][RSTRIDE], where the stages were
+  const uint32_t ring = smem_u32(dyn);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = cluster.num_blocks(), c = cluster.block_rank();
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t4 = lane & 3, tg = w & 3, kh = w >> 2;
+  const int cid = blockIdx.x / C;
+  const long long row0 = (long long)(cid / a.groups) * LORA_ROWS;
+  const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x);
+  find_units(units, a, row0, (int)min((long long)LORA_ROWS, a.T - row0), DOWN_ROWS);
+  bool pending = false;
+  for (int unit = cid % a.groups; unit < units.total; unit += a.groups) {
+    const int ad = units.ad[unit], m = units.rows[unit];
+    if (ad < 0) continue;
+    const short* order = units.order + units.base[unit];
+    const __nv_bfloat16* wd = reinterpret_cast<const __nv_bfloat16*>(a.down) + (long long)ad * a.down_adapter;
+    const float s = a.scale ? a.scale[ad] : a.scale_all;
+    // a thread copies the same 16 bytes of two rows in every step
+    const __nv_bfloat16* xr[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int tok = (tid >> 3) + 32 * i;
+      xr[i] = tok < m ? x + (row0 + order[tok]) * a.ldx + 8 * (tid & 7) : nullptr;
+    }
+    for (int sg = 0; sg < a.down_segs; ++sg) {
+      const LoraSeg seg = a.down_seg[sg];
+      const int all = (seg.c1 - seg.c0 + DOWN_K - 1) / DOWN_K, per = (all + C - 1) / C;
+      const int k0 = seg.c0 + min(all, c * per) * DOWN_K, steps = min(all, (c + 1) * per) - min(all, c * per);
+      for (int r0 = 0; r0 < seg.ru; r0 += 16 * RT) {
+        auto fill = [&](int step) {
+          const uint32_t dst = ring + (step % STAGES) * STAGE;
+          const int k = k0 + step * DOWN_K;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            cp_async<16>(dst + ((tid >> 3) + 32 * i) * DOWN_XROW + 16 * (tid & 7), xr[i] ? xr[i] + k : x, xr[i] && k + 8 * (tid & 7) < seg.c1);
+          const uint32_t wdst = dst + DOWN_ROWS * DOWN_XROW;
+          if constexpr (!DOWN_T) {
+            for (int i = tid; i < 16 * RT * 8; i += LORA_THREADS) {
+              const int rank = i >> 3, col = k + 8 * (i & 7);
+              const bool ok = r0 + rank < seg.ru && col < seg.c1;
+              cp_async<16>(wdst + rank * WROW + 16 * (i & 7), ok ? wd + (long long)(seg.u0 + r0 + rank) * a.ld_down + col : wd, ok);
+            }
+          } else {
+            for (int i = tid; i < DOWN_K * 4 * RT; i += LORA_THREADS) {
+              const int kk = i / (4 * RT), rank = 4 * (i % (4 * RT));
+              const bool ok = k + kk < seg.c1 && r0 + rank < seg.ru;
+              cp_async<8>(wdst + kk * WROW + 2 * rank, ok ? wd + (long long)(k + kk) * a.ld_down + r0 + rank : wd, ok);
+            }
+          }
+        };
+        float acc[RT][2][4];
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
+#pragma unroll
+        for (int st = 0; st < STAGES - 1; ++st) {
+          if (st < steps) fill(st);
+          cp_commit();
+        }
+        for (int step = 0; step < steps; ++step) {
+          cp_wait<STAGES - 2>();
+          __syncthreads();      // the step's copies are there, and nobody reads the stage that is filled next
+          if (step + STAGES - 1 < steps) fill(step + STAGES - 1);
+          cp_commit();
+          const uint32_t src = ring + (step % STAGES) * STAGE, wsrc = src + DOWN_ROWS * DOWN_XROW;
+          uint32_t b[2][4];      // [8 rows][columns 0-7, 8-15, 16-23, 24-31 of this half]
+#pragma unroll
+          for (int j = 0; j < 2; ++j) ldmatrix4<false>(b[j], src + (tg * 16 + 8 * j + (lane & 7)) * DOWN_XROW + kh * 64 + 16 * (lane >> 3));
+#pragma unroll
+          for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              uint32_t wa[4];
+              const int lo = (lane >> 3) & 1, hi = lane >> 4;
+              if constexpr (!DOWN_T) ldmatrix4<false>(wa, wsrc + (16 * i + 8 * lo + (lane & 7)) * WROW + kh * 64 + 32 * q + 16 * hi);
+              else ldmatrix4<true>(wa, wsrc + (kh * 32 + 16 * q + 8 * hi + (lane & 7)) * WROW + 32 * i + 16 * lo);
+#pragma unroll
+              for (int j = 0; j < 2; ++j) mma_bf16(acc[i][j], wa[0], wa[1], wa[2], wa[3], b[j][2 * q], b[j][2 * q + 1]);
+            }
+        }
+        cp_wait<0>();
+        __syncthreads();
+        auto each = [&](auto f) {
+#pragma unroll
+          for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) f(16 * tg + 8 * j + 2 * t4 + (e & 1), 16 * i + g + 8 * (e >> 1), acc[i][j][e]);
+        };
+        if (kh == 1) each([&](int tok, int rank, float v) { red[tok * RSTRIDE + rank] = v; });
+        if (pending) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");      // every CTA has read the last parts
+        __syncthreads();
+        if (kh == 0) each([&](int tok, int rank, float v) { part[tok * 16 * RT + rank] = v + red[tok * RSTRIDE + rank]; });
+        cluster_sync_all();
+        // ---- each CTA adds up and writes its share
+        const int r16 = round16(a.up_seg[0].ru), lo = seg.u0 + r0, hi = min(lo + 16 * RT, seg.u0 + seg.ru);
+        for (int e = c * LORA_THREADS + tid; e < m * a.ucols; e += C * LORA_THREADS) {
+          const int tok = e / a.ucols, col = e - tok * a.ucols;
+          const int p = a.up_segs > 1 ? col / r16 : 0, j = col - p * r16, rank = a.up_seg[p].u0 + j;
+          const bool pad = j >= a.up_seg[p].ru;
+          if (pad ? sg > 0 || r0 > 0 : rank < lo || rank >= hi) continue;
+          float v = 0.f;
+          if (!pad) {
+            for (int k = 0; k < C; ++k) v += cluster.map_shared_rank(part, k)[tok * 16 * RT + rank - lo];
+            v *= s;
+          }
+          unsigned short* dst = a.u + (row0 + order[tok]) * a.ucols + col;
+          if (parts == 2) {
+            uint32_t q[2];
+            split<2>(v, q);
+            dst[0] = (unsigned short)q[0];
+            dst[(long long)a.T * a.ucols] = (unsigned short)q[1];
+          } else {
+            uint32_t q[3];
+            split<3>(v, q);
+#pragma unroll
+            for (int k = 0; k < 3; ++k) dst[(long long)k * a.T * a.ucols] = (unsigned short)q[k];
+          }
+        }
+        asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+        pending = true;
+        __syncthreads();
+      }
+    }
+  }
+  if (pending) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+
+// --------------------------------------------------------------------------------------------------- many rows: u onto y
+// A CTA takes 256 columns (32 per warp) of up to `look` rows. The weights of a warp's columns stay in registers for all rows of an
+// adapter (up to 16 KC ranks); what remains per 16 rows is to read u (from L2), y, and to write out. The next rows' y is asked for before
+// this one's is used.
+template <typename TY, int KC, bool UP_T>
+__global__ void __launch_bounds__(LORA_THREADS, KC == 1 ? 3 : 2) lora_up_kernel(const __grid_constant__ LoraArgs a) {
+  constexpr int S = sizeof(TY) == 4 ? 3 : 2;
+  __shared__ RowUnits units;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t4 = lane & 3;
+  const long long row0 = (long long)(blockIdx.x / a.groups) * a.look;
+  find_units(units, a, row0, (int)min((long long)a.look, a.T - row0), 16);
+  int p = 0, gi = (blockIdx.x % a.groups) * LORA_WARPS + w;
+  while (p < a.up_segs) {
+    const int have = (a.up_seg[p].c1 - a.up_seg[p].c0 + 31) / 32;
+    if (gi < have) break;
+    gi -= have;
+    ++p;
+  }
+  if (p >= a.up_segs) return;
+  const LoraSeg seg = a.up_seg[p];
+  const int n0 = seg.c0 + 32 * gi, col = n0 + 8 * t4, r16 = round16(seg.ru);
+  const bool ok = col < seg.c1;
+  const int total = units.total;
+  const TY* y = reinterpret_cast<const TY*>(a.y) + col;
+  TY* out = reinterpret_cast<TY*>(a.out) + col;
+  const unsigned short* us = a.u + p * r16 + 4 * t4;
+  constexpr int W = sizeof(TY) / 2;      // 16-byte pieces of eight values
+  uint4 next[2][W];
+  auto row_of = [&](int unit, int h) -> long long { return 8 * h + g < units.rows[unit] ? row0 + units.order[units.base[unit] + 8 * h + g] : -1; };
+  auto ask = [&](int unit) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const long long row = row_of(unit, h);
+#pragma unroll
+      for (int q = 0; q < W; ++q) {
+        next[h][q] = make_uint4(0, 0, 0, 0);
+        if (a.y && ok && row >= 0) next[h][q] = reinterpret_cast<const uint4*>(y + row * a.ldy)[q];
+      }
+    }
+  };
+  if (total) ask(0);
+  int have = -1;
+  uint32_t wb[KC][4][1][2];
+  for (int unit = 0; unit < total; ++unit) {
+    const int ad = units.ad[unit];
+    long long row[2];
+    float yv[2][8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      row[h] = row_of(unit, h);
+      unpack_row<TY>(next[h], yv[h]);
+    }
+    if (ad >= 0) {
+      uint32_t ua[KC][S][4];
+      auto ask_u = [&](int kc0) {
+#pragma unroll
+        for (int i = 0; i < KC; ++i)
+#pragma unroll
+          for (int s = 0; s < S; ++s)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint2 v = make_uint2(0, 0);
+              if (row[h] >= 0 && kc0 + 16 * i < r16)
+                v = *reinterpret_cast<const uint2*>(us + ((long long)s * a.T + row[h]) * a.ucols + kc0 + 16 * i);
+              ua[i][s][h] = v.x;
+              ua[i][s][2 + h] = v.y;
+            }
+      };
+      ask_u(0);
+      if (unit + 1 < total) ask(unit + 1);
+      const __nv_bfloat16* wu = reinterpret_cast<const __nv_bfloat16*>(a.up) + (long long)ad * a.up_adapter;
+      float acc[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
+      for (int kc0 = 0; kc0 < r16; kc0 += 16 * KC) {
+        if (ad != have || r16 > 16 * KC) {
+#pragma unroll
+          for (int i = 0; i < KC; ++i) load_up<__nv_bfloat16, UP_T, true>(wu, a.ld_up, n0, seg, kc0 + 16 * i, wb[i]);
+          have = ad;
+        }
+        if (kc0) ask_u(kc0);
+#pragma unroll
+        for (int i = 0; i < KC; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mma_parts<S, 1>(acc[j], ua[i], wb[i][j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) yv[e >> 1][2 * j + (e & 1)] += acc[j][e];
+    } else if (unit + 1 < total) {
+      ask(unit + 1);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      store_row<TY, true>(out + row[h] * a.ldo, ok && row[h] >= 0 ? 8 : 0, yv[h]);
+  }
+}
+
+template <typename... E, typename... A>
+int launch_cluster(void (*k)(E...), dim3 grid, int cluster, int smem, cudaStream_t stream, const char* what, A... args) {
+  if (smem > 48 * 1024 && check_cuda(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), what)) return -1;
   cudaLaunchConfig_t cfg{};
-  const long long blocks = (a.T + LORA_ROWS - 1) / LORA_ROWS;
-  cfg.gridDim = dim3((unsigned)(blocks * a.groups * cluster));
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(LORA_THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -513,96 +787,122 @@ int launch_lora(const LoraArgs& a, int cluster, int tgroups, int smem, cudaStrea
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, k, a, tgroups), "lora launch");
+  return check_cuda(cudaLaunchKernelEx(&cfg, k, args...), what);
 }
 
 // ------------------------------------------------------------------------------------------------------------- gradients
 struct GradJob {
-  const void* z;         // [T, *] rows: x for dA, dy for dB
-  const float* p;        // [T, rtot]: g for dA, scaled u for dB
+  const void* z;               // [T, *] rows: x for dA, dy for dB
+  const unsigned short* p;     // parts of g for dA, of u for dB: [parts][T][pcols]
   void* out;
   long long ldz, out_adapter, ld_out;
-  int c0, c1, u0, ru;    // columns of z, ranks
-  int tiles;             // column tiles x rank passes
-  int across;            // out lies [column][rank] (dB) instead of [rank][column] (dA)
+  int c0, c1, u0, ru;          // columns of z, ranks
+  int pcols, p0;               // columns of p, the first one of these ranks
+  int tiles;                   // column tiles x rank passes
+  int across;                  // out lies [column][rank] (dB) instead of [rank][column] (dA)
 };
 
 struct GradArgs {
   const int* index;
-  int T, n, rtot, jobs, out_f32, accumulate;
+  int T, n, jobs, out_f32, accumulate;
   GradJob job[LORA_SEGS + 1];
 };
 
-constexpr int GRAD_COLS = 256, GRAD_LIST = 1024;
+constexpr int GRAD_COLS = 256, GRAD_LIST = 1024, GRAD_STRIDE = GRAD_COLS + 4;
 
-// out[rank, col] (+)= sum over the adapter's rows t of p[t, rank] z[t, col]: rank x 256 columns per cluster, the rows cut over its
-// CTAs. z is read once, along its rows, and turned in registers, as is p. A CTA's two row halves (warps 0-3, 4-7) are
-// added through shared memory, the CTAs' sums through each other's, both in a fixed order; each CTA writes its share of the tile.
-template <typename T, int S, int RT, bool WIDE>
-__global__ void __launch_bounds__(LORA_THREADS, 1) lora_grad_kernel(const GradArgs a) {
+// Rows of adapter `ad` among `len` rows from `at` on, in order; returns how many (all of them without an index: the list stays empty).
+__device__ __forceinline__ int list_rows(const GradArgs& a, int ad, long long at, int len, int* rows, int* scan) {
+  if (!a.index) return len;
+  const int tid = threadIdx.x;
+  int mine[GRAD_LIST / LORA_THREADS], cnt = 0, found;
+#pragma unroll
+  for (int i = 0; i < GRAD_LIST / LORA_THREADS; ++i) {
+    const int t = tid * (GRAD_LIST / LORA_THREADS) + i;
+    mine[i] = t < len && a.index[at + t] == ad;
+    cnt += mine[i];
+  }
+  int pos = cta_scan(cnt, scan, found);
+#pragma unroll
+  for (int i = 0; i < GRAD_LIST / LORA_THREADS; ++i)
+    if (mine[i]) rows[pos++] = (int)(at + tid * (GRAD_LIST / LORA_THREADS) + i);
+  __syncthreads();
+  return found;
+}
+
+struct GradTile {
+  GradJob job;
+  int r0, col0;      // first rank and column of the tile
+  long long lo, hi;  // rows of this CTA
+};
+__device__ __forceinline__ GradTile grad_tile(const GradArgs& a, int tile, int ranks, int C, int c) {
+  int jb = 0;
+  while (jb + 1 < a.jobs && tile >= a.job[jb].tiles) tile -= a.job[jb++].tiles;
+  GradTile t;
+  t.job = a.job[jb];
+  const int passes = (t.job.ru + ranks - 1) / ranks;
+  t.r0 = (tile % passes) * ranks;
+  t.col0 = t.job.c0 + (tile / passes) * GRAD_COLS;
+  const long long per = (((long long)a.T + C - 1) / C + 15) / 16 * 16;
+  t.lo = min((long long)a.T, per * c);
+  t.hi = min((long long)a.T, t.lo + per);
+  return t;
+}
+
+// Adds up the CTAs' tiles [ranks][GRAD_STRIDE] through each other's shared memory, in order; each writes its share.
+__device__ __forceinline__ void write_grad(cg::cluster_group& cluster, const GradArgs& a, const GradTile& t, float* tile, int ranks, int ad) {
+  const int C = cluster.num_blocks(), c = cluster.block_rank();
+  const GradJob& job = t.job;
+  cluster_sync_all();
+  const int all = ranks * GRAD_COLS, share = (all + C - 1) / C;
+  for (int e = c * share + threadIdx.x; e < min(all, (c + 1) * share); e += LORA_THREADS) {
+    const int rank = job.across ? e % ranks : e / GRAD_COLS, col = job.across ? e / ranks : e % GRAD_COLS;
+    if (t.r0 + rank >= job.ru || t.col0 + col >= job.c1) continue;
+    float v = 0.f;
+    for (int k = 0; k < C; ++k) v += cluster.map_shared_rank(tile, k)[rank * GRAD_STRIDE + col];
+    const long long pos = (long long)ad * job.out_adapter + (job.across ? (long long)(t.col0 + col) * job.ld_out + t.r0 + rank
+                                                                         : (long long)(job.u0 + t.r0 + rank) * job.ld_out + t.col0 + col);
+    if (a.out_f32) {
+      float* o = reinterpret_cast<float*>(job.out) + pos;
+      *o = a.accumulate ? *o + v : v;
+    } else {
+      reinterpret_cast<__nv_bfloat16*>(job.out)[pos] = __float2bfloat16_rn(v);
+    }
+  }
+  cluster_sync_all();      // no CTA leaves while its tile is read
+}
+
+// out[rank, col] (+)= sum over the adapter's rows t of p[t, rank] z[t, col]: ranks x 256 columns per cluster, the rows cut over its CTAs.
+// This form takes rows of any alignment and fp32 ones: 16 ranks at a time, operands along their rows from global memory, turned in registers.
+// Warps 0-3 and 4-7 take every other 16 rows.
+template <typename T, int S, bool WIDE>
+__global__ void __launch_bounds__(LORA_THREADS, 1) lora_grad_any_kernel(const __grid_constant__ GradArgs a) {
   constexpr int P = PARTS<T>;
-  constexpr int GSTRIDE = GRAD_COLS + 4;
   __shared__ int s_rows[GRAD_LIST];
   __shared__ int s_scan[LORA_WARPS];
-  extern __shared__ __align__(16) float tile[];      // [16 RT][GSTRIDE]
+  extern __shared__ __align__(16) uint8_t dyn[];
+  float* tile = reinterpret_cast<float*>(dyn);
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), c = cluster.block_rank();
-  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t4 = lane & 3;
-  const int cid = blockIdx.x / C, ad = blockIdx.y;
-  int jb = 0, ti = cid;
-  while (jb + 1 < a.jobs && ti >= a.job[jb].tiles) ti -= a.job[jb++].tiles;
-  const GradJob job = a.job[jb];
-  const int passes = (job.ru + 16 * RT - 1) / (16 * RT);
-  const int r0 = (ti % passes) * 16 * RT, col0 = job.c0 + (ti / passes) * GRAD_COLS;
-  const int cw = w & 3, half = w >> 2, colw = col0 + cw * 64;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
+  const int ad = blockIdx.y, cw = w & 3, half = w >> 2;
+  const GradTile t = grad_tile(a, blockIdx.x / C, 16, C, c);
+  const GradJob& job = t.job;
   const T* z = reinterpret_cast<const T*>(job.z);
+  const int colw = t.col0 + cw * 64;
 
-  float acc[RT][8][4];
+  float acc[8][4];
 #pragma unroll
-  for (int i = 0; i < RT; ++i)
+  for (int j = 0; j < 8; ++j)
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
-
-  const long long per = (((long long)a.T + C - 1) / C + 15) / 16 * 16, lo = min((long long)a.T, per * c), hi = min((long long)a.T, lo + per);
-  for (long long at = lo; at < hi; at += GRAD_LIST) {
-    const int len = (int)min((long long)GRAD_LIST, hi - at);
-    int found = len;
-    if (a.index) {      // the adapter's rows among these, in order
-      int mine[4], cnt = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = tid * 4 + i;
-        mine[i] = t < len && a.index[at + t] == ad;
-        cnt += mine[i];
-      }
-      int pos = cnt;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, pos, o);
-        if (lane >= o) pos += v;
-      }
-      if (lane == 31) s_scan[w] = pos;
-      __syncthreads();
-      found = 0;
-      for (int i = 0; i < LORA_WARPS; ++i) {
-        if (i < w) pos += s_scan[i];
-        found += s_scan[i];
-      }
-      pos -= cnt;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (mine[i]) s_rows[pos++] = (int)(at + tid * 4 + i);
-      __syncthreads();
-    }
-#pragma unroll(P == 1 && RT == 1 ? 2 : 1)
+    for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
+  for (long long at = t.lo; at < t.hi; at += GRAD_LIST) {
+    const int found = list_rows(a, ad, at, (int)min((long long)GRAD_LIST, t.hi - at), s_rows, s_scan);
     for (int t0 = 16 * half; t0 < found; t0 += 32) {
       long long row[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int t = t0 + 8 * h + g;
-        row[h] = t < found ? (a.index ? (long long)s_rows[t] : at + t) : -1;
+        const int i = t0 + 8 * h + g;
+        row[h] = i < found ? (a.index ? (long long)s_rows[i] : at + i) : -1;
       }
       uint32_t zb[8][P][2];      // [column tile][part][register]
 #pragma unroll
@@ -617,101 +917,134 @@ __global__ void __launch_bounds__(LORA_THREADS, 1) lora_grad_kernel(const GradAr
 #pragma unroll
             for (int s = 0; s < P; ++s) zb[4 * q + j][s][h] = turn(v[s][j]);
         }
+      uint32_t pa[S][4];      // rows of the product: ranks; its inner index: tokens
 #pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        uint32_t pa[S][4];
+      for (int s = 0; s < S; ++s)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)          // rows of the product: ranks; its inner index: tokens
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const int rank = r0 + 16 * i + 8 * h + 2 * t4;
-            float f0 = 0.f, f1 = 0.f;
-            if (row[k] >= 0) {
-              const float* src = job.p + row[k] * a.rtot + job.u0 + rank;
-              if (rank < job.ru) f0 = src[0];
-              if (rank + 1 < job.ru) f1 = src[1];
-            }
-            uint32_t p0[S], p1[S];
-            split<S>(f0, p0);
-            split<S>(f1, p1);
-#pragma unroll
-            for (int s = 0; s < S; ++s) pa[s][h + 2 * k] = turn(p0[s] | (p1[s] << 16));
+            uint32_t v = 0;
+            if (row[k] >= 0) v = *reinterpret_cast<const uint32_t*>(job.p + ((long long)s * a.T + row[k]) * job.pcols + job.p0 + t.r0 + 8 * h + 2 * t4);
+            pa[s][h + 2 * k] = turn(v);
           }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if constexpr (S == 3) {      // the tensor cores cut sums off: 32-bit results take a few products at a time and round the sum
-            float few[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_parts<S, P>(few, pa, zb[j]);
+      for (int j = 0; j < 8; ++j) {
+        if constexpr (S == 3) {      // the tensor cores cut sums off: 32-bit results take a few products at a time and round the sum
+          float few[4] = {0.f, 0.f, 0.f, 0.f};
+          mma_parts<S, P>(few, pa, zb[j]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][j][e] += few[e];
-          } else {
-            mma_parts<S, P>(acc[i][j], pa, zb[j]);
-          }
+          for (int e = 0; e < 4; ++e) acc[j][e] += few[e];
+        } else {
+          mma_parts<S, P>(acc[j], pa, zb[j]);
         }
       }
     }
     if (a.index) __syncthreads();
   }
-
-  // ---- sums over the halves and the CTAs
-  auto place = [&](int i, int j, int e) {      // position of accumulator e in the tile
-    const int rank = 16 * i + g + (e >> 1) * 8;
-    const int col = cw * 64 + 32 * (j >> 2) + 8 * t4 + 2 * (j & 3) + (e & 1);
-    return rank * GSTRIDE + col;
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        f((g + (e >> 1) * 8) * GRAD_STRIDE + cw * 64 + 32 * (j >> 2) + 8 * t4 + 2 * (j & 3) + (e & 1), acc[j][e]);
   };
-  if (half == 1)
-#pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) tile[place(i, j, e)] = acc[i][j][e];
+  if (half == 1) each([&](int at, float v) { tile[at] = v; });
   __syncthreads();
-  if (half == 0)
-#pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) tile[place(i, j, e)] += acc[i][j][e];
-  cluster_sync_all();
-  const int all = 16 * RT * GRAD_COLS, share = (all + C - 1) / C;
-  for (int e = c * share + tid; e < min(all, (c + 1) * share); e += LORA_THREADS) {
-    const int rank = job.across ? e % (16 * RT) : e / GRAD_COLS, col = job.across ? e / (16 * RT) : e % GRAD_COLS;
-    if (r0 + rank >= job.ru || col0 + col >= job.c1) continue;
-    float v = 0.f;
-    for (int k = 0; k < C; ++k) v += cluster.map_shared_rank(tile, k)[rank * GSTRIDE + col];
-    const long long pos = (long long)ad * job.out_adapter + (job.across ? (long long)(col0 + col) * job.ld_out + r0 + rank
-                                                                         : (long long)(job.u0 + r0 + rank) * job.ld_out + col0 + col);
-    if (a.out_f32) {
-      float* o = reinterpret_cast<float*>(job.out) + pos;
-      *o = a.accumulate ? *o + v : v;
-    } else {
-      reinterpret_cast<__nv_bfloat16*>(job.out)[pos] = __float2bfloat16_rn(v);
-    }
-  }
-  cluster_sync_all();      // no CTA leaves while its tile is read
+  if (half == 0) each([&](int at, float v) { tile[at] += v; });
+  write_grad(cluster, a, t, tile, 16, ad);
 }
 
-template <typename T, int S, int RT, bool WIDE>
-int launch_grad(const GradArgs& a, int tiles, int cluster, cudaStream_t stream) {
-  auto* k = lora_grad_kernel<T, S, RT, WIDE>;
-  const int smem = 16 * RT * (GRAD_COLS + 4) * 4;
-  if (smem > 48 * 1024 && check_cuda(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "lora gradient shared memory"))
-    return -1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(tiles * cluster), (unsigned)a.n);
-  cfg.blockDim = dim3(LORA_THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cluster;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, k, a), "lora gradient launch");
+// The same for bf16 rows that 16-byte copies fit: 32 rows at a time, z and both parts of p, go through a ring of shared-memory stages and enter
+// the products turned (`ldmatrix`). A warp takes 32 columns and all ranks. At rank 64 the products bound it, below the rows' traffic.
+constexpr int GRAD_ROWS = 32, GRAD_ZROW = GRAD_COLS * 2 + 16, GRAD_STAGES = 4;
+template <int RT> constexpr int GRAD_PROW = 32 * RT + 16;
+template <int RT> constexpr int GRAD_STAGE = GRAD_ROWS * (GRAD_ZROW + 2 * GRAD_PROW<RT>);
+template <int RT>
+__global__ void __launch_bounds__(LORA_THREADS, 2) lora_grad_kernel(const __grid_constant__ GradArgs a) {
+  constexpr int PROW = GRAD_PROW<RT>, STAGE = GRAD_STAGE<RT>;
+  __shared__ int s_rows[GRAD_LIST];
+  __shared__ int s_scan[LORA_WARPS];
+  extern __shared__ __align__(16) uint8_t dyn[];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = cluster.num_blocks(), c = cluster.block_rank();
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t4 = lane & 3;
+  const int ad = blockIdx.y;
+  const GradTile t = grad_tile(a, blockIdx.x / C, 16 * RT, C, c);
+  const GradJob& job = t.job;
+  const __nv_bfloat16* z = reinterpret_cast<const __nv_bfloat16*>(job.z);
+  const uint32_t ring = smem_u32(dyn);
+  const int r16 = round16(job.ru) - t.r0;      // ranks that p has from r0 on
+
+  float acc[RT][4][4];
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
+  for (long long at = t.lo; at < t.hi; at += GRAD_LIST) {
+    const int found = list_rows(a, ad, at, (int)min((long long)GRAD_LIST, t.hi - at), s_rows, s_scan);
+    const int steps = (found + GRAD_ROWS - 1) / GRAD_ROWS;
+    auto fill = [&](int step) {
+      const uint32_t dst = ring + (step % GRAD_STAGES) * STAGE;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = (tid >> 5) + 8 * i, k = step * GRAD_ROWS + r, col = t.col0 + 8 * lane;
+        const bool ok = k < found && col < job.c1;
+        const long long row = k < found ? (a.index ? (long long)s_rows[k] : at + k) : 0;
+        cp_async<16>(dst + r * GRAD_ZROW + 16 * lane, ok ? z + row * job.ldz + col : z, ok);
+      }
+      for (int i = tid; i < 2 * GRAD_ROWS * 2 * RT; i += LORA_THREADS) {
+        const int q = i % (2 * RT), r = (i / (2 * RT)) % GRAD_ROWS, s = i / (2 * RT * GRAD_ROWS), k = step * GRAD_ROWS + r;
+        const bool ok = k < found && 8 * q < r16;
+        const long long row = k < found ? (a.index ? (long long)s_rows[k] : at + k) : 0;
+        cp_async<16>(dst + GRAD_ROWS * GRAD_ZROW + (s * GRAD_ROWS + r) * PROW + 16 * q,
+                     ok ? job.p + ((long long)s * a.T + row) * job.pcols + job.p0 + t.r0 + 8 * q : job.p, ok);
+      }
+    };
+#pragma unroll
+    for (int st = 0; st < GRAD_STAGES - 1; ++st) {
+      if (st < steps) fill(st);
+      cp_commit();
+    }
+    for (int step = 0; step < steps; ++step) {
+      cp_wait<GRAD_STAGES - 2>();
+      __syncthreads();
+      if (step + GRAD_STAGES - 1 < steps) fill(step + GRAD_STAGES - 1);
+      cp_commit();
+      const uint32_t src = ring + (step % GRAD_STAGES) * STAGE;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        uint32_t b[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          ldmatrix4<true>(b[j], src + (16 * k + 8 * ((lane >> 3) & 1) + (lane & 7)) * GRAD_ZROW + w * 64 + 32 * j + 16 * (lane >> 4));
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          if (16 * i >= r16) break;
+#pragma unroll
+          for (int s = 1; s >= 0; --s) {
+            uint32_t pa[4];
+            ldmatrix4<true>(pa, src + GRAD_ROWS * GRAD_ZROW + (s * GRAD_ROWS + 16 * k + 8 * (lane >> 4) + (lane & 7)) * PROW + 32 * i +
+                                    16 * ((lane >> 3) & 1));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mma_bf16(acc[i][j], pa[0], pa[1], pa[2], pa[3], b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
+          }
+        }
+      }
+    }
+    cp_wait<0>();
+    __syncthreads();
+  }
+  float* tile = reinterpret_cast<float*>(dyn);      // [16 RT][GRAD_STRIDE], where the stages were
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) tile[(16 * i + g + 8 * (e >> 1)) * GRAD_STRIDE + w * 32 + 8 * j + 2 * t4 + (e & 1)] = acc[i][j][e];
+  write_grad(cluster, a, t, tile, 16 * RT, ad);
 }
 
 bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
@@ -722,26 +1055,27 @@ bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) 
 using namespace edl;
 
 // x [T, K], y and out [T, N] (y null: the adapters' part alone; y == out: in place), row strides in elements. widths: columns of the
-// `parts` parts of N. a: [n][parts * r][K], b: [n][N][r] with strides. backward = 0: out = y + s (x a^T) b^T, u_out [T, parts * r] (may
-// be null) takes s x a^T. backward = 1: x is dy [T, N], out dx [T, K] (null: u_out alone), y null; u_out takes s dy b.
+// `parts` parts of N. a: [n][parts * r][K], b: [n][N][r] with strides. backward = 0: out = y + s (x a^T) b^T. backward = 1: x is dy [T, N],
+// out dx [T, K] (null: u alone), y null. u: s x a^T or s dy b in bf16 parts (2 for bf16 results, 3 for fp32 ones), [parts][T][columns] with
+// parts * r rounded up to 16 per part (forward) or as a whole (backward); asked for above 256 rows of bf16, else it may be null.
 // index [T] int32 or null (adapter 0 everywhere), scale [n] fp32 or null (scale_all). x_f32: x and the weights are fp32 (then
 // y and out too), else bf16; y_f32: type of y and out. Indexes from n on set the status word and count as none.
 EDL_HOST_API int edl_lora_apply(const void* x, long long ldx, const void* y, long long ldy, void* out, long long ldo, const void* a,
                                 long long a_adapter, long long lda, const void* b, long long b_adapter, long long ldb,
-                                const int* index, const float* scale, float scale_all, float* u_out, int T, int K, int N, int n, int r,
-                                int parts, const int* widths, int x_f32, int y_f32, int backward, int* status, void* stream) {
+                                const int* index, const float* scale, float scale_all, void* u, long long u_size, int T, int K, int N,
+                                int n, int r, int parts, const int* widths, int x_f32, int y_f32, int backward, int* status, void* stream) {
   if (T <= 0) return 0;
   if (K <= 0 || N <= 0 || n <= 0 || r <= 0 || parts < 1 || parts > LORA_SEGS || r > 512 / parts) {
     set_last_error("edl_lora_apply: needs sizes above 0, up to %d parts and parts x rank up to 512", LORA_SEGS);
     return -1;
   }
-  if ((x_f32 && !y_f32) || (backward && x_f32 != y_f32) || (backward && y) || (!out && !(backward && u_out))) {
+  if ((x_f32 && !y_f32) || (backward && x_f32 != y_f32) || (backward && y) || (!out && !(backward && u))) {
     set_last_error("edl_lora_apply: fp32 inputs give fp32 results; the backward form takes one type and no y");
     return -1;
   }
   LoraArgs g{};
   g.x = x; g.ldx = ldx; g.y = y; g.ldy = ldy; g.out = out; g.ldo = ldo;
-  g.index = index; g.scale = scale; g.scale_all = scale_all; g.u_out = u_out; g.status = status;
+  g.index = index; g.scale = scale; g.scale_all = scale_all; g.u = (unsigned short*)u; g.status = status;
   g.T = T; g.n = n; g.rtot = parts * r;
   g.copy = out && out != y;
   int c0 = 0;
@@ -773,48 +1107,100 @@ EDL_HOST_API int edl_lora_apply(const void* x, long long ldx, const void* y, lon
     g.up = a; g.up_adapter = a_adapter; g.ld_up = lda;
     g.down_segs = parts;
     for (int p = 0; p < parts; ++p) g.down_seg[p] = seg[p];
-    g.up_segs = out ? 1 : 0;
+    g.up_segs = 1;
     g.up_seg[0] = whole;
+  }
+  g.ucols = g.up_segs * round16(g.up_seg[0].ru);
+  const int s = y_f32 ? 3 : 2;
+  if (u && (u_size < (long long)s * T * g.ucols || !aligned(u, 16))) {
+    set_last_error("edl_lora_apply: u needs %lld elements from a 16-byte boundary on", (long long)s * T * g.ucols);
+    return -1;
   }
   const int va = x_f32 ? 4 : 8, vy = y_f32 ? 4 : 8;      // elements in 16 bytes
   wide = wide && ldx % va == 0 && aligned(x, 16) && aligned(a, 16) && lda % va == 0 && a_adapter % va == 0 && aligned(b, x_f32 ? 16 : 8) &&
          ldb % 4 == 0 && b_adapter % 4 == 0 && (!y || (ldy % vy == 0 && aligned(y, 16))) && (!out || (ldo % vy == 0 && aligned(out, 16)));
-
-  // Chunks of 8 rows while the rows of a step fit one look (few rows per adapter, many clusters), of 64 above; wide ranks keep
-  // less so that u fits shared memory.
-  const int rt = wide && !x_f32 && (backward ? (r > 16 || parts * r > 16) : parts * r > 16) ? 4 : 1;
-  int nt = 1, tgroups = 1;
-  if (T > LORA_ROWS && g.rtot <= 256) {
-    nt = 4;
-    tgroups = g.rtot <= 128 ? 2 : 1;
-  }
-  const int chunk = 8 * nt * tgroups, cluster = 8;
-  const int in_block = T < LORA_ROWS ? T : LORA_ROWS;
-  const long long most = (long long)(index ? (n < in_block ? n + 1 : in_block) : 1) + in_block / chunk;      // pairs among a block's rows
-  const int blocks = (T + LORA_ROWS - 1) / LORA_ROWS;
-  int groups = 128 / blocks;
-  if (groups < LORA_ROWS / chunk) groups = LORA_ROWS / chunk;
-  if (groups > most) groups = (int)most;
-  if (groups > in_block) groups = in_block;
-  g.groups = groups;
-  const int s = y_f32 ? 3 : 2;
-  int ucols = g.up_segs ? g.up_segs * round16(g.up_seg[0].ru) : 0;
-  const int red = (LORA_WARPS / tgroups) * chunk * (16 * rt + 4) * 4, su = s * chunk * u_stride(ucols) * 2;
-  const int smem = ((chunk * g.rtot * 4 + 15) & ~15) + (red > su ? red : su);
   cudaStream_t st = (cudaStream_t)stream;
-#define EDL_LORA_NT(TX, TO, RTV, BW, W)                                                     \
-  return nt == 1 ? launch_lora<TX, TO, RTV, 1, BW, W>(g, cluster, tgroups, smem, st)        \
-                 : launch_lora<TX, TO, RTV, 4, BW, W>(g, cluster, tgroups, smem, st)
-#define EDL_LORA_BF(TO, BW)                                             \
-  {                                                                     \
-    if (!wide) { EDL_LORA_NT(__nv_bfloat16, TO, 1, BW, false); }        \
-    if (rt == 4) { EDL_LORA_NT(__nv_bfloat16, TO, 4, BW, true); }       \
-    EDL_LORA_NT(__nv_bfloat16, TO, 1, BW, true);                        \
+  const int blocks = (int)(((long long)T + LORA_ROWS - 1) / LORA_ROWS), in_block = T < LORA_ROWS ? T : LORA_ROWS, sms = sm_count();
+  // clusters for a block's units: as many as it can have, or fewer that take turns once there are enough for the GPU
+  auto groups_of = [&](int chunk) {
+    const long long most = (long long)(index ? (n < in_block ? n + 1 : in_block) : 1) + in_block / chunk;
+    int groups = 128 / blocks;
+    if (groups < LORA_ROWS / chunk) groups = LORA_ROWS / chunk;
+    if (groups > most) groups = (int)most;
+    return groups > in_block ? in_block : groups;
+  };
+
+  if (wide && !x_f32 && T > LORA_ROWS) {
+    if (!u) {
+      set_last_error("edl_lora_apply: more than %d rows need u", LORA_ROWS);
+      return -1;
+    }
+    g.groups = groups_of(DOWN_ROWS);
+    int ru = 0, cols = 0;
+    for (int i = 0; i < g.down_segs; ++i) {
+      ru = g.down_seg[i].ru > ru ? g.down_seg[i].ru : ru;
+      cols = g.down_seg[i].c1 - g.down_seg[i].c0 > cols ? g.down_seg[i].c1 - g.down_seg[i].c0 : cols;
+    }
+    // enough CTAs for two per SM, each with at least four steps of columns
+    int cluster = 1;
+    while (cluster < 8 && (long long)((T + DOWN_ROWS - 1) / DOWN_ROWS) * cluster < 2 * sms && cols >= 2 * cluster * 4 * DOWN_K) cluster *= 2;
+    const dim3 grid((unsigned)((long long)blocks * g.groups * cluster));
+#define EDL_LORA_DOWN(RTV)                                                                                                               \
+  {                                                                                                                                      \
+    if (backward ? launch_cluster(lora_down_kernel<RTV, true>, grid, cluster, DOWN_SMEM<RTV, true>, st, "lora down launch", g, s)        \
+                 : launch_cluster(lora_down_kernel<RTV, false>, grid, cluster, DOWN_SMEM<RTV, false>, st, "lora down launch", g, s))     \
+      return -1;                                                                                                                         \
   }
-#define EDL_LORA_F32(BW)                                        \
-  {                                                             \
-    if (!wide) { EDL_LORA_NT(float, float, 1, BW, false); }     \
-    EDL_LORA_NT(float, float, 1, BW, true);                     \
+    if (ru <= 16) EDL_LORA_DOWN(1)
+    else if (ru <= 32) EDL_LORA_DOWN(2)
+    else EDL_LORA_DOWN(4)
+#undef EDL_LORA_DOWN
+    if (!out) return 0;
+    int tiles = 0;
+    for (int i = 0; i < g.up_segs; ++i) tiles += (g.up_seg[i].c1 - g.up_seg[i].c0 + 31) / 32;
+    g.groups = (tiles + LORA_WARPS - 1) / LORA_WARPS;
+    g.look = LORA_ROWS;
+    while (g.look > 64 && (long long)g.groups * ((T + g.look - 1) / g.look) < 6LL * sms) g.look /= 2;
+    const long long ctas = (long long)g.groups * (((long long)T + g.look - 1) / g.look);
+    if (ctas > 0x7fffffffLL) {
+      set_last_error("edl_lora_apply: too many rows for one launch");
+      return -1;
+    }
+    const int kc = round16(g.up_seg[0].ru) / 16;
+#define EDL_LORA_UP(TO, BW)                                                              \
+  {                                                                                      \
+    if (kc == 1) lora_up_kernel<TO, 1, BW><<<(unsigned)ctas, LORA_THREADS, 0, st>>>(g);  \
+    else if (kc == 2) lora_up_kernel<TO, 2, BW><<<(unsigned)ctas, LORA_THREADS, 0, st>>>(g); \
+    else lora_up_kernel<TO, 4, BW><<<(unsigned)ctas, LORA_THREADS, 0, st>>>(g);          \
+  }
+    if (backward) EDL_LORA_UP(__nv_bfloat16, true)
+    else if (y_f32) EDL_LORA_UP(float, false)
+    else EDL_LORA_UP(__nv_bfloat16, false)
+#undef EDL_LORA_UP
+    return check_cuda(cudaGetLastError(), "lora up launch");
+  }
+
+  const int ranks = backward ? r : parts * r;      // that one pass over x can take
+  const int rt = !wide || x_f32 || ranks <= 16 ? 1 : ranks <= 32 ? 2 : 4;
+  g.groups = groups_of(16);
+  // clusters of eight while they all fit the GPU twice, then smaller ones
+  int cluster = 8;
+  while (cluster > 2 && (long long)blocks * g.groups * cluster > 4LL * sms) cluster /= 2;
+  const int red = LORA_WARPS * 16 * (16 * rt + 4) * 4, su = s * 16 * u_stride(g.ucols) * 2;
+  const int smem = ((16 * g.rtot * 4 + 15) & ~15) + (red > su ? red : su);
+  const dim3 grid((unsigned)((long long)blocks * g.groups * cluster));
+#define EDL_LORA(TX, TO, RTV, BW, W) return launch_cluster(lora_kernel<TX, TO, RTV, BW, W>, grid, cluster, smem, st, "lora launch", g)
+#define EDL_LORA_BF(TO, BW)                                    \
+  {                                                            \
+    if (!wide) EDL_LORA(__nv_bfloat16, TO, 1, BW, false);      \
+    if (rt == 4) EDL_LORA(__nv_bfloat16, TO, 4, BW, true);     \
+    if (rt == 2) EDL_LORA(__nv_bfloat16, TO, 2, BW, true);     \
+    EDL_LORA(__nv_bfloat16, TO, 1, BW, true);                  \
+  }
+#define EDL_LORA_F32(BW)                               \
+  {                                                    \
+    if (!wide) EDL_LORA(float, float, 1, BW, false);   \
+    EDL_LORA(float, float, 1, BW, true);               \
   }
   if (x_f32) {
     if (backward) EDL_LORA_F32(true) else EDL_LORA_F32(false)
@@ -822,14 +1208,15 @@ EDL_HOST_API int edl_lora_apply(const void* x, long long ldx, const void* y, lon
   if (backward) EDL_LORA_BF(__nv_bfloat16, true)
   if (y_f32) EDL_LORA_BF(float, false)
   EDL_LORA_BF(__nv_bfloat16, false)
-#undef EDL_LORA_NT
+#undef EDL_LORA
 #undef EDL_LORA_BF
 #undef EDL_LORA_F32
 }
 
-// da [n][parts * r][K] (+)= g^T x and db [n][N][r] (+)= dy^T u over each adapter's rows (either may be null). g, u: fp32 [T, parts * r]
-// as edl_lora_apply leaves them. out_f32: type of da and db; accumulate (fp32 only): add to them. Adapters without rows get zeros.
-EDL_HOST_API int edl_lora_grads(const void* x, long long ldx, const void* dy, long long ldy, const float* g, const float* u,
+// da [n][parts * r][K] (+)= g^T x and db [n][N][r] (+)= dy^T u over each adapter's rows (either may be null). g (for da), u (for db): what
+// edl_lora_apply left of the backward and the forward call. out_f32: type of da and db; accumulate (fp32 only): add to them.
+// Adapters without rows get zeros.
+EDL_HOST_API int edl_lora_grads(const void* x, long long ldx, const void* dy, long long ldy, const void* g, const void* u,
                                 const int* index, void* da, long long da_adapter, long long ld_da, void* db, long long db_adapter,
                                 long long ld_db, int T, int K, int N, int n, int r, int parts, const int* widths, int in_f32,
                                 int out_f32, int accumulate, void* stream) {
@@ -842,20 +1229,20 @@ EDL_HOST_API int edl_lora_grads(const void* x, long long ldx, const void* dy, lo
     return -1;
   }
   GradArgs a{};
-  a.index = index; a.T = T < 0 ? 0 : T; a.n = n; a.rtot = parts * r; a.out_f32 = out_f32; a.accumulate = accumulate;
+  a.index = index; a.T = T < 0 ? 0 : T; a.n = n; a.out_f32 = out_f32; a.accumulate = accumulate;
   const int va = in_f32 ? 4 : 8;
   bool wide = true;
-  const int rt = in_f32 || (da ? parts * r : r) <= 16 ? 1 : 4;      // ranks that one pass over the rows takes
-  auto tiles_of = [&](int cols, int ru) { return ((cols + GRAD_COLS - 1) / GRAD_COLS) * ((ru + 16 * rt - 1) / (16 * rt)); };
-  int tiles = 0;
+  int most = 0;
   if (da) {
-    a.job[a.jobs++] = GradJob{x, g, da, ldx, da_adapter, ld_da, 0, K, 0, parts * r, tiles_of(K, parts * r), 0};
+    a.job[a.jobs++] = GradJob{x, (const unsigned short*)g, da, ldx, da_adapter, ld_da, 0, K, 0, parts * r, round16(parts * r), 0, 0, 0};
     wide = wide && K % 8 == 0 && ldx % va == 0 && aligned(x, 16);
+    most = parts * r;
   }
   if (db) {
     int c0 = 0;
     for (int p = 0; p < parts; ++p) {
-      a.job[a.jobs++] = GradJob{dy, u, db, ldy, db_adapter, ld_db, c0, c0 + widths[p], p * r, r, tiles_of(widths[p], r), 1};
+      a.job[a.jobs++] = GradJob{dy, (const unsigned short*)u, db, ldy, db_adapter, ld_db, c0, c0 + widths[p], p * r, r, parts * round16(r),
+                                p * round16(r), 0, 1};
       c0 += widths[p];
       wide = wide && widths[p] % 8 == 0;
     }
@@ -864,21 +1251,30 @@ EDL_HOST_API int edl_lora_grads(const void* x, long long ldx, const void* dy, lo
       return -1;
     }
     wide = wide && ldy % va == 0 && aligned(dy, 16);
+    most = r > most ? r : most;
   }
   if (!a.jobs) return 0;
-  for (int j = 0; j < a.jobs; ++j) tiles += a.job[j].tiles;
-  int cluster = 8;      // rows of a cluster are cut into as many shares; short inputs need fewer
+  const bool fast = wide && !in_f32;
+  const int rt = !fast || most <= 16 ? 1 : most <= 32 ? 2 : 4;
+  int tiles = 0;
+  for (int j = 0; j < a.jobs; ++j) {
+    GradJob& job = a.job[j];
+    job.tiles = ((job.c1 - job.c0 + GRAD_COLS - 1) / GRAD_COLS) * ((job.ru + 16 * rt - 1) / (16 * rt));
+    tiles += job.tiles;
+  }
+  int cluster = 8;      // rows are cut into as many shares; short inputs need fewer
   while (cluster > 1 && a.T < cluster * 32) cluster /= 2;
   cudaStream_t st = (cudaStream_t)stream;
-  if (in_f32) return wide ? launch_grad<float, 3, 1, true>(a, tiles, cluster, st) : launch_grad<float, 3, 1, false>(a, tiles, cluster, st);
-#define EDL_LORA_GRAD(SV)                                                                        \
-  {                                                                                              \
-    if (rt == 4) return wide ? launch_grad<__nv_bfloat16, SV, 4, true>(a, tiles, cluster, st)    \
-                             : launch_grad<__nv_bfloat16, SV, 4, false>(a, tiles, cluster, st);  \
-    return wide ? launch_grad<__nv_bfloat16, SV, 1, true>(a, tiles, cluster, st)                 \
-                : launch_grad<__nv_bfloat16, SV, 1, false>(a, tiles, cluster, st);               \
+  const dim3 grid((unsigned)(tiles * cluster), (unsigned)n);
+  const char* what = "lora gradient launch";
+  if (fast) {
+    auto smem = [](int ring, int ranks) { const int t = ranks * GRAD_STRIDE * 4; return ring > t ? ring : t; };
+    if (rt == 1) return launch_cluster(lora_grad_kernel<1>, grid, cluster, smem(GRAD_STAGES * GRAD_STAGE<1>, 16), st, what, a);
+    if (rt == 2) return launch_cluster(lora_grad_kernel<2>, grid, cluster, smem(GRAD_STAGES * GRAD_STAGE<2>, 32), st, what, a);
+    return launch_cluster(lora_grad_kernel<4>, grid, cluster, smem(GRAD_STAGES * GRAD_STAGE<4>, 64), st, what, a);
   }
-  if (out_f32) EDL_LORA_GRAD(3)
-  EDL_LORA_GRAD(2)
-#undef EDL_LORA_GRAD
+  const int smem = 16 * GRAD_STRIDE * 4;
+  if (in_f32) return wide ? launch_cluster(lora_grad_any_kernel<float, 3, true>, grid, cluster, smem, st, what, a)
+                          : launch_cluster(lora_grad_any_kernel<float, 3, false>, grid, cluster, smem, st, what, a);
+  return launch_cluster(lora_grad_any_kernel<__nv_bfloat16, 2, false>, grid, cluster, smem, st, what, a);
 }

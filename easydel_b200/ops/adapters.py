@@ -18,13 +18,14 @@ import torch
 from . import _lib
 
 vp, i32, i64, f32 = _lib.vp, _lib.i32, _lib.i64, _lib.f32
-_lib.register("edl_lora_apply", i32, [vp, i64, vp, i64, vp, i64, vp, i64, i64, vp, i64, i64, vp, vp, f32, vp, i32, i32, i32, i32, i32,
-                                      i32, vp, i32, i32, i32, vp, vp])
+_lib.register("edl_lora_apply", i32, [vp, i64, vp, i64, vp, i64, vp, i64, i64, vp, i64, i64, vp, vp, f32, vp, i64, i32, i32, i32,
+                                      i32, i32, i32, vp, i32, i32, i32, vp, vp])
 _lib.register("edl_lora_grads", i32, [vp, i64, vp, i64, vp, vp, vp, vp, i64, i64, vp, i64, i64, i32, i32, i32, i32, i32, i32, vp, i32,
                                       i32, i32, vp])
 
 MAX_RANK = 512       # ranks of all parts together
 MAX_PARTS = 8
+FEW_ROWS = 256       # up to here the inner value stays in shared memory
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -77,14 +78,22 @@ def _check(y, x, a, b, index, scale, parts, out):
     return parts
 
 
+def _inner(T: int, r: int, parts: int, result: torch.dtype, device, backward: bool = False) -> torch.Tensor:
+    """Memory for the scaled inner value ``s x a^T`` (``s dy b`` of the backward pass) as bf16 parts ``[parts of a value, T, ranks]``."""
+    cols = (parts * r + 15) // 16 * 16 if backward else parts * ((r + 15) // 16 * 16)
+    return torch.empty((3 if result == torch.float32 else 2, T, cols), dtype=torch.bfloat16, device=device)
+
+
 def _apply(x, y, out, a, b, index, scale, u, parts, backward=False):
     n, N, r = b.shape
+    if u is None and x.shape[0] > FEW_ROWS:
+        u = _inner(x.shape[0], r, len(parts), out.dtype, x.device, backward)
     st = scale if isinstance(scale, torch.Tensor) else None
     ld = [0 if t is None else t.stride(0) if t.shape[0] > 1 else t.shape[1] for t in (x, y, out)]
     with _lib.on_device(x.device):
         _lib.call("edl_lora_apply", x.data_ptr(), ld[0], _lib.ptr(y), ld[1], _lib.ptr(out), ld[2], a.data_ptr(), a.stride(0), a.stride(1),
                   b.data_ptr(), b.stride(0), b.stride(1), _lib.ptr(index), _lib.ptr(st), 0.0 if st is not None else float(scale),
-                  _lib.ptr(u), x.shape[0], a.shape[2], N, n, r, len(parts), (C.c_int * len(parts))(*parts),
+                  _lib.ptr(u), 0 if u is None else u.numel(), x.shape[0], a.shape[2], N, n, r, len(parts), (C.c_int * len(parts))(*parts),
                   int(x.dtype == torch.float32), int((out if out is not None else x).dtype == torch.float32), int(backward),
                   _lib.status_word(x.device).data_ptr(), _lib.stream_ptr())
 
@@ -102,7 +111,7 @@ class _LoraAddFn(torch.autograd.Function):
     def forward(ctx, y, x, a, b, index, scale, parts):
         y2, x2, a2, b2 = _rows(y), _rows(x), _weights(a), _weights(b)
         out = torch.empty(y.shape, dtype=y.dtype, device=y.device)
-        u = torch.empty((x2.shape[0], a.shape[1]), dtype=torch.float32, device=x.device) if ctx.needs_input_grad[3] else None
+        u = _inner(x2.shape[0], b.shape[2], len(parts), x.dtype, x.device) if ctx.needs_input_grad[3] else None
         _apply(x2, y2, out.view(-1, out.shape[-1]), a2, b2, index, scale, u, parts)
         ctx.save_for_backward(x, a, b, u, index, scale if isinstance(scale, torch.Tensor) else None)
         ctx.scale, ctx.parts = scale, parts
@@ -118,7 +127,7 @@ class _LoraAddFn(torch.autograd.Function):
         dy2, x2 = _rows(dy), _rows(x)
         T, (n, N, r) = x2.shape[0], b.shape
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-        g = torch.empty((T, a.shape[1]), dtype=torch.float32, device=x.device) if need_a else None
+        g = _inner(T, r, len(parts), x.dtype, x.device, True) if need_a else None
         if need_x or need_a:
             _apply(dy2, None, None if dx is None else dx.view(-1, dx.shape[-1]), _weights(a), _weights(b), index, scale, g, parts, True)
         grads = []
