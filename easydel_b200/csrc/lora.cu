@@ -4,11 +4,11 @@
 //
 // Mathematics: two products with a small inner size r, one after the other, so what bounds them is the traffic of x, y
 // and out (or, with a token or two per adapter, of A and B), not arithmetic: at r = 16 a byte of x or y brings 16 products.
-// That is why they use warp-level `mma.sync` and leave tensor memory alone.
 //
 // Three forms. Few rows (or rows that no 16-byte access fits, or fp32): one launch, a cluster of CTAs per adapter and chunk of rows, which
 // keeps u = x A^T in shared memory. Many rows: a launch that reduces x to u and one that expands u onto y, each of which only
-// streams, with copies in flight that no register waits for. Gradients of A and B: a launch that contracts over rows.
+// streams. Gradients of A and B: a launch that contracts over rows. Long contractions run on tcgen05 with copies in flight that no
+// register waits for; where only a few ranks are contracted, and with few rows, warp-level `mma.sync` is enough.
 // Which rows go together is found by each CTA from the indexes of its rows, so a captured graph follows the indexes of the step and nothing
 // is sorted, counted or copied by the host.
 //
@@ -250,8 +250,8 @@ __device__ __forceinline__ int cta_scan(int v, int* scan, int& total) {
   return at - v;
 }
 
-// All threads of the CTA. Rows without an adapter form units (adapter -1) where they have to be copied. Most blocks belong to one
-// request: those take no comparisons.
+// All threads of the CTA. Rows without an adapter form units (adapter -1) where they have to be copied. Most blocks of a prompt or a
+// training batch belong to one request: those take no comparisons.
 __device__ __forceinline__ void find_units(RowUnits& u, const LoraArgs& a, long long row0, int rows, int chunk) {
   const int tid = threadIdx.x, lane = tid & 31, w0 = tid & ~31;
   int id = -2;
@@ -261,19 +261,28 @@ __device__ __forceinline__ void find_units(RowUnits& u, const LoraArgs& a, long 
     if (id < 0 || id >= a.n) id = -1;
   }
   u.idx[tid] = id;
+  u.order[tid] = (short)tid;
   __syncthreads();
-  int before = tid, count = rows, first_row = 0;
-  if (!__syncthreads_and(tid >= rows || id == u.idx[0])) {
-    before = count = 0;
-    for (int j = 0; j < rows; j += 4) {      // indexes behind the last row are -2
-      if (j == w0) before = count;
-      if (!count) first_row = j;
-      const int4 v = *reinterpret_cast<const int4*>(u.idx + j);
-      count += (v.x == id) + (v.y == id) + (v.z == id) + (v.w == id);
+  if (!a.index || __syncthreads_and(tid >= rows || id == u.idx[0])) {
+    const int all = u.idx[0] >= 0 || a.copy ? (rows + chunk - 1) / chunk : 0;
+    if (tid < all) {
+      u.base[tid] = (short)(tid * chunk);
+      u.rows[tid] = (short)min(chunk, rows - tid * chunk);
+      u.ad[tid] = u.idx[0];
     }
-    while (tid < rows && u.idx[first_row] != id) ++first_row;
-    before += __popc(__match_any_sync(0xffffffffu, id) & ((1u << lane) - 1));
+    if (tid == 0) u.total = all;
+    __syncthreads();
+    return;
   }
+  int before = 0, count = 0, first_row = 0;
+  for (int j = 0; j < rows; j += 4) {      // indexes behind the last row are -2
+    if (j == w0) before = count;
+    if (!count) first_row = j;
+    const int4 v = *reinterpret_cast<const int4*>(u.idx + j);
+    count += (v.x == id) + (v.y == id) + (v.z == id) + (v.w == id);
+  }
+  while (tid < rows && u.idx[first_row] != id) ++first_row;
+  before += __popc(__match_any_sync(0xffffffffu, id) & ((1u << lane) - 1));
   const bool taken = tid < rows && (id >= 0 || a.copy), first = taken && before == 0;
   int all;
   const int place = cta_scan(first ? count : 0, u.scan, all), unit = cta_scan(first ? (count + chunk - 1) / chunk : 0, u.scan, all);
@@ -506,13 +515,6 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const __grid_cons
 }
 
 // --------------------------------------------------------------------------------------------------- many rows: x to u
-constexpr int DOWN_ROWS = 64, DOWN_K = 64, DOWN_XROW = DOWN_K * 2 + 16;      // 16 bytes behind each row: no conflicts in `ldmatrix`
-template <int RT> constexpr int DOWN_STAGES = RT == 1 ? 6 : 5;
-template <int RT, bool DOWN_T> constexpr int DOWN_WROW = DOWN_T ? 32 * RT + 16 : DOWN_XROW;
-template <int RT, bool DOWN_T>
-constexpr int DOWN_STAGE = DOWN_ROWS * DOWN_XROW + (DOWN_T ? DOWN_K : 16 * RT) * DOWN_WROW<RT, DOWN_T>;
-template <int RT, bool DOWN_T> constexpr int DOWN_SMEM = DOWN_STAGES<RT> * DOWN_STAGE<RT, DOWN_T> + DOWN_ROWS * 16 * RT * 4;
-
 template <int BYTES>
 __device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool ok) {      // zeros where not ok
   if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
@@ -523,32 +525,104 @@ template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-template <bool TRANS>
-__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
-  if constexpr (TRANS)
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-  else
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+
+// A ring of shared-memory stages that all threads fill with `cp.async` (rows may be gathered; 128-byte rows, their 16-byte pieces swizzled as
+// the tensor cores read them) and one lane feeds to `tcgen05.mma`. A stage is filled again once its products are done.
+constexpr int RING_STAGES = 4;
+struct Ring {
+  uint32_t base, bars, tmem;      // stages; "products of this stage are done" barriers, then "all done"; accumulators
+  int bytes, used, passes;        // of a stage; stages fed so far; passes finished
+  volatile int* abort_flag;
+  int* status;
+  __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity) { mbar_wait(bar, parity, abort_flag, status, EDL_TIMEOUT_MMA); }
+};
+struct RingShared {
+  uint64_t bars[RING_STAGES + 1];
+  uint32_t tmem;
+  int abort_flag;
+};
+// All threads. Waits that run out leave their code in the status word; everything after them goes on, without meaning.
+__device__ __forceinline__ Ring ring_start(RingShared& sh, const uint8_t* stages, int bytes, int tmem_cols, int* status) {
+  if (threadIdx.x == 0) {
+    for (int i = 0; i <= RING_STAGES; ++i) mbar_init(smem_u32(&sh.bars[i]), 1);
+    sh.abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (threadIdx.x >> 5 == 1) {
+    tmem_alloc(smem_u32(&sh.tmem), tmem_cols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  return Ring{smem_u32(stages), smem_u32(sh.bars), sh.tmem, bytes, 0, 0, &sh.abort_flag, status};
+}
+// `fill(stage address, step)` copies, `feed(stage address, step)` issues the products (called by one lane of warp 0). Returns once all
+// products are done and visible in tensor memory.
+template <typename Fill, typename Feed>
+__device__ __forceinline__ void ring_run(Ring& r, int steps, Fill fill, Feed feed) {
+  if (!steps) return;
+  auto put = [&](int step) {
+    const int use = r.used + step, at = use % RING_STAGES;
+    if (use >= RING_STAGES) r.wait(r.bars + 8 * at, (use / RING_STAGES - 1) & 1);
+    fill(r.base + at * r.bytes, step);
+  };
+#pragma unroll
+  for (int i = 0; i < RING_STAGES - 1; ++i) {
+    if (i < steps) put(i);
+    cp_commit();
+  }
+  for (int step = 0; step < steps; ++step) {
+    cp_wait<RING_STAGES - 2>();
+    fence_proxy_async_smem();
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      const bool leader = elect_one();
+      tc_fence_after();
+      if (leader) {
+        const int at = (r.used + step) % RING_STAGES;
+        feed(r.base + at * r.bytes, step);
+        tc_commit(r.bars + 8 * at);
+        if (step == steps - 1) tc_commit(r.bars + 8 * RING_STAGES);
+      }
+      __syncwarp();
+    }
+    if (step + RING_STAGES - 1 < steps) put(step + RING_STAGES - 1);
+    cp_commit();
+  }
+  r.used += steps;
+  r.wait(r.bars + 8 * RING_STAGES, r.passes++ & 1);
+  cp_wait<0>();
+  tc_fence_after();
+}
+__device__ __forceinline__ void ring_end(Ring& r, int tmem_cols) {
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x >> 5 == 1) tmem_dealloc(r.tmem, tmem_cols);
 }
 
-// u of 64 rows of one adapter: columns in steps of 64 through a ring of shared-memory stages (`cp.async`, rows gathered as they are
-// copied), cut over the CTAs of a cluster where there are few rows. Warps 0-3 take 16 rows each and the first half of a step's columns,
-// warps 4-7 the second. Sums of the halves and of the CTAs are added in a fixed order.
-template <int RT, bool DOWN_T>
-__global__ void __launch_bounds__(LORA_THREADS, 2) lora_down_kernel(const __grid_constant__ LoraArgs a, int parts) {
-  constexpr int STAGES = DOWN_STAGES<RT>, STAGE = DOWN_STAGE<RT, DOWN_T>, WROW = DOWN_WROW<RT, DOWN_T>, RSTRIDE = 16 * RT + 4;
+// u of up to 128 rows of one adapter (the M side; ranks are the N side): columns in steps of 64 through the ring, cut over the CTAs of a
+// cluster where there are few rows. The CTAs' sums are added in a fixed order.
+constexpr int DOWN_ROWS = 128, DOWN_K = 64, DOWN_X = DOWN_ROWS * DOWN_K * 2, DOWN_RANKS = 64;
+__host__ __device__ constexpr int down_stage(int np, bool down_t) { return DOWN_X + (down_t ? DOWN_K : np) * 128; }
+
+template <bool DOWN_T>
+__global__ void __launch_bounds__(LORA_THREADS, 2) lora_down_kernel(const __grid_constant__ LoraArgs a, int parts, int np) {
   __shared__ RowUnits units;
-  extern __shared__ __align__(16) uint8_t dyn[];
-  float* part = reinterpret_cast<float*>(dyn + STAGES * STAGE);      // [64][16 RT]
-  float* red = reinterpret_cast<float*>(dyn);                        // [64][RSTRIDE], where the stages were
-  const uint32_t ring = smem_u32(dyn);
+  __shared__ RingShared shared;
+  extern __shared__ uint8_t raw[];
+  uint8_t* dyn = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  float* part = reinterpret_cast<float*>(dyn);      // [128][np + 4], where the stages were
+  const int pstride = np + 4;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), c = cluster.block_rank();
-  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t4 = lane & 3, tg = w & 3, kh = w >> 2;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int cid = blockIdx.x / C;
   const long long row0 = (long long)(cid / a.groups) * LORA_ROWS;
   const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x);
+  Ring ring = ring_start(shared, dyn, down_stage(np, DOWN_T), 64, a.status);
   find_units(units, a, row0, (int)min((long long)LORA_ROWS, a.T - row0), DOWN_ROWS);
+  const uint32_t idesc = umma_idesc_bf16(128, np, 0, DOWN_T);
   bool pending = false;
   for (int unit = cid % a.groups; unit < units.total; unit += a.groups) {
     const int ad = units.ad[unit], m = units.rows[unit];
@@ -556,89 +630,64 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_down_kernel(const __grid
     const short* order = units.order + units.base[unit];
     const __nv_bfloat16* wd = reinterpret_cast<const __nv_bfloat16*>(a.down) + (long long)ad * a.down_adapter;
     const float s = a.scale ? a.scale[ad] : a.scale_all;
-    // a thread copies the same 16 bytes of two rows in every step
-    const __nv_bfloat16* xr[2];
+    const __nv_bfloat16* xr[4];      // a thread copies the same piece of four rows in every step
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       const int tok = (tid >> 3) + 32 * i;
       xr[i] = tok < m ? x + (row0 + order[tok]) * a.ldx + 8 * (tid & 7) : nullptr;
     }
+    const uint32_t piece = 16 * ((tid & 7) ^ ((tid >> 3) & 7));
     for (int sg = 0; sg < a.down_segs; ++sg) {
       const LoraSeg seg = a.down_seg[sg];
       const int all = (seg.c1 - seg.c0 + DOWN_K - 1) / DOWN_K, per = (all + C - 1) / C;
       const int k0 = seg.c0 + min(all, c * per) * DOWN_K, steps = min(all, (c + 1) * per) - min(all, c * per);
-      for (int r0 = 0; r0 < seg.ru; r0 += 16 * RT) {
-        auto fill = [&](int step) {
-          const uint32_t dst = ring + (step % STAGES) * STAGE;
+      for (int r0 = 0; r0 < seg.ru; r0 += np) {
+        if (pending) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");      // every CTA has read the last parts
+        auto fill = [&](uint32_t dst, int step) {
           const int k = k0 + step * DOWN_K;
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            cp_async<16>(dst + ((tid >> 3) + 32 * i) * DOWN_XROW + 16 * (tid & 7), xr[i] ? xr[i] + k : x, xr[i] && k + 8 * (tid & 7) < seg.c1);
-          const uint32_t wdst = dst + DOWN_ROWS * DOWN_XROW;
+          for (int i = 0; i < 4; ++i)
+            cp_async<16>(dst + ((tid >> 3) + 32 * i) * 128 + piece, xr[i] ? xr[i] + k : x, xr[i] && k + 8 * (tid & 7) < seg.c1);
+          const uint32_t wdst = dst + DOWN_X;
           if constexpr (!DOWN_T) {
-            for (int i = tid; i < 16 * RT * 8; i += LORA_THREADS) {
+            for (int i = tid; i < np * 8; i += LORA_THREADS) {
               const int rank = i >> 3, col = k + 8 * (i & 7);
               const bool ok = r0 + rank < seg.ru && col < seg.c1;
-              cp_async<16>(wdst + rank * WROW + 16 * (i & 7), ok ? wd + (long long)(seg.u0 + r0 + rank) * a.ld_down + col : wd, ok);
+              cp_async<16>(wdst + rank * 128 + 16 * ((i & 7) ^ (rank & 7)), ok ? wd + (long long)(seg.u0 + r0 + rank) * a.ld_down + col : wd, ok);
             }
           } else {
-            for (int i = tid; i < DOWN_K * 4 * RT; i += LORA_THREADS) {
-              const int kk = i / (4 * RT), rank = 4 * (i % (4 * RT));
+            for (int i = tid; i < DOWN_K * (np / 4); i += LORA_THREADS) {
+              const int kk = i / (np / 4), rank = 4 * (i % (np / 4));
               const bool ok = k + kk < seg.c1 && r0 + rank < seg.ru;
-              cp_async<8>(wdst + kk * WROW + 2 * rank, ok ? wd + (long long)(k + kk) * a.ld_down + r0 + rank : wd, ok);
+              cp_async<8>(wdst + kk * 128 + 16 * ((rank >> 3) ^ (kk & 7)) + 2 * (rank & 7),
+                          ok ? wd + (long long)(k + kk) * a.ld_down + r0 + rank : wd, ok);
             }
           }
         };
-        float acc[RT][2][4];
+        auto feed = [&](uint32_t src, int step) {
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
-#pragma unroll
-        for (int st = 0; st < STAGES - 1; ++st) {
-          if (st < steps) fill(st);
-          cp_commit();
-        }
-        for (int step = 0; step < steps; ++step) {
-          cp_wait<STAGES - 2>();
-          __syncthreads();      // the step's copies are there, and nobody reads the stage that is filled next
-          if (step + STAGES - 1 < steps) fill(step + STAGES - 1);
-          cp_commit();
-          const uint32_t src = ring + (step % STAGES) * STAGE, wsrc = src + DOWN_ROWS * DOWN_XROW;
-          uint32_t b[2][4];      // [8 rows][columns 0-7, 8-15, 16-23, 24-31 of this half]
-#pragma unroll
-          for (int j = 0; j < 2; ++j) ldmatrix4<false>(b[j], src + (tg * 16 + 8 * j + (lane & 7)) * DOWN_XROW + kh * 64 + 16 * (lane >> 3));
-#pragma unroll
-          for (int i = 0; i < RT; ++i)
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              uint32_t wa[4];
-              const int lo = (lane >> 3) & 1, hi = lane >> 4;
-              if constexpr (!DOWN_T) ldmatrix4<false>(wa, wsrc + (16 * i + 8 * lo + (lane & 7)) * WROW + kh * 64 + 32 * q + 16 * hi);
-              else ldmatrix4<true>(wa, wsrc + (kh * 32 + 16 * q + 8 * hi + (lane & 7)) * WROW + 32 * i + 16 * lo);
-#pragma unroll
-              for (int j = 0; j < 2; ++j) mma_bf16(acc[i][j], wa[0], wa[1], wa[2], wa[3], b[j][2 * q], b[j][2 * q + 1]);
-            }
-        }
-        cp_wait<0>();
-        __syncthreads();
-        auto each = [&](auto f) {
-#pragma unroll
-          for (int i = 0; i < RT; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) f(16 * tg + 8 * j + 2 * t4 + (e & 1), 16 * i + g + 8 * (e >> 1), acc[i][j][e]);
+          for (int q = 0; q < DOWN_K / 16; ++q)
+            umma_f16_ss(ring.tmem, umma_smem_desc_sw128(src + 32 * q, 16, 1024),
+                        umma_smem_desc_sw128(src + DOWN_X + (DOWN_T ? 2048 : 32) * q, DOWN_T ? 8192 : 16, 1024), idesc, step || q);
         };
-        if (kh == 1) each([&](int tok, int rank, float v) { red[tok * RSTRIDE + rank] = v; });
-        if (pending) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");      // every CTA has read the last parts
-        __syncthreads();
-        if (kh == 0) each([&](int tok, int rank, float v) { part[tok * 16 * RT + rank] = v + red[tok * RSTRIDE + rank]; });
+        ring_run(ring, steps, fill, feed);
+        __syncthreads();      // part takes the stages' place
+        if (w < 4) {
+          float* dst = part + (32 * w + lane) * pstride;
+          for (int r = 0; r < np; r += 16) {
+            uint32_t v[16];
+            tmem_ld_32x32b_x16(ring.tmem + (uint32_t(32 * w) << 16) + r, v);
+            tc_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 16; j += 4)
+              *reinterpret_cast<uint4*>(dst + r + j) = steps ? make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]) : make_uint4(0, 0, 0, 0);
+          }
+          tc_fence_before();
+        }
         cluster_sync_all();
+        tc_fence_after();
         // ---- each CTA adds up and writes its share
-        const int r16 = round16(a.up_seg[0].ru), lo = seg.u0 + r0, hi = min(lo + 16 * RT, seg.u0 + seg.ru);
+        const int r16 = round16(a.up_seg[0].ru), lo = seg.u0 + r0, hi = min(lo + np, seg.u0 + seg.ru);
         for (int e = c * LORA_THREADS + tid; e < m * a.ucols; e += C * LORA_THREADS) {
           const int tok = e / a.ucols, col = e - tok * a.ucols;
           const int p = a.up_segs > 1 ? col / r16 : 0, j = col - p * r16, rank = a.up_seg[p].u0 + j;
@@ -646,7 +695,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_down_kernel(const __grid
           if (pad ? sg > 0 || r0 > 0 : rank < lo || rank >= hi) continue;
           float v = 0.f;
           if (!pad) {
-            for (int k = 0; k < C; ++k) v += cluster.map_shared_rank(part, k)[tok * 16 * RT + rank - lo];
+            for (int k = 0; k < C; ++k) v += cluster.map_shared_rank(part, k)[tok * pstride + rank - lo];
             v *= s;
           }
           unsigned short* dst = a.u + (row0 + order[tok]) * a.ucols + col;
@@ -664,83 +713,76 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_down_kernel(const __grid
         }
         asm volatile("barrier.cluster.arrive.release;" ::: "memory");
         pending = true;
-        __syncthreads();
       }
     }
   }
   if (pending) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  ring_end(ring, 64);
 }
 
 // --------------------------------------------------------------------------------------------------- many rows: u onto y
-// A CTA takes 256 columns (32 per warp) of up to `look` rows. The weights of a warp's columns stay in registers for all rows of an
-// adapter (up to 16 KC ranks); what remains per 16 rows is to read u (from L2), y, and to write out. The next rows' y is asked for before
-// this one's is used.
+// A CTA takes 256 columns of one part (32 per warp) of up to `look` rows. The rows' u goes to shared memory once, the weights of a
+// warp's columns stay in registers for all rows of an adapter (up to 16 KC ranks); what remains per 16 rows is to read y, asked for two
+// turns ahead, and to write out.
+constexpr int UP_COLS = 32 * LORA_WARPS;
 template <typename TY, int KC, bool UP_T>
-__global__ void __launch_bounds__(LORA_THREADS, KC == 1 ? 3 : 2) lora_up_kernel(const __grid_constant__ LoraArgs a) {
+__global__ void __launch_bounds__(LORA_THREADS, 2) lora_up_kernel(const __grid_constant__ LoraArgs a) {
   constexpr int S = sizeof(TY) == 4 ? 3 : 2;
   __shared__ RowUnits units;
+  extern __shared__ __align__(16) uint8_t dyn[];
+  unsigned short* su = reinterpret_cast<unsigned short*>(dyn);      // [S][look][ustride], in the units' order
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t4 = lane & 3;
   const long long row0 = (long long)(blockIdx.x / a.groups) * a.look;
-  find_units(units, a, row0, (int)min((long long)a.look, a.T - row0), 16);
-  int p = 0, gi = (blockIdx.x % a.groups) * LORA_WARPS + w;
-  while (p < a.up_segs) {
-    const int have = (a.up_seg[p].c1 - a.up_seg[p].c0 + 31) / 32;
-    if (gi < have) break;
-    gi -= have;
-    ++p;
-  }
-  if (p >= a.up_segs) return;
+  int p = 0, tile = blockIdx.x % a.groups;
+  for (; tile >= (a.up_seg[p].c1 - a.up_seg[p].c0 + UP_COLS - 1) / UP_COLS; ++p) tile -= (a.up_seg[p].c1 - a.up_seg[p].c0 + UP_COLS - 1) / UP_COLS;
   const LoraSeg seg = a.up_seg[p];
-  const int n0 = seg.c0 + 32 * gi, col = n0 + 8 * t4, r16 = round16(seg.ru);
+  const int n0 = seg.c0 + tile * UP_COLS + 32 * w, col = n0 + 8 * t4, r16 = round16(seg.ru), ustride = u_stride(r16);
   const bool ok = col < seg.c1;
+  find_units(units, a, row0, (int)min((long long)a.look, a.T - row0), 16);
   const int total = units.total;
+  if (!total) return;
   const TY* y = reinterpret_cast<const TY*>(a.y) + col;
   TY* out = reinterpret_cast<TY*>(a.out) + col;
-  const unsigned short* us = a.u + p * r16 + 4 * t4;
   constexpr int W = sizeof(TY) / 2;      // 16-byte pieces of eight values
-  uint4 next[2][W];
+  uint4 ring[2][2][W];
   auto row_of = [&](int unit, int h) -> long long { return 8 * h + g < units.rows[unit] ? row0 + units.order[units.base[unit] + 8 * h + g] : -1; };
-  auto ask = [&](int unit) {
+  auto ask = [&](int unit, uint4 (&into)[2][W]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const long long row = row_of(unit, h);
+      const long long row = unit < total && a.y && ok ? row_of(unit, h) : -1;
 #pragma unroll
       for (int q = 0; q < W; ++q) {
-        next[h][q] = make_uint4(0, 0, 0, 0);
-        if (a.y && ok && row >= 0) next[h][q] = reinterpret_cast<const uint4*>(y + row * a.ldy)[q];
+        into[h][q] = make_uint4(0, 0, 0, 0);
+        if (row >= 0) into[h][q] = reinterpret_cast<const uint4*>(y + row * a.ldy)[q];
       }
     }
   };
-  if (total) ask(0);
+  {
+    const int places = units.base[total - 1] + units.rows[total - 1], per = r16 / 8;
+    for (int i = tid; i < S * places * per; i += LORA_THREADS) {
+      const int q = i % per, place = (i / per) % places, s = i / (per * places);
+      cp_async<16>(smem_u32(su + (s * a.look + place) * ustride + 8 * q),
+                   a.u + ((long long)s * a.T + row0 + units.order[place]) * a.ucols + p * r16 + 8 * q, true);
+    }
+    cp_commit();
+  }
+  ask(0, ring[0]);
+  ask(1, ring[1]);
+  cp_wait<0>();
+  __syncthreads();
   int have = -1;
   uint32_t wb[KC][4][1][2];
-  for (int unit = 0; unit < total; ++unit) {
-    const int ad = units.ad[unit];
+  auto turn_of = [&](int unit, uint4 (&yq)[2][W]) {
+    const int ad = units.ad[unit], base = units.base[unit];
     long long row[2];
     float yv[2][8];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       row[h] = row_of(unit, h);
-      unpack_row<TY>(next[h], yv[h]);
+      unpack_row<TY>(yq[h], yv[h]);
     }
+    ask(unit + 2, yq);
     if (ad >= 0) {
-      uint32_t ua[KC][S][4];
-      auto ask_u = [&](int kc0) {
-#pragma unroll
-        for (int i = 0; i < KC; ++i)
-#pragma unroll
-          for (int s = 0; s < S; ++s)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint2 v = make_uint2(0, 0);
-              if (row[h] >= 0 && kc0 + 16 * i < r16)
-                v = *reinterpret_cast<const uint2*>(us + ((long long)s * a.T + row[h]) * a.ucols + kc0 + 16 * i);
-              ua[i][s][h] = v.x;
-              ua[i][s][2 + h] = v.y;
-            }
-      };
-      ask_u(0);
-      if (unit + 1 < total) ask(unit + 1);
       const __nv_bfloat16* wu = reinterpret_cast<const __nv_bfloat16*>(a.up) + (long long)ad * a.up_adapter;
       float acc[4][4];
 #pragma unroll
@@ -753,22 +795,34 @@ __global__ void __launch_bounds__(LORA_THREADS, KC == 1 ? 3 : 2) lora_up_kernel(
           for (int i = 0; i < KC; ++i) load_up<__nv_bfloat16, UP_T, true>(wu, a.ld_up, n0, seg, kc0 + 16 * i, wb[i]);
           have = ad;
         }
-        if (kc0) ask_u(kc0);
 #pragma unroll
-        for (int i = 0; i < KC; ++i)
+        for (int i = 0; i < KC; ++i) {
+          if (kc0 + 16 * i >= r16) break;
+          uint32_t ua[S][4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) mma_parts<S, 1>(acc[j], ua[i], wb[i][j]);
+          for (int s = 0; s < S; ++s)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              // places behind the last row: whatever lies there goes into rows that are not written
+              const uint2 v = *reinterpret_cast<const uint2*>(su + (s * a.look + min(base + 8 * h + g, a.look - 1)) * ustride + kc0 + 16 * i + 4 * t4);
+              ua[s][h] = v.x;
+              ua[s][2 + h] = v.y;
+            }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mma_parts<S, 1>(acc[j], ua, wb[i][j]);
+        }
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) yv[e >> 1][2 * j + (e & 1)] += acc[j][e];
-    } else if (unit + 1 < total) {
-      ask(unit + 1);
     }
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      store_row<TY, true>(out + row[h] * a.ldo, ok && row[h] >= 0 ? 8 : 0, yv[h]);
+    for (int h = 0; h < 2; ++h) store_row<TY, true>(out + row[h] * a.ldo, ok && row[h] >= 0 ? 8 : 0, yv[h]);
+  };
+  for (int unit = 0; unit < total; unit += 2) {
+    turn_of(unit, ring[0]);
+    if (unit + 1 < total) turn_of(unit + 1, ring[1]);
   }
 }
 
@@ -804,6 +858,7 @@ struct GradJob {
 
 struct GradArgs {
   const int* index;
+  int* status;
   int T, n, jobs, out_f32, accumulate;
   GradJob job[LORA_SEGS + 1];
 };
@@ -955,96 +1010,71 @@ __global__ void __launch_bounds__(LORA_THREADS, 1) lora_grad_any_kernel(const __
   write_grad(cluster, a, t, tile, 16, ad);
 }
 
-// The same for bf16 rows that 16-byte copies fit: 32 rows at a time, z and both parts of p, go through a ring of shared-memory stages and enter
-// the products turned (`ldmatrix`). A warp takes 32 columns and all ranks. At rank 64 the products bound it, below the rows' traffic.
-constexpr int GRAD_ROWS = 32, GRAD_ZROW = GRAD_COLS * 2 + 16, GRAD_STAGES = 4;
-template <int RT> constexpr int GRAD_PROW = 32 * RT + 16;
-template <int RT> constexpr int GRAD_STAGE = GRAD_ROWS * (GRAD_ZROW + 2 * GRAD_PROW<RT>);
-template <int RT>
-__global__ void __launch_bounds__(LORA_THREADS, 2) lora_grad_kernel(const __grid_constant__ GradArgs a) {
-  constexpr int PROW = GRAD_PROW<RT>, STAGE = GRAD_STAGE<RT>;
+// The same for bf16 rows that 16-byte copies fit: 32 rows at a time through the ring. z's columns are the M side (128 at a time), both parts of
+// p side by side the N side, and the rows the inner index of the products; both operands lie along M and N.
+constexpr int GRAD_ROWS = 32, GRAD_Z = GRAD_ROWS * GRAD_COLS * 2, GRAD_BOX = GRAD_ROWS * 128;
+__host__ __device__ constexpr int grad_stage(int rp) { return GRAD_Z + (rp > 32 ? 2 : 1) * GRAD_BOX; }
+__global__ void __launch_bounds__(LORA_THREADS, 2) lora_grad_kernel(const __grid_constant__ GradArgs a, int rp) {
   __shared__ int s_rows[GRAD_LIST];
   __shared__ int s_scan[LORA_WARPS];
-  extern __shared__ __align__(16) uint8_t dyn[];
+  __shared__ RingShared shared;
+  extern __shared__ uint8_t raw[];
+  uint8_t* dyn = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), c = cluster.block_rank();
-  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t4 = lane & 3;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int ad = blockIdx.y;
-  const GradTile t = grad_tile(a, blockIdx.x / C, 16 * RT, C, c);
+  const GradTile t = grad_tile(a, blockIdx.x / C, rp, C, c);
   const GradJob& job = t.job;
   const __nv_bfloat16* z = reinterpret_cast<const __nv_bfloat16*>(job.z);
-  const uint32_t ring = smem_u32(dyn);
   const int r16 = round16(job.ru) - t.r0;      // ranks that p has from r0 on
-
-  float acc[RT][4][4];
-#pragma unroll
-  for (int i = 0; i < RT; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
+  const int tmem_cols = 4 * rp;
+  Ring ring = ring_start(shared, dyn, grad_stage(rp), tmem_cols, a.status);
+  const uint32_t idesc = umma_idesc_bf16(128, 2 * rp, 1, 1);
+  bool any = false;
   for (long long at = t.lo; at < t.hi; at += GRAD_LIST) {
     const int found = list_rows(a, ad, at, (int)min((long long)GRAD_LIST, t.hi - at), s_rows, s_scan);
-    const int steps = (found + GRAD_ROWS - 1) / GRAD_ROWS;
-    auto fill = [&](int step) {
-      const uint32_t dst = ring + (step % GRAD_STAGES) * STAGE;
+    auto row_of = [&](int k) -> long long { return k < found ? (a.index ? (long long)s_rows[k] : at + k) : 0; };
+    auto fill = [&](uint32_t dst, int step) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = (tid >> 5) + 8 * i, k = step * GRAD_ROWS + r, col = t.col0 + 8 * lane;
+      for (int i = 0; i < 4; ++i) {      // a warp copies whole rows
+        const int r = w + 8 * i, k = step * GRAD_ROWS + r, col = t.col0 + 8 * lane;
         const bool ok = k < found && col < job.c1;
-        const long long row = k < found ? (a.index ? (long long)s_rows[k] : at + k) : 0;
-        cp_async<16>(dst + r * GRAD_ZROW + 16 * lane, ok ? z + row * job.ldz + col : z, ok);
+        cp_async<16>(dst + (lane >> 3) * GRAD_BOX + r * 128 + 16 * ((lane & 7) ^ (r & 7)), ok ? z + row_of(k) * job.ldz + col : z, ok);
       }
-      for (int i = tid; i < 2 * GRAD_ROWS * 2 * RT; i += LORA_THREADS) {
-        const int q = i % (2 * RT), r = (i / (2 * RT)) % GRAD_ROWS, s = i / (2 * RT * GRAD_ROWS), k = step * GRAD_ROWS + r;
-        const bool ok = k < found && 8 * q < r16;
-        const long long row = k < found ? (a.index ? (long long)s_rows[k] : at + k) : 0;
-        cp_async<16>(dst + GRAD_ROWS * GRAD_ZROW + (s * GRAD_ROWS + r) * PROW + 16 * q,
-                     ok ? job.p + ((long long)s * a.T + row) * job.pcols + job.p0 + t.r0 + 8 * q : job.p, ok);
+      for (int i = tid; i < GRAD_ROWS * (rp / 4); i += LORA_THREADS) {
+        const int r = i / (rp / 4), q = i % (rp / 4), s = q / (rp / 8), j = q % (rp / 8), k = step * GRAD_ROWS + r;
+        const bool ok = k < found && 8 * j < r16;
+        cp_async<16>(dst + GRAD_Z + (q >> 3) * GRAD_BOX + r * 128 + 16 * ((q & 7) ^ (r & 7)),
+                     ok ? job.p + ((long long)s * a.T + row_of(k)) * job.pcols + job.p0 + t.r0 + 8 * j : job.p, ok);
       }
     };
+    const bool start = !any;
+    auto feed = [&](uint32_t src, int step) {
 #pragma unroll
-    for (int st = 0; st < GRAD_STAGES - 1; ++st) {
-      if (st < steps) fill(st);
-      cp_commit();
-    }
-    for (int step = 0; step < steps; ++step) {
-      cp_wait<GRAD_STAGES - 2>();
-      __syncthreads();
-      if (step + GRAD_STAGES - 1 < steps) fill(step + GRAD_STAGES - 1);
-      cp_commit();
-      const uint32_t src = ring + (step % GRAD_STAGES) * STAGE;
+      for (int q = 0; q < GRAD_ROWS / 16; ++q)
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        uint32_t b[2][4];
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          ldmatrix4<true>(b[j], src + (16 * k + 8 * ((lane >> 3) & 1) + (lane & 7)) * GRAD_ZROW + w * 64 + 32 * j + 16 * (lane >> 4));
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
-          if (16 * i >= r16) break;
-#pragma unroll
-          for (int s = 1; s >= 0; --s) {
-            uint32_t pa[4];
-            ldmatrix4<true>(pa, src + GRAD_ROWS * GRAD_ZROW + (s * GRAD_ROWS + 16 * k + 8 * (lane >> 4) + (lane & 7)) * PROW + 32 * i +
-                                    16 * ((lane >> 3) & 1));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) mma_bf16(acc[i][j], pa[0], pa[1], pa[2], pa[3], b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
-          }
-        }
-      }
-    }
-    cp_wait<0>();
-    __syncthreads();
+        for (int h = 0; h < 2; ++h)
+          umma_f16_ss(ring.tmem + 2 * rp * h, umma_smem_desc_sw128(src + 2 * h * GRAD_BOX + 2048 * q, GRAD_BOX, 1024),
+                      umma_smem_desc_sw128(src + GRAD_Z + 2048 * q, GRAD_BOX, 1024), idesc, !start || step || q);
+    };
+    const int steps = (found + GRAD_ROWS - 1) / GRAD_ROWS;
+    ring_run(ring, steps, fill, feed);
+    any = any || steps;
+    __syncthreads();      // the list makes way
   }
-  float* tile = reinterpret_cast<float*>(dyn);      // [16 RT][GRAD_STRIDE], where the stages were
+  float* tile = reinterpret_cast<float*>(dyn);      // [rp][GRAD_STRIDE], where the stages were
+  for (int r = 0; r < rp; r += 16) {
+    uint32_t hi[16], lo[16];
+    const uint32_t src = ring.tmem + (uint32_t(32 * (w & 3)) << 16) + 2 * rp * (w >> 2) + r;
+    tmem_ld_32x32b_x16(src, hi);
+    tmem_ld_32x32b_x16(src + rp, lo);
+    tc_wait_ld();
 #pragma unroll
-  for (int i = 0; i < RT; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) tile[(16 * i + g + 8 * (e >> 1)) * GRAD_STRIDE + w * 32 + 8 * j + 2 * t4 + (e & 1)] = acc[i][j][e];
-  write_grad(cluster, a, t, tile, 16 * RT, ad);
+    for (int j = 0; j < 16; ++j) tile[(r + j) * GRAD_STRIDE + 32 * w + lane] = any ? __uint_as_float(hi[j]) + __uint_as_float(lo[j]) : 0.f;
+  }
+  write_grad(cluster, a, t, tile, rp, ad);
+  ring_end(ring, tmem_cols);
 }
 
 bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
@@ -1141,43 +1171,39 @@ EDL_HOST_API int edl_lora_apply(const void* x, long long ldx, const void* y, lon
       ru = g.down_seg[i].ru > ru ? g.down_seg[i].ru : ru;
       cols = g.down_seg[i].c1 - g.down_seg[i].c0 > cols ? g.down_seg[i].c1 - g.down_seg[i].c0 : cols;
     }
-    // enough CTAs for two per SM, each with at least four steps of columns
+    const int np = ru < DOWN_RANKS ? round16(ru) : DOWN_RANKS;
+    // as many CTAs as run at once (two per SM), each with at least four steps of columns
     int cluster = 1;
-    while (cluster < 8 && (long long)((T + DOWN_ROWS - 1) / DOWN_ROWS) * cluster < 2 * sms && cols >= 2 * cluster * 4 * DOWN_K) cluster *= 2;
+    while (cluster < 8 && (long long)((T + DOWN_ROWS - 1) / DOWN_ROWS) * cluster * 2 <= 2 * sms && cols >= 2 * cluster * 4 * DOWN_K) cluster *= 2;
     const dim3 grid((unsigned)((long long)blocks * g.groups * cluster));
-#define EDL_LORA_DOWN(RTV)                                                                                                               \
-  {                                                                                                                                      \
-    if (backward ? launch_cluster(lora_down_kernel<RTV, true>, grid, cluster, DOWN_SMEM<RTV, true>, st, "lora down launch", g, s)        \
-                 : launch_cluster(lora_down_kernel<RTV, false>, grid, cluster, DOWN_SMEM<RTV, false>, st, "lora down launch", g, s))     \
-      return -1;                                                                                                                         \
-  }
-    if (ru <= 16) EDL_LORA_DOWN(1)
-    else if (ru <= 32) EDL_LORA_DOWN(2)
-    else EDL_LORA_DOWN(4)
-#undef EDL_LORA_DOWN
+    const int ring = RING_STAGES * down_stage(np, backward), part = DOWN_ROWS * (np + 4) * 4, down_smem = (ring > part ? ring : part) + 1024;
+    if (backward ? launch_cluster(lora_down_kernel<true>, grid, cluster, down_smem, st, "lora down launch", g, s, np)
+                 : launch_cluster(lora_down_kernel<false>, grid, cluster, down_smem, st, "lora down launch", g, s, np))
+      return -1;
     if (!out) return 0;
-    int tiles = 0;
-    for (int i = 0; i < g.up_segs; ++i) tiles += (g.up_seg[i].c1 - g.up_seg[i].c0 + 31) / 32;
-    g.groups = (tiles + LORA_WARPS - 1) / LORA_WARPS;
-    g.look = LORA_ROWS;
-    while (g.look > 64 && (long long)g.groups * ((T + g.look - 1) / g.look) < 6LL * sms) g.look /= 2;
+    g.groups = 0;
+    for (int i = 0; i < g.up_segs; ++i) g.groups += (g.up_seg[i].c1 - g.up_seg[i].c0 + UP_COLS - 1) / UP_COLS;
+    const int r16 = round16(g.up_seg[0].ru), row_bytes = s * u_stride(r16) * 2;
+    g.look = LORA_ROWS;      // fewer rows per CTA where their u takes much shared memory, or where there are few CTAs
+    while (g.look > 16 && (g.look * row_bytes > 48 * 1024 || (g.look > 64 && (long long)g.groups * ((T + g.look - 1) / g.look) < 4LL * sms))) g.look /= 2;
     const long long ctas = (long long)g.groups * (((long long)T + g.look - 1) / g.look);
     if (ctas > 0x7fffffffLL) {
       set_last_error("edl_lora_apply: too many rows for one launch");
       return -1;
     }
-    const int kc = round16(g.up_seg[0].ru) / 16;
-#define EDL_LORA_UP(TO, BW)                                                              \
-  {                                                                                      \
-    if (kc == 1) lora_up_kernel<TO, 1, BW><<<(unsigned)ctas, LORA_THREADS, 0, st>>>(g);  \
-    else if (kc == 2) lora_up_kernel<TO, 2, BW><<<(unsigned)ctas, LORA_THREADS, 0, st>>>(g); \
-    else lora_up_kernel<TO, 4, BW><<<(unsigned)ctas, LORA_THREADS, 0, st>>>(g);          \
+    const int kc = r16 / 16;
+#define EDL_LORA_UP(TO, BW)                                                                                                      \
+  {                                                                                                                              \
+    const dim3 up((unsigned)ctas);                                                                                               \
+    const int smem = g.look * row_bytes;                                                                                         \
+    if (kc == 1) return launch_cluster(lora_up_kernel<TO, 1, BW>, up, 1, smem, st, "lora up launch", g);                         \
+    if (kc == 2) return launch_cluster(lora_up_kernel<TO, 2, BW>, up, 1, smem, st, "lora up launch", g);                         \
+    return launch_cluster(lora_up_kernel<TO, 4, BW>, up, 1, smem, st, "lora up launch", g);                                      \
   }
     if (backward) EDL_LORA_UP(__nv_bfloat16, true)
-    else if (y_f32) EDL_LORA_UP(float, false)
-    else EDL_LORA_UP(__nv_bfloat16, false)
+    if (y_f32) EDL_LORA_UP(float, false)
+    EDL_LORA_UP(__nv_bfloat16, false)
 #undef EDL_LORA_UP
-    return check_cuda(cudaGetLastError(), "lora up launch");
   }
 
   const int ranks = backward ? r : parts * r;      // that one pass over x can take
@@ -1219,7 +1245,7 @@ EDL_HOST_API int edl_lora_apply(const void* x, long long ldx, const void* y, lon
 EDL_HOST_API int edl_lora_grads(const void* x, long long ldx, const void* dy, long long ldy, const void* g, const void* u,
                                 const int* index, void* da, long long da_adapter, long long ld_da, void* db, long long db_adapter,
                                 long long ld_db, int T, int K, int N, int n, int r, int parts, const int* widths, int in_f32,
-                                int out_f32, int accumulate, void* stream) {
+                                int out_f32, int accumulate, int* status, void* stream) {
   if (K <= 0 || N <= 0 || n <= 0 || r <= 0 || parts < 1 || parts > LORA_SEGS || r > 512 / parts || n > 65535 || (!index && n != 1 && T > 0)) {
     set_last_error("edl_lora_grads: needs sizes above 0, up to %d parts, parts x rank up to 512, up to 65535 adapters, one without an index", LORA_SEGS);
     return -1;
@@ -1229,7 +1255,7 @@ EDL_HOST_API int edl_lora_grads(const void* x, long long ldx, const void* dy, lo
     return -1;
   }
   GradArgs a{};
-  a.index = index; a.T = T < 0 ? 0 : T; a.n = n; a.out_f32 = out_f32; a.accumulate = accumulate;
+  a.index = index; a.status = status; a.T = T < 0 ? 0 : T; a.n = n; a.out_f32 = out_f32; a.accumulate = accumulate;
   const int va = in_f32 ? 4 : 8;
   bool wide = true;
   int most = 0;
@@ -1255,11 +1281,11 @@ EDL_HOST_API int edl_lora_grads(const void* x, long long ldx, const void* dy, lo
   }
   if (!a.jobs) return 0;
   const bool fast = wide && !in_f32;
-  const int rt = !fast || most <= 16 ? 1 : most <= 32 ? 2 : 4;
+  const int rp = !fast || most <= 16 ? 16 : most <= 32 ? 32 : 64;      // ranks of a pass over the rows
   int tiles = 0;
   for (int j = 0; j < a.jobs; ++j) {
     GradJob& job = a.job[j];
-    job.tiles = ((job.c1 - job.c0 + GRAD_COLS - 1) / GRAD_COLS) * ((job.ru + 16 * rt - 1) / (16 * rt));
+    job.tiles = ((job.c1 - job.c0 + GRAD_COLS - 1) / GRAD_COLS) * ((job.ru + rp - 1) / rp);
     tiles += job.tiles;
   }
   int cluster = 8;      // rows are cut into as many shares; short inputs need fewer
@@ -1268,10 +1294,8 @@ EDL_HOST_API int edl_lora_grads(const void* x, long long ldx, const void* dy, lo
   const dim3 grid((unsigned)(tiles * cluster), (unsigned)n);
   const char* what = "lora gradient launch";
   if (fast) {
-    auto smem = [](int ring, int ranks) { const int t = ranks * GRAD_STRIDE * 4; return ring > t ? ring : t; };
-    if (rt == 1) return launch_cluster(lora_grad_kernel<1>, grid, cluster, smem(GRAD_STAGES * GRAD_STAGE<1>, 16), st, what, a);
-    if (rt == 2) return launch_cluster(lora_grad_kernel<2>, grid, cluster, smem(GRAD_STAGES * GRAD_STAGE<2>, 32), st, what, a);
-    return launch_cluster(lora_grad_kernel<4>, grid, cluster, smem(GRAD_STAGES * GRAD_STAGE<4>, 64), st, what, a);
+    const int ring = RING_STAGES * grad_stage(rp), tile = rp * GRAD_STRIDE * 4;
+    return launch_cluster(lora_grad_kernel, grid, cluster, (ring > tile ? ring : tile) + 1024, st, what, a, rp);
   }
   const int smem = 16 * GRAD_STRIDE * 4;
   if (in_f32) return wide ? launch_cluster(lora_grad_any_kernel<float, 3, true>, grid, cluster, smem, st, what, a)

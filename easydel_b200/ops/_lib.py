@@ -9,7 +9,6 @@ callers use the fp32 reference math in :mod:`easydel_b200.ops.reference`.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import os
 import threading
@@ -137,11 +136,13 @@ def stream_ptr() -> int:
     return _raw_stream(_device_index())
 
 
-def on_device(device: torch.device):
-    """Launches go to a stream of the current device: makes ``device`` the current one where it is not."""
-    if device.index in (None, torch.cuda.current_device()):
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def call_on(device: torch.device, name: str, *args) -> None:
+    """:func:`call` on ``device``'s current stream, which is the launcher's last argument, whichever device is the current one."""
+    if _device_index is not None and device.index == _device_index():
+        call(name, *args, stream_ptr())
+        return
+    with torch.cuda.device(device):
+        call(name, *args, stream_ptr())
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

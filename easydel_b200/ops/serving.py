@@ -432,32 +432,44 @@ def adjust_logits(logits: torch.Tensor, *, counts: torch.Tensor | None = None, c
     R_, V = logits.shape
     ptr, ids, values = bias if bias is not None else (None, None, None)
     bits, mask_rows = mask if mask is not None else (None, None)
-    for name, t, dtype, shape in (("count_rows", count_rows, torch.int32, (R_,)), ("presence", presence, torch.float32, (R_,)),
-                                  ("frequency", frequency, torch.float32, (R_,)), ("repetition", repetition, torch.float32, (R_,)),
-                                  ("bias ptr", ptr, torch.int32, (R_ + 1,)), ("bias ids", ids, torch.int32, None),
-                                  ("bias values", values, torch.float32, None if ids is None else tuple(ids.shape)),
-                                  ("mask rows", mask_rows, torch.int32, (R_,))):
-        if t is None:
-            if name.startswith("bias") and bias is not None:
-                raise ValueError("bias is (ptr, ids, values)")
-            continue
-        if t.dtype != dtype or t.dim() != 1 or not t.is_contiguous() or (shape is not None and tuple(t.shape) != shape):
-            raise ValueError(f"{name} is a contiguous {dtype} tensor of shape {shape or '[entries]'}, got {tuple(t.shape)} of {t.dtype}")
+    dev, f32_, i32_ = logits.device, torch.float32, torch.int32
+
+    def vector(t, name, dtype, n):
+        if t.dtype != dtype or t.dim() != 1 or (n >= 0 and t.shape[0] != n) or not t.is_contiguous() or t.device != dev:
+            raise ValueError(f"{name} is a contiguous {dtype} tensor of {n if n >= 0 else 'all'} entries on {dev}, got {tuple(t.shape)} "
+                             f"of {t.dtype} on {t.device}")
+
+    if presence is not None:
+        vector(presence, "presence", f32_, R_)
+    if frequency is not None:
+        vector(frequency, "frequency", f32_, R_)
+    if repetition is not None:
+        vector(repetition, "repetition", f32_, R_)
     if counts is None:
         if count_rows is not None:
             raise ValueError("count_rows without counts")
-    elif counts.dim() != 2 or counts.dtype != torch.int32 or counts.shape[1] < V or (V > 1 and counts.stride(1) != 1) or \
-            (count_rows is None and counts.shape[0] < R_):
-        raise ValueError(f"counts are int32 rows of at least {V} tokens, one for each row without count_rows, got {tuple(counts.shape)} "
-                         f"of {counts.dtype}")
-    if mask is not None and (bits.dim() != 2 or bits.dtype != torch.int32 or bits.shape[1] < (V + 31) // 32 or
-                             (bits.shape[1] > 1 and bits.stride(1) != 1) or (mask_rows is None and bits.shape[0] < R_)):
-        raise ValueError(f"masks are int32 rows of at least {(V + 31) // 32} words, got {tuple(bits.shape)} of {bits.dtype}")
-    if out is not None and (out.shape != logits.shape or out.dtype not in (torch.bfloat16, torch.float32)):
-        raise ValueError(f"out is {tuple(out.shape)} of {out.dtype}, logits {tuple(logits.shape)}")
-    for t in (counts, count_rows, presence, frequency, repetition, ptr, ids, values, bits, mask_rows, out):
-        if t is not None and t.device != logits.device:
-            raise ValueError(f"tensors on {logits.device} and {t.device}")
+    else:
+        if count_rows is not None:
+            vector(count_rows, "count_rows", i32_, R_)
+        if counts.dim() != 2 or counts.dtype != i32_ or counts.shape[1] < V or (V > 1 and counts.stride(1) != 1) or \
+                (count_rows is None and counts.shape[0] < R_) or counts.device != dev:
+            raise ValueError(f"counts are int32 rows of at least {V} tokens on {dev}, one for each row without count_rows, got "
+                             f"{tuple(counts.shape)} of {counts.dtype} on {counts.device}")
+    if bias is not None:
+        if ptr is None or ids is None or values is None:
+            raise ValueError("bias is (ptr, ids, values)")
+        vector(ptr, "bias ptr", i32_, R_ + 1)
+        vector(ids, "bias ids", i32_, -1)
+        vector(values, "bias values", f32_, ids.shape[0])
+    if mask is not None:
+        if mask_rows is not None:
+            vector(mask_rows, "mask rows", i32_, R_)
+        if bits.dim() != 2 or bits.dtype != i32_ or bits.shape[1] < (V + 31) // 32 or (bits.shape[1] > 1 and bits.stride(1) != 1) or \
+                (mask_rows is None and bits.shape[0] < R_) or bits.device != dev:
+            raise ValueError(f"masks are int32 rows of at least {(V + 31) // 32} words on {dev}, got {tuple(bits.shape)} of {bits.dtype} on "
+                             f"{bits.device}")
+    if out is not None and (out.shape != logits.shape or out.dtype not in (torch.bfloat16, f32_) or out.device != dev):
+        raise ValueError(f"out is {tuple(out.shape)} of {out.dtype} on {out.device}, logits {tuple(logits.shape)} on {dev}")
     if not logits.is_cuda:
         z = adjust_logits_reference(logits, counts, count_rows, presence, frequency, repetition, bias, mask)
         return z if out is None else out.copy_(z)
@@ -471,13 +483,12 @@ def adjust_logits(logits: torch.Tensor, *, counts: torch.Tensor | None = None, c
     elif V > 1 and out.stride(1) != 1:
         return out.copy_(adjust_logits(logits, counts=counts, count_rows=count_rows, presence=presence, frequency=frequency,
                                        repetition=repetition, bias=bias, mask=mask))
-    with _lib.on_device(logits.device):
-        _lib.call("edl_adjust_logits", logits.data_ptr(), int(logits.dtype == torch.float32), logits.stride(0), out.data_ptr(),
-                  int(out.dtype == torch.float32), out.stride(0), R_, V, _lib.ptr(counts), 0 if counts is None else counts.stride(0),
-                  0 if counts is None else counts.shape[0], _lib.ptr(count_rows), _lib.ptr(presence), _lib.ptr(frequency),
-                  _lib.ptr(repetition), _lib.ptr(ptr), _lib.ptr(ids), _lib.ptr(values), 0 if ids is None else ids.numel(),
-                  _lib.ptr(bits), 0 if bits is None else bits.stride(0), 0 if bits is None else bits.shape[0], _lib.ptr(mask_rows),
-                  _lib.status_word(logits.device).data_ptr(), _lib.stream_ptr())
+    _lib.call_on(logits.device, "edl_adjust_logits", logits.data_ptr(), logits.dtype == torch.float32, logits.stride(0), out.data_ptr(),
+                 out.dtype == torch.float32, out.stride(0), R_, V, _lib.ptr(counts), 0 if counts is None else counts.stride(0),
+                 0 if counts is None else counts.shape[0], _lib.ptr(count_rows), _lib.ptr(presence), _lib.ptr(frequency),
+                 _lib.ptr(repetition), _lib.ptr(ptr), _lib.ptr(ids), _lib.ptr(values), 0 if ids is None else ids.numel(),
+                 _lib.ptr(bits), 0 if bits is None else bits.stride(0), 0 if bits is None else bits.shape[0], _lib.ptr(mask_rows),
+                 _lib.status_word(logits.device).data_ptr())
     return out
 
 
