@@ -46,6 +46,14 @@ static CUtensorMapSwizzle swz(int s) {
   }
 }
 
+// The driver encodes tensor maps only for a thread with a current context. A thread that has called nothing but this library (autograd's
+// in a first backward pass) has none yet: naming its device makes one current.
+static void bind_context() {
+  static thread_local int bound = -1;
+  int dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev != bound && cudaSetDevice(dev) == cudaSuccess) bound = dev;
+}
+
 int make_tmap_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows,
                  uint32_t box_cols, int elem_bytes, int swizzle) {
   auto fn = encode_fn();
@@ -57,6 +65,7 @@ int make_tmap_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t col
     set_last_error("tensor map: base %p / leading dimension %llu not 16-byte aligned", base, (unsigned long long)ld);
     return -1;
   }
+  bind_context();
   cuuint64_t dims[2] = {cols, rows};
   cuuint64_t strides[1] = {ld * (uint64_t)elem_bytes};
   cuuint32_t box[2] = {box_cols, box_rows};
@@ -88,6 +97,7 @@ int make_tmap_3d_16b(CUtensorMap* map, const void* base, uint64_t d0, uint64_t d
     set_last_error("tensor map 3d: base/strides not 16-byte aligned");
     return -1;
   }
+  bind_context();
   cuuint64_t dims[3] = {d0, d1, d2};
   cuuint64_t strides[2] = {stride1 * 2, stride2 * 2};
   cuuint32_t box[3] = {box0, box1, box2};

@@ -526,25 +526,38 @@ __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// A ring of shared-memory stages that all threads fill with `cp.async` (rows may be gathered; 128-byte rows, their 16-byte pieces swizzled as
-// the tensor cores read them) and one lane feeds to `tcgen05.mma`. A stage is filled again once its products are done.
+// A ring of shared-memory stages (rows of 128 bytes, swizzled) that one lane feeds to `tcgen05.mma`. Rows that lie one after the other in
+// memory come by TMA; others are gathered by all threads with `cp.async`, which costs instructions for every piece. A stage is filled
+// again once its products are done.
 constexpr int RING_STAGES = 4;
 struct Ring {
-  uint32_t base, bars, tmem;      // stages; "products of this stage are done" barriers, then "all done"; accumulators
-  int bytes, used, passes;        // of a stage; stages fed so far; passes finished
+  uint32_t base, done, all, full, tmem;      // stages; barriers: a stage's products, all products, a stage's copies; accumulators
+  int bytes, used, passes;                   // of a stage; stages fed so far; passes finished
   volatile int* abort_flag;
   int* status;
-  __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity) { mbar_wait(bar, parity, abort_flag, status, EDL_TIMEOUT_MMA); }
+  __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, int code) { mbar_wait(bar, parity, abort_flag, status, code); }
+  __device__ __forceinline__ int at(int step) const { return (used + step) % RING_STAGES; }
+  // until the stage that `step` takes is free
+  __device__ __forceinline__ uint32_t free_stage(int step) {
+    const int use = used + step;
+    if (use >= RING_STAGES) wait(done + 8 * at(step), (use / RING_STAGES - 1) & 1, EDL_TIMEOUT_PRODUCER);
+    return base + at(step) * bytes;
+  }
+  __device__ __forceinline__ void finish(int steps) {
+    used += steps;
+    wait(all, passes++ & 1, EDL_TIMEOUT_MMA);
+    tc_fence_after();
+  }
 };
 struct RingShared {
-  uint64_t bars[RING_STAGES + 1];
+  uint64_t bars[2 * RING_STAGES + 1];
   uint32_t tmem;
   int abort_flag;
 };
 // All threads. Waits that run out leave their code in the status word; everything after them goes on, without meaning.
 __device__ __forceinline__ Ring ring_start(RingShared& sh, const uint8_t* stages, int bytes, int tmem_cols, int* status) {
   if (threadIdx.x == 0) {
-    for (int i = 0; i <= RING_STAGES; ++i) mbar_init(smem_u32(&sh.bars[i]), 1);
+    for (int i = 0; i <= 2 * RING_STAGES; ++i) mbar_init(smem_u32(&sh.bars[i]), 1);
     sh.abort_flag = 0;
     fence_mbar_init();
   }
@@ -555,21 +568,17 @@ __device__ __forceinline__ Ring ring_start(RingShared& sh, const uint8_t* stages
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  return Ring{smem_u32(stages), smem_u32(sh.bars), sh.tmem, bytes, 0, 0, &sh.abort_flag, status};
+  const uint32_t bars = smem_u32(sh.bars);
+  return Ring{smem_u32(stages), bars, bars + 8 * RING_STAGES, bars + 8 * (RING_STAGES + 1), sh.tmem, bytes, 0, 0, &sh.abort_flag, status};
 }
-// `fill(stage address, step)` copies, `feed(stage address, step)` issues the products (called by one lane of warp 0). Returns once all
-// products are done and visible in tensor memory.
+// Both return once all products are done and visible in tensor memory. `feed(stage address, step)` issues a stage's products (one lane).
+// `fill(stage address, step)`: every thread copies its share.
 template <typename Fill, typename Feed>
-__device__ __forceinline__ void ring_run(Ring& r, int steps, Fill fill, Feed feed) {
+__device__ __forceinline__ void ring_gather(Ring& r, int steps, Fill fill, Feed feed) {
   if (!steps) return;
-  auto put = [&](int step) {
-    const int use = r.used + step, at = use % RING_STAGES;
-    if (use >= RING_STAGES) r.wait(r.bars + 8 * at, (use / RING_STAGES - 1) & 1);
-    fill(r.base + at * r.bytes, step);
-  };
 #pragma unroll
   for (int i = 0; i < RING_STAGES - 1; ++i) {
-    if (i < steps) put(i);
+    if (i < steps) fill(r.free_stage(i), i);
     cp_commit();
   }
   for (int step = 0; step < steps; ++step) {
@@ -580,20 +589,49 @@ __device__ __forceinline__ void ring_run(Ring& r, int steps, Fill fill, Feed fee
       const bool leader = elect_one();
       tc_fence_after();
       if (leader) {
-        const int at = (r.used + step) % RING_STAGES;
-        feed(r.base + at * r.bytes, step);
-        tc_commit(r.bars + 8 * at);
-        if (step == steps - 1) tc_commit(r.bars + 8 * RING_STAGES);
+        feed(r.base + r.at(step) * r.bytes, step);
+        tc_commit(r.done + 8 * r.at(step));
+        mbar_arrive(r.full + 8 * r.at(step));      // keeps step with the copies by TMA
+        if (step == steps - 1) tc_commit(r.all);
       }
       __syncwarp();
     }
-    if (step + RING_STAGES - 1 < steps) put(step + RING_STAGES - 1);
+    if (step + RING_STAGES - 1 < steps) fill(r.free_stage(step + RING_STAGES - 1), step + RING_STAGES - 1);
     cp_commit();
   }
-  r.used += steps;
-  r.wait(r.bars + 8 * RING_STAGES, r.passes++ & 1);
   cp_wait<0>();
-  tc_fence_after();
+  r.finish(steps);
+}
+// `load(stage address, barrier, step)`: one lane of warp 0 issues copies of `bytes` bytes.
+template <typename Load, typename Feed>
+__device__ __forceinline__ void ring_tma(Ring& r, int steps, int bytes, Load load, Feed feed) {
+  if (!steps) return;
+  fence_proxy_async_smem();      // what lay in the stages before
+  __syncthreads();
+  const int w = threadIdx.x >> 5;
+  if (w == 0) {
+    if (elect_one()) {
+      for (int step = 0; step < steps; ++step) {
+        const uint32_t dst = r.free_stage(step), bar = r.full + 8 * r.at(step);
+        mbar_expect_tx(bar, bytes);
+        load(dst, bar, step);
+      }
+    }
+    __syncwarp();
+  } else if (w == 1) {
+    const bool leader = elect_one();
+    for (int step = 0; step < steps; ++step) {
+      r.wait(r.full + 8 * r.at(step), ((r.used + step) / RING_STAGES) & 1, EDL_TIMEOUT_MMA);
+      tc_fence_after();
+      if (leader) {
+        feed(r.base + r.at(step) * r.bytes, step);
+        tc_commit(r.done + 8 * r.at(step));
+        if (step == steps - 1) tc_commit(r.all);
+      }
+    }
+    __syncwarp();
+  }
+  r.finish(steps);
 }
 __device__ __forceinline__ void ring_end(Ring& r, int tmem_cols) {
   tc_fence_before();
@@ -607,7 +645,8 @@ constexpr int DOWN_ROWS = 128, DOWN_K = 64, DOWN_X = DOWN_ROWS * DOWN_K * 2, DOW
 __host__ __device__ constexpr int down_stage(int np, bool down_t) { return DOWN_X + (down_t ? DOWN_K : np) * 128; }
 
 template <bool DOWN_T>
-__global__ void __launch_bounds__(LORA_THREADS, 2) lora_down_kernel(const __grid_constant__ LoraArgs a, int parts, int np) {
+__global__ void __launch_bounds__(LORA_THREADS, 2) lora_down_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ CUtensorMap map_x,
+                                                                  const __grid_constant__ CUtensorMap map_w, int tma, int parts, int np) {
   __shared__ RowUnits units;
   __shared__ RingShared shared;
   extern __shared__ uint8_t raw[];
@@ -670,7 +709,18 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_down_kernel(const __grid
             umma_f16_ss(ring.tmem, umma_smem_desc_sw128(src + 32 * q, 16, 1024),
                         umma_smem_desc_sw128(src + DOWN_X + (DOWN_T ? 2048 : 32) * q, DOWN_T ? 8192 : 16, 1024), idesc, step || q);
         };
-        ring_run(ring, steps, fill, feed);
+        if (tma && order[m - 1] - order[0] == m - 1) {      // rows behind the unit's come along and are not looked at
+          const int at_row = (int)row0 + order[0];
+          auto load = [&](uint32_t dst, uint32_t bar, int step) {
+            const int k = k0 + step * DOWN_K;
+            tma_load_2d(dst, &map_x, bar, k, at_row);
+            if constexpr (!DOWN_T) tma_load_3d(dst + DOWN_X, &map_w, bar, k, seg.u0 + r0, ad);
+            else tma_load_3d(dst + DOWN_X, &map_w, bar, r0, k, ad);
+          };
+          ring_tma(ring, steps, down_stage(np, DOWN_T), load, feed);
+        } else {
+          ring_gather(ring, steps, fill, feed);
+        }
         __syncthreads();      // part takes the stages' place
         if (w < 4) {
           float* dst = part + (32 * w + lane) * pstride;
@@ -745,15 +795,18 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_up_kernel(const __grid_c
   TY* out = reinterpret_cast<TY*>(a.out) + col;
   constexpr int W = sizeof(TY) / 2;      // 16-byte pieces of eight values
   uint4 ring[2][2][W];
-  auto row_of = [&](int unit, int h) -> long long { return 8 * h + g < units.rows[unit] ? row0 + units.order[units.base[unit] + 8 * h + g] : -1; };
-  auto ask = [&](int unit, uint4 (&into)[2][W]) {
+  long long rows[2][2];      // of the units asked for
+  auto ask = [&](int unit, uint4 (&into)[2][W], long long (&row)[2]) {
+    const int m = unit < total ? units.rows[unit] : 0;
+    const short* order = units.order + (m ? units.base[unit] : 0);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const long long row = unit < total && a.y && ok ? row_of(unit, h) : -1;
+      row[h] = 8 * h + g < m ? row0 + order[8 * h + g] : -1;
+      const bool read = a.y && ok && row[h] >= 0;
 #pragma unroll
       for (int q = 0; q < W; ++q) {
         into[h][q] = make_uint4(0, 0, 0, 0);
-        if (row >= 0) into[h][q] = reinterpret_cast<const uint4*>(y + row * a.ldy)[q];
+        if (read) into[h][q] = reinterpret_cast<const uint4*>(y + row[h] * a.ldy)[q];
       }
     }
   };
@@ -766,63 +819,62 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_up_kernel(const __grid_c
     }
     cp_commit();
   }
-  ask(0, ring[0]);
-  ask(1, ring[1]);
+  ask(0, ring[0], rows[0]);
+  ask(1, ring[1], rows[1]);
   cp_wait<0>();
   __syncthreads();
   int have = -1;
   uint32_t wb[KC][4][1][2];
-  auto turn_of = [&](int unit, uint4 (&yq)[2][W]) {
+  auto turn_of = [&](int unit, uint4 (&yq)[2][W], long long (&row)[2]) {
     const int ad = units.ad[unit], base = units.base[unit];
-    long long row[2];
-    float yv[2][8];
+    // [column tile][row half, column]: y and what is added to it. The tensor cores cut sums off, so 32-bit results add y to the sum of products.
+    float acc[4][4], yv[2][8];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      row[h] = row_of(unit, h);
       unpack_row<TY>(yq[h], yv[h]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e >> 1][2 * h + (e & 1)] = S == 3 ? 0.f : yv[h][e];
     }
-    ask(unit + 2, yq);
+    TY* dst[2] = {row[0] >= 0 ? out + row[0] * a.ldo : nullptr, row[1] >= 0 ? out + row[1] * a.ldo : nullptr};
+    ask(unit + 2, yq, row);
     if (ad >= 0) {
-      const __nv_bfloat16* wu = reinterpret_cast<const __nv_bfloat16*>(a.up) + (long long)ad * a.up_adapter;
-      float acc[4][4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
+      // places behind the unit's rows: whatever lies there goes into rows that are not written
+      const unsigned short* su0 = su + min(base + g, a.look - 1) * ustride + 4 * t4;
+      const unsigned short* su1 = su + min(base + 8 + g, a.look - 1) * ustride + 4 * t4;
       for (int kc0 = 0; kc0 < r16; kc0 += 16 * KC) {
         if (ad != have || r16 > 16 * KC) {
+          const __nv_bfloat16* wu = reinterpret_cast<const __nv_bfloat16*>(a.up) + (long long)ad * a.up_adapter;
 #pragma unroll
           for (int i = 0; i < KC; ++i) load_up<__nv_bfloat16, UP_T, true>(wu, a.ld_up, n0, seg, kc0 + 16 * i, wb[i]);
           have = ad;
         }
 #pragma unroll
         for (int i = 0; i < KC; ++i) {
-          if (kc0 + 16 * i >= r16) break;
+          if (KC > 1 && kc0 + 16 * i >= r16) break;
           uint32_t ua[S][4];
 #pragma unroll
-          for (int s = 0; s < S; ++s)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              // places behind the last row: whatever lies there goes into rows that are not written
-              const uint2 v = *reinterpret_cast<const uint2*>(su + (s * a.look + min(base + 8 * h + g, a.look - 1)) * ustride + kc0 + 16 * i + 4 * t4);
-              ua[s][h] = v.x;
-              ua[s][2 + h] = v.y;
-            }
+          for (int s = 0; s < S; ++s) {
+            const int at = s * a.look * ustride + kc0 + 16 * i;
+            const uint2 v0 = *reinterpret_cast<const uint2*>(su0 + at), v1 = *reinterpret_cast<const uint2*>(su1 + at);
+            ua[s][0] = v0.x; ua[s][1] = v1.x;
+            ua[s][2] = v0.y; ua[s][3] = v1.y;
+          }
 #pragma unroll
           for (int j = 0; j < 4; ++j) mma_parts<S, 1>(acc[j], ua, wb[i][j]);
         }
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) yv[e >> 1][2 * j + (e & 1)] += acc[j][e];
     }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) store_row<TY, true>(out + row[h] * a.ldo, ok && row[h] >= 0 ? 8 : 0, yv[h]);
+    for (int h = 0; h < 2; ++h) {
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = acc[e >> 1][2 * h + (e & 1)] + (S == 3 ? yv[h][e] : 0.f);
+      store_row<TY, true>(dst[h], ok && dst[h] ? 8 : 0, v);
+    }
   };
   for (int unit = 0; unit < total; unit += 2) {
-    turn_of(unit, ring[0]);
-    if (unit + 1 < total) turn_of(unit + 1, ring[1]);
+    turn_of(unit, ring[0], rows[0]);
+    if (unit + 1 < total) turn_of(unit + 1, ring[1], rows[1]);
   }
 }
 
@@ -897,7 +949,7 @@ __device__ __forceinline__ GradTile grad_tile(const GradArgs& a, int tile, int r
   const int passes = (t.job.ru + ranks - 1) / ranks;
   t.r0 = (tile % passes) * ranks;
   t.col0 = t.job.c0 + (tile / passes) * GRAD_COLS;
-  const long long per = (((long long)a.T + C - 1) / C + 15) / 16 * 16;
+  const long long per = (((long long)a.T + C - 1) / C + 31) / 32 * 32;
   t.lo = min((long long)a.T, per * c);
   t.hi = min((long long)a.T, t.lo + per);
   return t;
@@ -1012,9 +1064,12 @@ __global__ void __launch_bounds__(LORA_THREADS, 1) lora_grad_any_kernel(const __
 
 // The same for bf16 rows that 16-byte copies fit: 32 rows at a time through the ring. z's columns are the M side (128 at a time), both parts of
 // p side by side the N side, and the rows the inner index of the products; both operands lie along M and N.
-constexpr int GRAD_ROWS = 32, GRAD_Z = GRAD_ROWS * GRAD_COLS * 2, GRAD_BOX = GRAD_ROWS * 128;
-__host__ __device__ constexpr int grad_stage(int rp) { return GRAD_Z + (rp > 32 ? 2 : 1) * GRAD_BOX; }
-__global__ void __launch_bounds__(LORA_THREADS, 2) lora_grad_kernel(const __grid_constant__ GradArgs a, int rp) {
+constexpr int GRAD_ROWS = 32, GRAD_Z = GRAD_ROWS * GRAD_COLS * 2, GRAD_BOX = GRAD_ROWS * 128, GRAD_STAGE = GRAD_Z + 2 * GRAD_BOX;
+struct GradMaps {
+  CUtensorMap z[2], p[2];      // of dA's and dB's inputs
+};
+__global__ void __launch_bounds__(LORA_THREADS, 2) lora_grad_kernel(const __grid_constant__ GradArgs a, const __grid_constant__ GradMaps maps,
+                                                                    int rp) {
   __shared__ int s_rows[GRAD_LIST];
   __shared__ int s_scan[LORA_WARPS];
   __shared__ RingShared shared;
@@ -1029,8 +1084,8 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_grad_kernel(const __grid
   const __nv_bfloat16* z = reinterpret_cast<const __nv_bfloat16*>(job.z);
   const int r16 = round16(job.ru) - t.r0;      // ranks that p has from r0 on
   const int tmem_cols = 4 * rp;
-  Ring ring = ring_start(shared, dyn, grad_stage(rp), tmem_cols, a.status);
-  const uint32_t idesc = umma_idesc_bf16(128, 2 * rp, 1, 1);
+  Ring ring = ring_start(shared, dyn, GRAD_STAGE, tmem_cols, a.status);
+  const uint32_t idesc = umma_idesc_bf16(128, rp, 1, 1);
   bool any = false;
   for (long long at = t.lo; at < t.hi; at += GRAD_LIST) {
     const int found = list_rows(a, ad, at, (int)min((long long)GRAD_LIST, t.hi - at), s_rows, s_scan);
@@ -1042,10 +1097,10 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_grad_kernel(const __grid
         const bool ok = k < found && col < job.c1;
         cp_async<16>(dst + (lane >> 3) * GRAD_BOX + r * 128 + 16 * ((lane & 7) ^ (r & 7)), ok ? z + row_of(k) * job.ldz + col : z, ok);
       }
-      for (int i = tid; i < GRAD_ROWS * (rp / 4); i += LORA_THREADS) {
-        const int r = i / (rp / 4), q = i % (rp / 4), s = q / (rp / 8), j = q % (rp / 8), k = step * GRAD_ROWS + r;
+      for (int i = tid; i < GRAD_ROWS * 16; i += LORA_THREADS) {
+        const int r = i >> 4, s = (i >> 3) & 1, j = i & 7, k = step * GRAD_ROWS + r;
         const bool ok = k < found && 8 * j < r16;
-        cp_async<16>(dst + GRAD_Z + (q >> 3) * GRAD_BOX + r * 128 + 16 * ((q & 7) ^ (r & 7)),
+        cp_async<16>(dst + GRAD_Z + s * GRAD_BOX + r * 128 + 16 * (j ^ (r & 7)),
                      ok ? job.p + ((long long)s * a.T + row_of(k)) * job.pcols + job.p0 + t.r0 + 8 * j : job.p, ok);
       }
     };
@@ -1055,11 +1110,24 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_grad_kernel(const __grid
       for (int q = 0; q < GRAD_ROWS / 16; ++q)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          umma_f16_ss(ring.tmem + 2 * rp * h, umma_smem_desc_sw128(src + 2 * h * GRAD_BOX + 2048 * q, GRAD_BOX, 1024),
-                      umma_smem_desc_sw128(src + GRAD_Z + 2048 * q, GRAD_BOX, 1024), idesc, !start || step || q);
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+            umma_f16_ss(ring.tmem + rp * (2 * h + s), umma_smem_desc_sw128(src + 2 * h * GRAD_BOX + 2048 * q, GRAD_BOX, 1024),
+                        umma_smem_desc_sw128(src + GRAD_Z + s * GRAD_BOX + 2048 * q, GRAD_BOX, 1024), idesc, !start || step || q);
     };
-    const int steps = (found + GRAD_ROWS - 1) / GRAD_ROWS;
-    ring_run(ring, steps, fill, feed);
+    // whole steps of neighbouring rows by TMA (behind the last row of all there are zeros), the rest row by row
+    const long long first = found ? (a.index ? (long long)s_rows[0] : at) : 0;
+    const bool run = found && (!a.index || s_rows[found - 1] - s_rows[0] == found - 1);
+    const int steps = (found + GRAD_ROWS - 1) / GRAD_ROWS, whole = !run ? 0 : first + found == a.T ? steps : found / GRAD_ROWS;
+    auto load = [&](uint32_t dst, uint32_t bar, int step) {
+      const int row = (int)first + step * GRAD_ROWS;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tma_load_2d(dst + i * GRAD_BOX, &maps.z[job.across], bar, t.col0 + 64 * i, row);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) tma_load_3d(dst + GRAD_Z + s * GRAD_BOX, &maps.p[job.across], bar, job.p0 + t.r0, row, s);
+    };
+    ring_tma(ring, whole, GRAD_STAGE, load, feed);
+    ring_gather(ring, steps - whole, [&](uint32_t dst, int step) { fill(dst, whole + step); }, [&](uint32_t src, int step) { feed(src, whole + step); });
     any = any || steps;
     __syncthreads();      // the list makes way
   }
@@ -1177,8 +1245,18 @@ EDL_HOST_API int edl_lora_apply(const void* x, long long ldx, const void* y, lon
     while (cluster < 8 && (long long)((T + DOWN_ROWS - 1) / DOWN_ROWS) * cluster * 2 <= 2 * sms && cols >= 2 * cluster * 4 * DOWN_K) cluster *= 2;
     const dim3 grid((unsigned)((long long)blocks * g.groups * cluster));
     const int ring = RING_STAGES * down_stage(np, backward), part = DOWN_ROWS * (np + 4) * 4, down_smem = (ring > part ? ring : part) + 1024;
-    if (backward ? launch_cluster(lora_down_kernel<true>, grid, cluster, down_smem, st, "lora down launch", g, s, np)
-                 : launch_cluster(lora_down_kernel<false>, grid, cluster, down_smem, st, "lora down launch", g, s, np))
+    // TMA takes weights whose rows start on 16 bytes; a box of the backward pass must not reach into the next part's columns
+    bool tma = !backward || (r % 8 == 0 && ldb % 8 == 0 && b_adapter % 8 == 0 && aligned(b, 16));
+    for (int p = 0; backward && p + 1 < parts; ++p) tma = tma && widths[p] % DOWN_K == 0;
+    CUtensorMap map_x{}, map_w{};
+    if (tma) {
+      if (make_tmap_2d_16b(&map_x, x, T, backward ? N : K, ldx, DOWN_ROWS, DOWN_K)) return -1;
+      if (backward ? make_tmap_3d_16b(&map_w, b, r, N, n, ldb, b_adapter, 64, DOWN_K, 1, 3)
+                   : make_tmap_3d_16b(&map_w, a, K, parts * r, n, lda, a_adapter, DOWN_K, np, 1, 3))
+        return -1;
+    }
+    if (backward ? launch_cluster(lora_down_kernel<true>, grid, cluster, down_smem, st, "lora down launch", g, map_x, map_w, (int)tma, s, np)
+                 : launch_cluster(lora_down_kernel<false>, grid, cluster, down_smem, st, "lora down launch", g, map_x, map_w, (int)tma, s, np))
       return -1;
     if (!out) return 0;
     g.groups = 0;
@@ -1294,8 +1372,14 @@ EDL_HOST_API int edl_lora_grads(const void* x, long long ldx, const void* dy, lo
   const dim3 grid((unsigned)(tiles * cluster), (unsigned)n);
   const char* what = "lora gradient launch";
   if (fast) {
-    const int ring = RING_STAGES * grad_stage(rp), tile = rp * GRAD_STRIDE * 4;
-    return launch_cluster(lora_grad_kernel, grid, cluster, (ring > tile ? ring : tile) + 1024, st, what, a, rp);
+    GradMaps maps{};
+    if (a.T && da && (make_tmap_2d_16b(&maps.z[0], x, a.T, K, ldx, GRAD_ROWS, 64) ||
+                      make_tmap_3d_16b(&maps.p[0], g, round16(parts * r), a.T, 2, round16(parts * r), (uint64_t)a.T * round16(parts * r), 64, GRAD_ROWS, 1, 3)))
+      return -1;
+    if (a.T && db && (make_tmap_2d_16b(&maps.z[1], dy, a.T, N, ldy, GRAD_ROWS, 64) ||
+                      make_tmap_3d_16b(&maps.p[1], u, parts * round16(r), a.T, 2, parts * round16(r), (uint64_t)a.T * parts * round16(r), 64, GRAD_ROWS, 1, 3)))
+      return -1;
+    return launch_cluster(lora_grad_kernel, grid, cluster, RING_STAGES * GRAD_STAGE + 1024, st, what, a, maps, rp);
   }
   const int smem = 16 * GRAD_STRIDE * 4;
   if (in_f32) return wide ? launch_cluster(lora_grad_any_kernel<float, 3, true>, grid, cluster, smem, st, what, a)
