@@ -23,7 +23,7 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int LORA_THREADS = 256, LORA_WARPS = 8;
+constexpr int LORA_THREADS = 256, LORA_WARPS = 8, LORA_MAX_WARPS = 10;
 constexpr int LORA_ROWS = 256;       // rows whose adapters a cluster looks through
 constexpr int LORA_SEGS = 8;
 
@@ -212,7 +212,8 @@ struct LoraArgs {
   unsigned short* u;     // [parts of u][T][ucols] scaled, bf16; may be null in the one-launch form
   int* status;
   float scale_all;
-  int T, n, rtot, ucols, groups, look, down_segs, up_segs, copy;
+  int T, n, rtot, ucols, groups, splits, down_segs, up_segs, copy;
+  int* mixed;            // [blocks of rows] written by the kernel that reduces, read by the one-launch form, which then takes mixed blocks alone
   LoraSeg down_seg[LORA_SEGS], up_seg[LORA_SEGS];
 };
 
@@ -225,9 +226,15 @@ struct RowUnits {
   short place[LORA_ROWS];                                       // of an adapter's rows in `order`, at its first row
   short order[LORA_ROWS], base[LORA_ROWS], rows[LORA_ROWS];     // row of a place; first place and rows of a unit
   int ad[LORA_ROWS];
-  int scan[LORA_WARPS];
+  int scan[LORA_MAX_WARPS];
   int total;
+  bool mixed;                                                   // rows of more than MIXED adapters
 };
+
+// Among many rows, a block of LORA_ROWS rows of more adapters than this (the single tokens of a step) goes to the one-launch kernel, whose
+// clusters take a few rows of an adapter each; the streaming kernels take the others. Every kernel of a call decides so for itself.
+// 3900 rows, 256 of them single tokens of 64 adapters: see the end of edl_lora_apply.
+constexpr int MIXED = 4;
 
 // Exclusive sum over the CTA's threads; `total` gets the sum of all.
 __device__ __forceinline__ int cta_scan(int v, int* scan, int& total) {
@@ -241,8 +248,7 @@ __device__ __forceinline__ int cta_scan(int v, int* scan, int& total) {
   if (lane == 31) scan[w] = at;
   __syncthreads();
   total = 0;
-#pragma unroll
-  for (int i = 0; i < LORA_WARPS; ++i) {
+  for (int i = 0; i < (int)(blockDim.x >> 5); ++i) {
     if (i < w) at += scan[i];
     total += scan[i];
   }
@@ -260,8 +266,10 @@ __device__ __forceinline__ void find_units(RowUnits& u, const LoraArgs& a, long 
     if (id >= a.n && a.status) atomicCAS(a.status, 0, EDL_BAD_INDEX);
     if (id < 0 || id >= a.n) id = -1;
   }
-  u.idx[tid] = id;
-  u.order[tid] = (short)tid;
+  if (tid < LORA_ROWS) {
+    u.idx[tid] = id;
+    u.order[tid] = (short)tid;
+  }
   __syncthreads();
   if (!a.index || __syncthreads_and(tid >= rows || id == u.idx[0])) {
     const int all = u.idx[0] >= 0 || a.copy ? (rows + chunk - 1) / chunk : 0;
@@ -270,7 +278,10 @@ __device__ __forceinline__ void find_units(RowUnits& u, const LoraArgs& a, long 
       u.rows[tid] = (short)min(chunk, rows - tid * chunk);
       u.ad[tid] = u.idx[0];
     }
-    if (tid == 0) u.total = all;
+    if (tid == 0) {
+      u.total = all;
+      u.mixed = false;
+    }
     __syncthreads();
     return;
   }
@@ -294,8 +305,11 @@ __device__ __forceinline__ void find_units(RowUnits& u, const LoraArgs& a, long 
       u.ad[unit + q] = id;
     }
   }
-  if (tid == 0) u.total = all;
-  __syncthreads();
+  const int adapters = __syncthreads_count(tid < rows && before == 0);
+  if (tid == 0) {
+    u.total = all;
+    u.mixed = adapters > MIXED;
+  }
   if (taken) u.order[u.place[first_row] + before] = (short)tid;
   __syncthreads();
 }
@@ -320,8 +334,6 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const __grid_cons
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), c = cluster.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t4 = lane & 3;
-  const int cid = blockIdx.x / C;
-  const long long row0 = (long long)(cid / a.groups) * LORA_ROWS;
   const int r16 = a.up_segs ? round16(a.up_seg[0].ru) : 0, ucols = a.ucols, ustride = u_stride(ucols);
   const int pstride = a.rtot;
   float* part = reinterpret_cast<float*>(dyn);                                      // [CHUNK][rtot]: this CTA's share of u
@@ -329,9 +341,13 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const __grid_cons
   float* red = reinterpret_cast<float*>(second);                                    // [warps][CHUNK][RSTRIDE], then
   unsigned short* su = reinterpret_cast<unsigned short*>(second);                   // [S][CHUNK][ustride]: scaled u in parts
 
-  find_units(units, a, row0, (int)min((long long)LORA_ROWS, a.T - row0), CHUNK);
-
+  // a cluster works on one block of rows, or, where only mixed ones are left, on its share of each of those
+  const int cid = blockIdx.x / C, nblocks = (int)(((long long)a.T + LORA_ROWS - 1) / LORA_ROWS);
   bool pending = false;
+  for (int block = a.mixed ? 0 : cid / a.groups, step = a.mixed ? 1 : nblocks; block < nblocks; block += step) {
+  if (a.mixed && !a.mixed[block]) continue;
+  const long long row0 = (long long)block * LORA_ROWS;
+  find_units(units, a, row0, (int)min((long long)LORA_ROWS, a.T - row0), CHUNK);
   for (int unit = cid % a.groups; unit < units.total; unit += a.groups) {
     const int ad = units.ad[unit], m = units.rows[unit];
     const short* order = units.order + units.base[unit];
@@ -511,6 +527,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const __grid_cons
     }
     __syncthreads();      // parts of u make way for the next unit
   }
+  }
   if (pending) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");      // no CTA leaves while its parts are read
 }
 
@@ -661,9 +678,10 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_down_kernel(const __grid
   const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x);
   Ring ring = ring_start(shared, dyn, down_stage(np, DOWN_T), 64, a.status);
   find_units(units, a, row0, (int)min((long long)LORA_ROWS, a.T - row0), DOWN_ROWS);
+  if (a.mixed && tid == 0) a.mixed[row0 / LORA_ROWS] = units.mixed;
   const uint32_t idesc = umma_idesc_bf16(128, np, 0, DOWN_T);
   bool pending = false;
-  for (int unit = cid % a.groups; unit < units.total; unit += a.groups) {
+  for (int unit = cid % a.groups; unit < (units.mixed ? 0 : units.total); unit += a.groups) {
     const int ad = units.ad[unit], m = units.rows[unit];
     if (ad < 0) continue;
     const short* order = units.order + units.base[unit];
@@ -771,26 +789,29 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_down_kernel(const __grid
 }
 
 // --------------------------------------------------------------------------------------------------- many rows: u onto y
-// A CTA takes 256 columns of one part (32 per warp) of up to `look` rows. The rows' u goes to shared memory once, the weights of a
-// warp's columns stay in registers for all rows of an adapter (up to 16 KC ranks); what remains per 16 rows is to read y, asked for two
-// turns ahead, and to write out.
+// What no TMA box fits or tensor memory holds (fp32 outputs, ranks that are no multiple of 8 or above 64), on `mma.sync`. A CTA takes 256
+// columns of one part (32 per warp) of some of a block's units of 16 rows. The rows' u goes to shared memory once, the weights of
+// a warp's columns stay in registers for all rows of an adapter (up to 16 KC ranks); what remains per 16 rows is to read y, asked for
+// two turns ahead, and to write out.
 constexpr int UP_COLS = 32 * LORA_WARPS;
 template <typename TY, int KC, bool UP_T>
-__global__ void __launch_bounds__(LORA_THREADS, 2) lora_up_kernel(const __grid_constant__ LoraArgs a) {
+__global__ void __launch_bounds__(LORA_THREADS, 2) lora_up_any_kernel(const __grid_constant__ LoraArgs a) {
   constexpr int S = sizeof(TY) == 4 ? 3 : 2;
   __shared__ RowUnits units;
   extern __shared__ __align__(16) uint8_t dyn[];
-  unsigned short* su = reinterpret_cast<unsigned short*>(dyn);      // [S][look][ustride], in the units' order
+  unsigned short* su = reinterpret_cast<unsigned short*>(dyn);      // [S][own rows][ustride], in the units' order
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t4 = lane & 3;
-  const long long row0 = (long long)(blockIdx.x / a.groups) * a.look;
+  const long long row0 = (long long)(blockIdx.x / (a.groups * a.splits)) * LORA_ROWS;
   int p = 0, tile = blockIdx.x % a.groups;
   for (; tile >= (a.up_seg[p].c1 - a.up_seg[p].c0 + UP_COLS - 1) / UP_COLS; ++p) tile -= (a.up_seg[p].c1 - a.up_seg[p].c0 + UP_COLS - 1) / UP_COLS;
   const LoraSeg seg = a.up_seg[p];
   const int n0 = seg.c0 + tile * UP_COLS + 32 * w, col = n0 + 8 * t4, r16 = round16(seg.ru), ustride = u_stride(r16);
   const bool ok = col < seg.c1;
-  find_units(units, a, row0, (int)min((long long)a.look, a.T - row0), 16);
-  const int total = units.total;
-  if (!total) return;
+  find_units(units, a, row0, (int)min((long long)LORA_ROWS, a.T - row0), 16);
+  const int share = (units.total + a.splits - 1) / a.splits, unit0 = min(units.total, (int)(blockIdx.x / a.groups % a.splits) * share);
+  const int total = min(units.total, unit0 + share);
+  if (units.mixed || unit0 >= total) return;
+  const int place0 = units.base[unit0], places = units.base[total - 1] + units.rows[total - 1] - place0;
   const TY* y = reinterpret_cast<const TY*>(a.y) + col;
   TY* out = reinterpret_cast<TY*>(a.out) + col;
   constexpr int W = sizeof(TY) / 2;      // 16-byte pieces of eight values
@@ -811,22 +832,22 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_up_kernel(const __grid_c
     }
   };
   {
-    const int places = units.base[total - 1] + units.rows[total - 1], per = r16 / 8;
+    const int per = r16 / 8;
     for (int i = tid; i < S * places * per; i += LORA_THREADS) {
       const int q = i % per, place = (i / per) % places, s = i / (per * places);
-      cp_async<16>(smem_u32(su + (s * a.look + place) * ustride + 8 * q),
-                   a.u + ((long long)s * a.T + row0 + units.order[place]) * a.ucols + p * r16 + 8 * q, true);
+      cp_async<16>(smem_u32(su + (s * places + place) * ustride + 8 * q),
+                   a.u + ((long long)s * a.T + row0 + units.order[place0 + place]) * a.ucols + p * r16 + 8 * q, true);
     }
     cp_commit();
   }
-  ask(0, ring[0], rows[0]);
-  ask(1, ring[1], rows[1]);
+  ask(unit0, ring[0], rows[0]);
+  ask(unit0 + 1, ring[1], rows[1]);
   cp_wait<0>();
   __syncthreads();
   int have = -1;
   uint32_t wb[KC][4][1][2];
   auto turn_of = [&](int unit, uint4 (&yq)[2][W], long long (&row)[2]) {
-    const int ad = units.ad[unit], base = units.base[unit];
+    const int ad = units.ad[unit], base = units.base[unit] - place0;
     // [column tile][row half, column]: y and what is added to it. The tensor cores cut sums off, so 32-bit results add y to the sum of products.
     float acc[4][4], yv[2][8];
 #pragma unroll
@@ -839,8 +860,8 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_up_kernel(const __grid_c
     ask(unit + 2, yq, row);
     if (ad >= 0) {
       // places behind the unit's rows: whatever lies there goes into rows that are not written
-      const unsigned short* su0 = su + min(base + g, a.look - 1) * ustride + 4 * t4;
-      const unsigned short* su1 = su + min(base + 8 + g, a.look - 1) * ustride + 4 * t4;
+      const unsigned short* su0 = su + min(base + g, places - 1) * ustride + 4 * t4;
+      const unsigned short* su1 = su + min(base + 8 + g, places - 1) * ustride + 4 * t4;
       for (int kc0 = 0; kc0 < r16; kc0 += 16 * KC) {
         if (ad != have || r16 > 16 * KC) {
           const __nv_bfloat16* wu = reinterpret_cast<const __nv_bfloat16*>(a.up) + (long long)ad * a.up_adapter;
@@ -854,7 +875,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_up_kernel(const __grid_c
           uint32_t ua[S][4];
 #pragma unroll
           for (int s = 0; s < S; ++s) {
-            const int at = s * a.look * ustride + kc0 + 16 * i;
+            const int at = s * places * ustride + kc0 + 16 * i;
             const uint2 v0 = *reinterpret_cast<const uint2*>(su0 + at), v1 = *reinterpret_cast<const uint2*>(su1 + at);
             ua[s][0] = v0.x; ua[s][1] = v1.x;
             ua[s][2] = v0.y; ua[s][3] = v1.y;
@@ -872,18 +893,232 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_up_kernel(const __grid_c
       store_row<TY, true>(dst[h], ok && dst[h] ? 8 : 0, v);
     }
   };
-  for (int unit = 0; unit < total; unit += 2) {
+  for (int unit = unit0; unit < total; unit += 2) {
     turn_of(unit, ring[0], rows[0]);
     if (unit + 1 < total) turn_of(unit + 1, ring[1], rows[1]);
   }
 }
 
+// The same on tcgen05: 128 rows of one adapter are the M side, 64 columns at a time the N side, the ranks of both parts of u the inner index.
+// A lane loads tiles of y and of the weights ahead (TMA), a lane of the second warp issues the products into one of two
+// accumulators, and eight warps add them to y in shared memory, a row per lane, and write whole row segments out. What bounds it is the
+// traffic of y and out: a 16-byte piece costs about 30 instructions of a lane, a seventh of what `mma.sync` fragments took.
+constexpr int UP_THREADS = 320, UP_ROWS = 128, UP_TILE = 64, UP_STAGES = 3;
+constexpr int UP_Y = UP_ROWS * UP_TILE * 2, UP_W = 64 * 128, UP_U = UP_ROWS * 128;
+constexpr int UP_SMEM = UP_STAGES * (UP_Y + UP_W) + 2 * UP_U + 1024;
+
+template <bool UP_T>
+__global__ void __launch_bounds__(UP_THREADS, 2) lora_up_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ CUtensorMap map_y,
+                                                               const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_u) {
+  __shared__ RowUnits units;
+  __shared__ uint64_t s_bars[2 * UP_STAGES + 6];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort;
+  extern __shared__ uint8_t raw[];
+  uint8_t* dyn = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t stages = smem_u32(dyn), su = stages + UP_STAGES * (UP_Y + UP_W);
+  const uint32_t full = smem_u32(s_bars), empty = full + 8 * UP_STAGES, dfull = empty + 8 * UP_STAGES, dempty = dfull + 16, ufull = dempty + 16,
+                 ufree = ufull + 8;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  const long long row0 = (long long)(blockIdx.x / a.splits) * LORA_ROWS;
+  if (tid == 0) {
+    for (int i = 0; i < UP_STAGES; ++i) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, 8);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(dfull + 8 * i, 1);
+      mbar_init(dempty + 8 * i, 8);
+    }
+    mbar_init(ufull, 1);
+    mbar_init(ufree, 1);
+    s_abort = 0;
+    fence_mbar_init();
+  }
+  if (w == 1) {
+    tmem_alloc(smem_u32(&s_tmem), 2 * UP_TILE);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  find_units(units, a, row0, (int)min((long long)LORA_ROWS, a.T - row0), UP_ROWS);
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  const int r16 = round16(a.up_seg[0].ru), share = (a.groups + a.splits - 1) / a.splits;      // column tiles: all, of a CTA
+  const int tile0 = min(a.groups, (int)(blockIdx.x % a.splits) * share), tile1 = min(a.groups, tile0 + share);
+  volatile int* abort_flag = &s_abort;
+  auto wait = [&](uint32_t bar, int use, int code) { mbar_wait(bar, use & 1, abort_flag, a.status, code); };
+
+  // Every role walks the same runs: a unit's tiles within one part (whose u they share). `runs` counts those with an adapter, `tiles` all tiles.
+  auto walk = [&](auto begin, auto each, auto end) {
+    int runs = 0, tiles = 0;
+    for (int unit = 0; unit < (units.mixed ? 0 : units.total); ++unit) {
+      const int ad = units.ad[unit], m = units.rows[unit];
+      const short* order = units.order + units.base[unit];
+      const bool line = order[m - 1] - order[0] == m - 1;      // neighbouring rows
+      int first = 0;      // of part p's tiles
+      for (int p = 0; p < a.up_segs; ++p) {
+        const int c0 = a.up_seg[p].c0, last = first + (a.up_seg[p].c1 - c0 + UP_TILE - 1) / UP_TILE;
+        const int lo = max(first, tile0), hi = min(last, tile1);
+        if (lo < hi) {
+          if (ad >= 0) begin(ad, m, order, line, p, runs);
+          for (int t = lo; t < hi; ++t, ++tiles) each(ad, m, order, line, p, c0 + (t - first) * UP_TILE, tiles);
+          if (ad >= 0) end(runs++);
+        }
+        first = last;
+      }
+    }
+  };
+  if (w == 0) {
+    if (elect_one()) {
+      walk(
+          [&](int ad, int m, const short* order, bool line, int p, int run) {
+            if (run) wait(ufree, run - 1, EDL_TIMEOUT_PRODUCER);
+            if (!line) return;
+            mbar_expect_tx(ufull, 2 * UP_U);
+            for (int s = 0; s < 2; ++s) tma_load_3d(su + s * UP_U, &map_u, ufull, p * r16, (int)row0 + order[0], s);
+          },
+          [&](int ad, int m, const short* order, bool line, int p, int n0, int tile) {
+            const int at = tile % UP_STAGES, use = tile / UP_STAGES;
+            if (use) wait(empty + 8 * at, use - 1, EDL_TIMEOUT_PRODUCER);
+            const uint32_t dst = stages + at * (UP_Y + UP_W), bar = full + 8 * at;
+            const bool read = a.y && line;
+            mbar_expect_tx(bar, (read ? UP_Y : 0) + (ad < 0 ? 0 : UP_T ? r16 * 128 : UP_W));
+            if (read) tma_load_2d(dst, &map_y, bar, n0, (int)row0 + order[0]);
+            if (ad >= 0) {
+              if constexpr (UP_T) tma_load_3d(dst + UP_Y, &map_w, bar, n0, 0, ad);
+              else tma_load_3d(dst + UP_Y, &map_w, bar, 0, n0, ad);
+            }
+          },
+          [](int) {});
+    }
+    __syncwarp();
+  } else if (w == 1) {
+    const bool leader = elect_one();
+    const uint32_t idesc = umma_idesc_bf16(UP_ROWS, UP_TILE, 0, UP_T);
+    walk([&](int, int, const short*, bool, int, int run) { wait(ufull, run, EDL_TIMEOUT_MMA); },
+         [&](int ad, int, const short*, bool, int, int, int tile) {
+           const int at = tile % UP_STAGES, buf = tile & 1;
+           wait(full + 8 * at, tile / UP_STAGES, EDL_TIMEOUT_MMA);
+           if (tile > 1) wait(dempty + 8 * buf, tile / 2 - 1, EDL_TIMEOUT_MMA);
+           tc_fence_after();
+           if (!leader) return;
+           const uint32_t src = stages + at * (UP_Y + UP_W) + UP_Y;
+           for (int s = 1; ad >= 0 && s >= 0; --s)
+             for (int k = 0; k < r16 / 16; ++k)
+               umma_f16_ss(tmem + buf * UP_TILE, umma_smem_desc_sw128(su + s * UP_U + 32 * k, 16, 1024),
+                           umma_smem_desc_sw128(src + (UP_T ? 2048 : 32) * k, UP_T ? 8192 : 16, 1024), idesc, s == 0 || k);
+           tc_commit(dfull + 8 * buf);
+         },
+         [&](int) {
+           if (leader) tc_commit(ufree);
+         });
+    __syncwarp();
+  } else {
+    const int q = w & 3, h = (w - 2) >> 2, r = 32 * q + lane;      // this lane's row of a tile; which 32 of its columns
+    walk(
+        [&](int, int m, const short* order, bool line, int p, int run) {
+          if (line) return;
+          if (run) wait(ufree, run - 1, EDL_TIMEOUT_EPILOGUE);
+          for (int i = tid - 64; i < 2 * UP_ROWS * (r16 / 8); i += 256) {
+            const int j = i % (r16 / 8), tok = i / (r16 / 8) % UP_ROWS, s = i / (r16 / 8 * UP_ROWS);
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (tok < m) v = *reinterpret_cast<const uint4*>(a.u + ((long long)s * a.T + row0 + order[tok]) * a.ucols + p * r16 + 8 * j);
+            *reinterpret_cast<uint4*>(dyn + (su - stages) + s * UP_U + tok * 128 + 16 * (j ^ (tok & 7))) = v;
+          }
+          fence_proxy_async_smem();
+          asm volatile("bar.sync 1, 256;" ::: "memory");
+          if (tid == 64) mbar_arrive(ufull);
+        },
+        [&](int ad, int m, const short* order, bool line, int p, int n0, int tile) {
+          const int at = tile % UP_STAGES, buf = tile & 1;
+          uint8_t* box = dyn + at * (UP_Y + UP_W);
+          wait(full + 8 * at, tile / UP_STAGES, EDL_TIMEOUT_EPILOGUE);
+          wait(dfull + 8 * buf, tile / 2, EDL_TIMEOUT_EPILOGUE);
+          tc_fence_after();
+          uint32_t d[32];
+          tmem_ld_32x32b_x32(tmem + (uint32_t(32 * q) << 16) + buf * UP_TILE + 32 * h, d);
+          // rows as they leave: eight rows of four pieces at a time
+          const int sub = 4 * ((lane >> 2) & 1) + (lane >> 3), piece = 4 * h + (lane & 3);
+          const bool col = n0 + 8 * piece < a.up_seg[p].c1;
+          if (a.y && !line) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int rr = 32 * q + 8 * i + sub;
+              if (rr < m && col)
+                *reinterpret_cast<uint4*>(box + rr * 128 + 16 * (piece ^ (rr & 7))) =
+                    *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.y) + (row0 + order[rr]) * a.ldy + n0 + 8 * piece);
+            }
+            __syncwarp();
+          }
+          tc_wait_ld();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(dempty + 8 * buf);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint4* slot = reinterpret_cast<uint4*>(box + r * 128 + 16 * ((4 * h + i) ^ (r & 7)));
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (a.y) v = *slot;
+            if (ad >= 0) {
+              uint32_t* e = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                e[k] = pack_bf16x2(__uint_as_float(e[k] << 16) + __uint_as_float(d[8 * i + 2 * k]),
+                                   __uint_as_float(e[k] & 0xffff0000u) + __uint_as_float(d[8 * i + 2 * k + 1]));
+            }
+            *slot = v;
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int rr = 32 * q + 8 * i + sub;
+            if (rr < m && col)
+              *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(a.out) + (row0 + order[rr]) * a.ldo + n0 + 8 * piece) =
+                  *reinterpret_cast<const uint4*>(box + rr * 128 + 16 * (piece ^ (rr & 7)));
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(empty + 8 * at);
+        },
+        [](int) {});
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (w == 1) tmem_dealloc(tmem, 2 * UP_TILE);
+}
+
+// Raises a kernel's limit of dynamic shared memory on the current device, once.
+int shared_memory(const void* kernel, int bytes, const char* what) {
+  struct Limit {
+    const void* kernel;
+    int dev, bytes;
+  };
+  static thread_local Limit known[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  Limit* free_slot = nullptr;
+  for (Limit& l : known) {
+    if (l.kernel == kernel && l.dev == dev) {
+      if (l.bytes >= bytes) return 0;
+      free_slot = &l;
+      break;
+    }
+    if (!l.kernel) {
+      free_slot = &l;
+      break;
+    }
+  }
+  if (check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), what)) return -1;
+  if (free_slot) *free_slot = Limit{kernel, dev, bytes};
+  return 0;
+}
+
 template <typename... E, typename... A>
-int launch_cluster(void (*k)(E...), dim3 grid, int cluster, int smem, cudaStream_t stream, const char* what, A... args) {
-  if (smem > 48 * 1024 && check_cuda(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), what)) return -1;
+int launch_sized(void (*k)(E...), dim3 grid, int threads, int cluster, int smem, cudaStream_t stream, const char* what, const A&... args) {
+  if (smem > 40 * 1024 && shared_memory(reinterpret_cast<const void*>(k), smem, what)) return -1;      // 48 KB with the static part
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(LORA_THREADS);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -894,6 +1129,11 @@ int launch_cluster(void (*k)(E...), dim3 grid, int cluster, int smem, cudaStream
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return check_cuda(cudaLaunchKernelEx(&cfg, k, args...), what);
+}
+
+template <typename... E, typename... A>
+int launch_cluster(void (*k)(E...), dim3 grid, int cluster, int smem, cudaStream_t stream, const char* what, const A&... args) {
+  return launch_sized(k, grid, LORA_THREADS, cluster, smem, stream, what, args...);
 }
 
 // ------------------------------------------------------------------------------------------------------------- gradients
@@ -1156,12 +1396,14 @@ using namespace edl;
 // `parts` parts of N. a: [n][parts * r][K], b: [n][N][r] with strides. backward = 0: out = y + s (x a^T) b^T. backward = 1: x is dy [T, N],
 // out dx [T, K] (null: u alone), y null. u: s x a^T or s dy b in bf16 parts (2 for bf16 results, 3 for fp32 ones), [parts][T][columns] with
 // parts * r rounded up to 16 per part (forward) or as a whole (backward); asked for above 256 rows of bf16, else it may be null.
-// index [T] int32 or null (adapter 0 everywhere), scale [n] fp32 or null (scale_all). x_f32: x and the weights are fp32 (then
+// mixed: a flag per 256 rows, scratch; asked for above 256 rows of bf16 with an index. index [T] int32 or null (adapter 0 everywhere), scale
+// [n] fp32 or null (scale_all). x_f32: x and the weights are fp32 (then
 // y and out too), else bf16; y_f32: type of y and out. Indexes from n on set the status word and count as none.
 EDL_HOST_API int edl_lora_apply(const void* x, long long ldx, const void* y, long long ldy, void* out, long long ldo, const void* a,
                                 long long a_adapter, long long lda, const void* b, long long b_adapter, long long ldb,
-                                const int* index, const float* scale, float scale_all, void* u, long long u_size, int T, int K, int N,
-                                int n, int r, int parts, const int* widths, int x_f32, int y_f32, int backward, int* status, void* stream) {
+                                const int* index, const float* scale, float scale_all, void* u, long long u_size, int* mixed, int T,
+                                int K, int N, int n, int r, int parts, const int* widths, int x_f32, int y_f32, int backward, int* status,
+                                void* stream) {
   if (T <= 0) return 0;
   if (K <= 0 || N <= 0 || n <= 0 || r <= 0 || parts < 1 || parts > LORA_SEGS || r > 512 / parts) {
     set_last_error("edl_lora_apply: needs sizes above 0, up to %d parts and parts x rank up to 512", LORA_SEGS);
@@ -1221,7 +1463,7 @@ EDL_HOST_API int edl_lora_apply(const void* x, long long ldx, const void* y, lon
   const int blocks = (int)(((long long)T + LORA_ROWS - 1) / LORA_ROWS), in_block = T < LORA_ROWS ? T : LORA_ROWS, sms = sm_count();
   // clusters for a block's units: as many as it can have, or fewer that take turns once there are enough for the GPU
   auto groups_of = [&](int chunk) {
-    const long long most = (long long)(index ? (n < in_block ? n + 1 : in_block) : 1) + in_block / chunk;
+    const long long most = index ? (long long)(n < in_block ? n + 1 : in_block) + in_block / chunk : (in_block + chunk - 1) / chunk;
     int groups = 128 / blocks;
     if (groups < LORA_ROWS / chunk) groups = LORA_ROWS / chunk;
     if (groups > most) groups = (int)most;
@@ -1233,6 +1475,12 @@ EDL_HOST_API int edl_lora_apply(const void* x, long long ldx, const void* y, lon
       set_last_error("edl_lora_apply: more than %d rows need u", LORA_ROWS);
       return -1;
     }
+    const bool may_mix = index && n + 1 > MIXED;      // rows without an adapter count as one
+    if (may_mix && !mixed) {
+      set_last_error("edl_lora_apply: more than %d rows of %d adapters need a flag per block of rows", LORA_ROWS, n);
+      return -1;
+    }
+    g.mixed = may_mix ? mixed : nullptr;
     g.groups = groups_of(DOWN_ROWS);
     int ru = 0, cols = 0;
     for (int i = 0; i < g.down_segs; ++i) {
@@ -1258,41 +1506,62 @@ EDL_HOST_API int edl_lora_apply(const void* x, long long ldx, const void* y, lon
     if (backward ? launch_cluster(lora_down_kernel<true>, grid, cluster, down_smem, st, "lora down launch", g, map_x, map_w, (int)tma, s, np)
                  : launch_cluster(lora_down_kernel<false>, grid, cluster, down_smem, st, "lora down launch", g, map_x, map_w, (int)tma, s, np))
       return -1;
-    if (!out) return 0;
-    g.groups = 0;
-    for (int i = 0; i < g.up_segs; ++i) g.groups += (g.up_seg[i].c1 - g.up_seg[i].c0 + UP_COLS - 1) / UP_COLS;
-    const int r16 = round16(g.up_seg[0].ru), row_bytes = s * u_stride(r16) * 2;
-    g.look = LORA_ROWS;      // fewer rows per CTA where their u takes much shared memory, or where there are few CTAs
-    while (g.look > 16 && (g.look * row_bytes > 48 * 1024 || (g.look > 64 && (long long)g.groups * ((T + g.look - 1) / g.look) < 4LL * sms))) g.look /= 2;
-    const long long ctas = (long long)g.groups * (((long long)T + g.look - 1) / g.look);
-    if (ctas > 0x7fffffffLL) {
-      set_last_error("edl_lora_apply: too many rows for one launch");
-      return -1;
-    }
-    const int kc = r16 / 16;
-#define EDL_LORA_UP(TO, BW)                                                                                                      \
-  {                                                                                                                              \
-    const dim3 up((unsigned)ctas);                                                                                               \
-    const int smem = g.look * row_bytes;                                                                                         \
-    if (kc == 1) return launch_cluster(lora_up_kernel<TO, 1, BW>, up, 1, smem, st, "lora up launch", g);                         \
-    if (kc == 2) return launch_cluster(lora_up_kernel<TO, 2, BW>, up, 1, smem, st, "lora up launch", g);                         \
-    return launch_cluster(lora_up_kernel<TO, 4, BW>, up, 1, smem, st, "lora up launch", g);                                      \
-  }
-    if (backward) EDL_LORA_UP(__nv_bfloat16, true)
-    if (y_f32) EDL_LORA_UP(float, false)
-    EDL_LORA_UP(__nv_bfloat16, false)
+    if (out) {
+      const int r16 = round16(g.up_seg[0].ru), columns = backward ? K : N;
+      const bool tiles = r16 <= 64 && !y_f32 && (backward || (r % 8 == 0 && ldb % 8 == 0 && b_adapter % 8 == 0 && aligned(b, 16)));
+      const int width = tiles ? UP_TILE : UP_COLS;
+      g.groups = 0;
+      for (int i = 0; i < g.up_segs; ++i) g.groups += (g.up_seg[i].c1 - g.up_seg[i].c0 + width - 1) / width;
+      if (tiles) {
+        // a block's columns are cut into as many CTAs as run at once (two per SM), or three times that where blocks may have more
+        // units than others, of at least four tiles
+        const int ctas = (index ? 6 : 2) * sms / blocks;
+        g.splits = ctas < g.groups / 4 ? ctas : g.groups / 4;
+        if (g.splits < 1) g.splits = 1;
+        g.splits = (g.groups + (g.groups + g.splits - 1) / g.splits - 1) / ((g.groups + g.splits - 1) / g.splits);
+        CUtensorMap map_y{}, map_u{};
+        if (y && make_tmap_2d_16b(&map_y, y, T, columns, ldy, UP_ROWS, UP_TILE)) return -1;
+        if (make_tmap_3d_16b(&map_u, u, g.ucols, T, 2, g.ucols, (uint64_t)T * g.ucols, 64, UP_ROWS, 1, 3)) return -1;
+        if (backward ? make_tmap_3d_16b(&map_w, a, K, parts * r, n, lda, a_adapter, UP_TILE, r16, 1, 3)
+                     : make_tmap_3d_16b(&map_w, b, r, N, n, ldb, b_adapter, 64, UP_TILE, 1, 3))
+          return -1;
+        const dim3 up((unsigned)((long long)blocks * g.splits));
+        if (backward ? launch_sized(lora_up_kernel<true>, up, UP_THREADS, 1, UP_SMEM, st, "lora up launch", g, map_y, map_w, map_u)
+                     : launch_sized(lora_up_kernel<false>, up, UP_THREADS, 1, UP_SMEM, st, "lora up launch", g, map_y, map_w, map_u))
+          return -1;
+      } else {
+        // a block that is not mixed has at most 16 + MIXED units: they are shared out where there are few CTAs, or where u takes much memory
+        const int row_bytes = s * u_stride(r16) * 2, units = LORA_ROWS / 16 + MIXED;
+        auto own = [&](int splits) { return ((units + splits - 1) / splits) * 16 * row_bytes; };
+        g.splits = 1;
+        while (g.splits < 8 && (own(g.splits) > 56 * 1024 || (g.splits < 4 && (long long)g.groups * blocks * g.splits < 4LL * sms))) g.splits *= 2;
+        const long long ctas = (long long)g.groups * blocks * g.splits;
+        if (ctas > 0x7fffffffLL) {
+          set_last_error("edl_lora_apply: too many rows for one launch");
+          return -1;
+        }
+        const int kc = r16 / 16;
+#define EDL_LORA_UP(TO, BW)                                                                                                          \
+  (kc == 1   ? launch_cluster(lora_up_any_kernel<TO, 1, BW>, dim3((unsigned)ctas), 1, own(g.splits), st, "lora up launch", g)        \
+   : kc == 2 ? launch_cluster(lora_up_any_kernel<TO, 2, BW>, dim3((unsigned)ctas), 1, own(g.splits), st, "lora up launch", g)        \
+             : launch_cluster(lora_up_any_kernel<TO, 4, BW>, dim3((unsigned)ctas), 1, own(g.splits), st, "lora up launch", g))
+        if (backward ? EDL_LORA_UP(__nv_bfloat16, true) : y_f32 ? EDL_LORA_UP(float, false) : EDL_LORA_UP(__nv_bfloat16, false)) return -1;
 #undef EDL_LORA_UP
+      }
+    }
+    if (!g.mixed) return 0;      // what is left: blocks of single tokens
   }
 
   const int ranks = backward ? r : parts * r;      // that one pass over x can take
   const int rt = !wide || x_f32 || ranks <= 16 ? 1 : ranks <= 32 ? 2 : 4;
-  g.groups = groups_of(16);
   // clusters of eight while they all fit the GPU twice, then smaller ones
   int cluster = 8;
-  while (cluster > 2 && (long long)blocks * g.groups * cluster > 4LL * sms) cluster /= 2;
+  g.groups = g.mixed ? 2 * sms / cluster : groups_of(16);
+  const long long grid_blocks = g.mixed ? 1 : blocks;
+  while (cluster > 2 && grid_blocks * g.groups * cluster > 4LL * sms) cluster /= 2;
   const int red = LORA_WARPS * 16 * (16 * rt + 4) * 4, su = s * 16 * u_stride(g.ucols) * 2;
   const int smem = ((16 * g.rtot * 4 + 15) & ~15) + (red > su ? red : su);
-  const dim3 grid((unsigned)((long long)blocks * g.groups * cluster));
+  const dim3 grid((unsigned)(grid_blocks * g.groups * cluster));
 #define EDL_LORA(TX, TO, RTV, BW, W) return launch_cluster(lora_kernel<TX, TO, RTV, BW, W>, grid, cluster, smem, st, "lora launch", g)
 #define EDL_LORA_BF(TO, BW)                                    \
   {                                                            \

@@ -19,8 +19,8 @@ import torch
 from . import _lib
 
 vp, i32, i64, f32 = _lib.vp, _lib.i32, _lib.i64, _lib.f32
-_lib.register("edl_lora_apply", i32, [vp, i64, vp, i64, vp, i64, vp, i64, i64, vp, i64, i64, vp, vp, f32, vp, i64, i32, i32, i32,
-                                      i32, i32, i32, vp, i32, i32, i32, vp, vp])
+_lib.register("edl_lora_apply", i32, [vp, i64, vp, i64, vp, i64, vp, i64, i64, vp, i64, i64, vp, vp, f32, vp, i64, vp, i32, i32,
+                                      i32, i32, i32, i32, vp, i32, i32, i32, vp, vp])
 _lib.register("edl_lora_grads", i32, [vp, i64, vp, i64, vp, vp, vp, vp, i64, i64, vp, i64, i64, i32, i32, i32, i32, i32, i32, vp, i32,
                                       i32, i32, vp, vp])
 
@@ -96,12 +96,13 @@ def _apply(x, y, out, a, b, index, scale, u, parts, backward=False):
     T, dev = x.shape[0], x.device
     if u is None and T > FEW_ROWS:
         u = _inner(x, r, len(parts), x.dtype if out is None else out.dtype, backward)
+    mixed = None if index is None or T <= FEW_ROWS else index.new_empty(-(-T // FEW_ROWS))      # which blocks of rows have many adapters
     st = scale if isinstance(scale, torch.Tensor) else None
     _lib.call_on(dev, "edl_lora_apply", x.data_ptr(), x.stride(0), None if y is None else y.data_ptr(), 0 if y is None else y.stride(0),
                  None if out is None else out.data_ptr(), 0 if out is None else out.stride(0), a.data_ptr(), a.stride(0), a.stride(1),
                  b.data_ptr(), b.stride(0), b.stride(1), None if index is None else index.data_ptr(), None if st is None else st.data_ptr(),
-                 0.0 if st is not None else scale, None if u is None else u.data_ptr(), 0 if u is None else u.numel(), T, a.shape[2], N, n, r,
-                 len(parts), _widths(parts), x.dtype == torch.float32, (x if out is None else out).dtype == torch.float32, backward,
+                 0.0 if st is not None else scale, None if u is None else u.data_ptr(), 0 if u is None else u.numel(),
+                 None if mixed is None else mixed.data_ptr(), T, a.shape[2], N, n, r, len(parts), _widths(parts), x.dtype == torch.float32, (x if out is None else out).dtype == torch.float32, backward,
                  _lib.status_word(dev).data_ptr())
 
 
