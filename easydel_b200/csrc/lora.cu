@@ -163,6 +163,21 @@ __device__ __forceinline__ void mma_parts(float (&d)[4], const uint32_t (&a)[PA]
       if (o - i >= 0 && o - i < PB) mma_bf16(d, a[i][0], a[i][1], a[i][2], a[i][3], b[o - i][0], b[o - i][1]);
 }
 
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
+// Sum of the values at `addr` (shared memory) of the CTAs of a cluster, in rank order; all are asked for before the first is used.
+__device__ __forceinline__ float cluster_sum(uint32_t addr, int C) {
+  float v[8], sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    v[k] = 0.f;
+    if (k < C) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[k]) : "r"(mapa_shared(addr, k)) : "memory");
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) sum += v[k];
+  return sum;
+}
+
 // ---------------------------------------------------------------------------------------------------------- which rows
 struct LoraSeg {
   int c0, c1;       // columns of the matrix this side works on
@@ -451,18 +466,30 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const __grid_cons
           __syncthreads();
         }
       }
-      // ---- u of all CTAs, scaled, as bf16 parts
+      // ---- u of all CTAs, scaled, as bf16 parts; meanwhile the second product's weights and y come to L2
+      if (a.out) {
+        for (int grp = c * LORA_WARPS + w;; grp += C * LORA_WARPS) {
+          int p = 0, gi = grp;
+          for (; p < a.up_segs && gi >= (a.up_seg[p].c1 - a.up_seg[p].c0 + 31) / 32; ++p) gi -= (a.up_seg[p].c1 - a.up_seg[p].c0 + 31) / 32;
+          if (p >= a.up_segs) break;
+          const int n0 = a.up_seg[p].c0 + 32 * gi;
+          const T* wu = reinterpret_cast<const T*>(a.up) + (long long)ad * a.up_adapter;
+          if constexpr (!DOWN_T) {
+            if (n0 + lane < a.up_seg[p].c1)
+              for (int r = 0; r < a.up_seg[p].ru; r += 64 / (int)sizeof(T)) prefetch_l2(wu + (long long)(n0 + lane) * a.ld_up + r);
+          } else {
+            for (int r = lane; r < a.up_seg[p].ru; r += 32) prefetch_l2(wu + (long long)r * a.ld_up + n0);
+          }
+          if (a.y && lane < m) prefetch_l2(reinterpret_cast<const TY*>(a.y) + (row0 + order[lane]) * a.ldy + n0);
+        }
+      }
       cluster_sync_all();
       const float s = a.scale ? a.scale[ad] : a.scale_all;
       for (int e = tid; e < CHUNK * ucols; e += LORA_THREADS) {
         const int tok = e / ucols, col = e - tok * ucols;
         const int p = a.up_segs > 1 ? col / r16 : 0, rank = col - p * r16;
         float v = 0.f;
-        if (tok < m && rank < a.up_seg[p].ru) {
-          const int pos = tok * pstride + a.up_seg[p].u0 + rank;
-          for (int k = 0; k < C; ++k) v += cluster.map_shared_rank(part, k)[pos];
-          v *= s;
-        }
+        if (tok < m && rank < a.up_seg[p].ru) v = cluster_sum(smem_u32(part + tok * pstride + a.up_seg[p].u0 + rank), C) * s;
         uint32_t parts[S];
         split<S>(v, parts);
 #pragma unroll
@@ -657,8 +684,9 @@ __device__ __forceinline__ void ring_end(Ring& r, int tmem_cols) {
 }
 
 // u of up to 128 rows of one adapter (the M side; ranks are the N side): columns in steps of 64 through the ring, cut over the CTAs of a
-// cluster where there are few rows. The CTAs' sums are added in a fixed order.
-constexpr int DOWN_ROWS = 128, DOWN_K = 64, DOWN_X = DOWN_ROWS * DOWN_K * 2, DOWN_RANKS = 64;
+// cluster where there are few rows. Passes (up to 64 ranks of a part) run one after the other into columns of their own of tensor memory,
+// up to 128 at a time, before the CTAs' sums are added, in a fixed order.
+constexpr int DOWN_ROWS = 128, DOWN_K = 64, DOWN_X = DOWN_ROWS * DOWN_K * 2, DOWN_RANKS = 64, DOWN_COLS = 128;
 __host__ __device__ constexpr int down_stage(int np, bool down_t) { return DOWN_X + (down_t ? DOWN_K : np) * 128; }
 
 template <bool DOWN_T>
@@ -668,18 +696,28 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_down_kernel(const __grid
   __shared__ RingShared shared;
   extern __shared__ uint8_t raw[];
   uint8_t* dyn = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  float* part = reinterpret_cast<float*>(dyn);      // [128][np + 4], where the stages were
-  const int pstride = np + 4;
+  float* part = reinterpret_cast<float*>(dyn);      // [128][pstride], where the stages were
+  constexpr int pstride = DOWN_COLS + 4;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), c = cluster.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int cid = blockIdx.x / C;
   const long long row0 = (long long)(cid / a.groups) * LORA_ROWS;
   const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x);
-  Ring ring = ring_start(shared, dyn, down_stage(np, DOWN_T), 64, a.status);
+  Ring ring = ring_start(shared, dyn, down_stage(np, DOWN_T), DOWN_COLS, a.status);
   find_units(units, a, row0, (int)min((long long)LORA_ROWS, a.T - row0), DOWN_ROWS);
   if (a.mixed && tid == 0) a.mixed[row0 / LORA_ROWS] = units.mixed;
   const uint32_t idesc = umma_idesc_bf16(128, np, 0, DOWN_T);
+  // passes: `each` of a part's ranks in all parts; `at_once` of them fit tensor memory
+  const int each = (a.down_seg[0].ru + np - 1) / np, passes = a.down_segs * each, at_once = DOWN_COLS / np;
+  struct Pass {
+    int c0, c1, r0, k0, steps, lo, hi;      // columns of the part; first rank in it; first column and steps of this CTA; ranks in u
+  };
+  auto pass_of = [&](int i) {
+    const LoraSeg& seg = a.down_seg[i / each];
+    const int r0 = i % each * np, all = (seg.c1 - seg.c0 + DOWN_K - 1) / DOWN_K, per = (all + C - 1) / C, first = min(all, c * per);
+    return Pass{seg.c0, seg.c1, r0, seg.c0 + first * DOWN_K, min(all, first + per) - first, seg.u0 + r0, min(seg.u0 + r0 + np, seg.u0 + seg.ru)};
+  };
   bool pending = false;
   for (int unit = cid % a.groups; unit < (units.mixed ? 0 : units.total); unit += a.groups) {
     const int ad = units.ad[unit], m = units.rows[unit];
@@ -687,105 +725,125 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_down_kernel(const __grid
     const short* order = units.order + units.base[unit];
     const __nv_bfloat16* wd = reinterpret_cast<const __nv_bfloat16*>(a.down) + (long long)ad * a.down_adapter;
     const float s = a.scale ? a.scale[ad] : a.scale_all;
-    const __nv_bfloat16* xr[4];      // a thread copies the same piece of four rows in every step
+    const bool line = tma && order[m - 1] - order[0] == m - 1;      // neighbouring rows; those behind the unit's come along and are not looked at
+    for (int pass0 = 0; pass0 < passes; pass0 += at_once) {
+      const int pass1 = min(passes, pass0 + at_once);
+      int steps = 0;
+      for (int i = pass0; i < pass1; ++i) steps += pass_of(i).steps;
+      // the pass that a step belongs to (steps come in order)
+      struct At {
+        Pass p;
+        int i, base;
+      };
+      const At start{pass_of(pass0), pass0, 0};
+      auto go = [&](At& at, int step) {
+        while (step - at.base >= at.p.steps) {
+          at.base += at.p.steps;
+          at.p = pass_of(++at.i);
+        }
+        return step - at.base;
+      };
+      At fed = start, loaded = start;
+      if (pending) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");      // every CTA has read the last parts
+      pending = false;
+      auto feed = [&](uint32_t src, int step) {
+        step = go(fed, step);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int tok = (tid >> 3) + 32 * i;
-      xr[i] = tok < m ? x + (row0 + order[tok]) * a.ldx + 8 * (tid & 7) : nullptr;
-    }
-    const uint32_t piece = 16 * ((tid & 7) ^ ((tid >> 3) & 7));
-    for (int sg = 0; sg < a.down_segs; ++sg) {
-      const LoraSeg seg = a.down_seg[sg];
-      const int all = (seg.c1 - seg.c0 + DOWN_K - 1) / DOWN_K, per = (all + C - 1) / C;
-      const int k0 = seg.c0 + min(all, c * per) * DOWN_K, steps = min(all, (c + 1) * per) - min(all, c * per);
-      for (int r0 = 0; r0 < seg.ru; r0 += np) {
-        if (pending) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");      // every CTA has read the last parts
+        for (int q = 0; q < DOWN_K / 16; ++q)
+          umma_f16_ss(ring.tmem + (fed.i - pass0) * np, umma_smem_desc_sw128(src + 32 * q, 16, 1024),
+                      umma_smem_desc_sw128(src + DOWN_X + (DOWN_T ? 2048 : 32) * q, DOWN_T ? 8192 : 16, 1024), idesc, step || q);
+      };
+      if (line) {
+        const int at_row = (int)row0 + order[0];
+        auto load = [&](uint32_t dst, uint32_t bar, int step) {
+          const int k = go(loaded, step) * DOWN_K + loaded.p.k0;
+          const Pass& p = loaded.p;
+          tma_load_2d(dst, &map_x, bar, k, at_row);
+          if constexpr (!DOWN_T) tma_load_3d(dst + DOWN_X, &map_w, bar, k, p.r0, ad);
+          else tma_load_3d(dst + DOWN_X, &map_w, bar, p.r0, k, ad);
+        };
+        ring_tma(ring, steps, down_stage(np, DOWN_T), load, feed);
+      } else {
+        const __nv_bfloat16* xr[4];      // a thread copies the same piece of four rows in every step
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int tok = (tid >> 3) + 32 * i;
+          xr[i] = tok < m ? x + (row0 + order[tok]) * a.ldx + 8 * (tid & 7) : nullptr;
+        }
+        const uint32_t piece = 16 * ((tid & 7) ^ ((tid >> 3) & 7));
         auto fill = [&](uint32_t dst, int step) {
-          const int k = k0 + step * DOWN_K;
+          const int k = go(loaded, step) * DOWN_K + loaded.p.k0, ru = loaded.p.hi - loaded.p.lo;
+          const Pass& p = loaded.p;
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            cp_async<16>(dst + ((tid >> 3) + 32 * i) * 128 + piece, xr[i] ? xr[i] + k : x, xr[i] && k + 8 * (tid & 7) < seg.c1);
+            cp_async<16>(dst + ((tid >> 3) + 32 * i) * 128 + piece, xr[i] ? xr[i] + k : x, xr[i] && k + 8 * (tid & 7) < p.c1);
           const uint32_t wdst = dst + DOWN_X;
           if constexpr (!DOWN_T) {
             for (int i = tid; i < np * 8; i += LORA_THREADS) {
               const int rank = i >> 3, col = k + 8 * (i & 7);
-              const bool ok = r0 + rank < seg.ru && col < seg.c1;
-              cp_async<16>(wdst + rank * 128 + 16 * ((i & 7) ^ (rank & 7)), ok ? wd + (long long)(seg.u0 + r0 + rank) * a.ld_down + col : wd, ok);
+              const bool ok = rank < ru && col < p.c1;
+              cp_async<16>(wdst + rank * 128 + 16 * ((i & 7) ^ (rank & 7)), ok ? wd + (long long)(p.r0 + rank) * a.ld_down + col : wd, ok);
             }
           } else {
-            for (int i = tid; i < DOWN_K * (np / 4); i += LORA_THREADS) {
-              const int kk = i / (np / 4), rank = 4 * (i % (np / 4));
-              const bool ok = k + kk < seg.c1 && r0 + rank < seg.ru;
+            for (int i = tid; i < DOWN_K * 16; i += LORA_THREADS) {
+              const int kk = i >> 4, rank = 4 * (i & 15);
+              const bool ok = k + kk < p.c1 && rank < ru;
               cp_async<8>(wdst + kk * 128 + 16 * ((rank >> 3) ^ (kk & 7)) + 2 * (rank & 7),
-                          ok ? wd + (long long)(k + kk) * a.ld_down + r0 + rank : wd, ok);
+                          ok ? wd + (long long)(k + kk) * a.ld_down + p.r0 + rank : wd, ok);
             }
           }
         };
-        auto feed = [&](uint32_t src, int step) {
-#pragma unroll
-          for (int q = 0; q < DOWN_K / 16; ++q)
-            umma_f16_ss(ring.tmem, umma_smem_desc_sw128(src + 32 * q, 16, 1024),
-                        umma_smem_desc_sw128(src + DOWN_X + (DOWN_T ? 2048 : 32) * q, DOWN_T ? 8192 : 16, 1024), idesc, step || q);
-        };
-        if (tma && order[m - 1] - order[0] == m - 1) {      // rows behind the unit's come along and are not looked at
-          const int at_row = (int)row0 + order[0];
-          auto load = [&](uint32_t dst, uint32_t bar, int step) {
-            const int k = k0 + step * DOWN_K;
-            tma_load_2d(dst, &map_x, bar, k, at_row);
-            if constexpr (!DOWN_T) tma_load_3d(dst + DOWN_X, &map_w, bar, k, seg.u0 + r0, ad);
-            else tma_load_3d(dst + DOWN_X, &map_w, bar, r0, k, ad);
-          };
-          ring_tma(ring, steps, down_stage(np, DOWN_T), load, feed);
-        } else {
-          ring_gather(ring, steps, fill, feed);
-        }
-        __syncthreads();      // part takes the stages' place
-        if (w < 4) {
-          float* dst = part + (32 * w + lane) * pstride;
-          for (int r = 0; r < np; r += 16) {
+        ring_gather(ring, steps, fill, feed);
+      }
+      __syncthreads();      // part takes the stages' place
+      if (w < 4) {
+        float* dst = part + (32 * w + lane) * pstride;
+        for (int i = pass0; i < pass1; ++i) {
+          const bool any = pass_of(i).steps;
+          for (int r = (i - pass0) * np; r < (i - pass0 + 1) * np; r += 16) {
             uint32_t v[16];
             tmem_ld_32x32b_x16(ring.tmem + (uint32_t(32 * w) << 16) + r, v);
             tc_wait_ld();
 #pragma unroll
             for (int j = 0; j < 16; j += 4)
-              *reinterpret_cast<uint4*>(dst + r + j) = steps ? make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]) : make_uint4(0, 0, 0, 0);
-          }
-          tc_fence_before();
-        }
-        cluster_sync_all();
-        tc_fence_after();
-        // ---- each CTA adds up and writes its share
-        const int r16 = round16(a.up_seg[0].ru), lo = seg.u0 + r0, hi = min(lo + np, seg.u0 + seg.ru);
-        for (int e = c * LORA_THREADS + tid; e < m * a.ucols; e += C * LORA_THREADS) {
-          const int tok = e / a.ucols, col = e - tok * a.ucols;
-          const int p = a.up_segs > 1 ? col / r16 : 0, j = col - p * r16, rank = a.up_seg[p].u0 + j;
-          const bool pad = j >= a.up_seg[p].ru;
-          if (pad ? sg > 0 || r0 > 0 : rank < lo || rank >= hi) continue;
-          float v = 0.f;
-          if (!pad) {
-            for (int k = 0; k < C; ++k) v += cluster.map_shared_rank(part, k)[tok * pstride + rank - lo];
-            v *= s;
-          }
-          unsigned short* dst = a.u + (row0 + order[tok]) * a.ucols + col;
-          if (parts == 2) {
-            uint32_t q[2];
-            split<2>(v, q);
-            dst[0] = (unsigned short)q[0];
-            dst[(long long)a.T * a.ucols] = (unsigned short)q[1];
-          } else {
-            uint32_t q[3];
-            split<3>(v, q);
-#pragma unroll
-            for (int k = 0; k < 3; ++k) dst[(long long)k * a.T * a.ucols] = (unsigned short)q[k];
+              *reinterpret_cast<uint4*>(dst + r + j) = any ? make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]) : make_uint4(0, 0, 0, 0);
           }
         }
-        asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-        pending = true;
+        tc_fence_before();
       }
+      cluster_sync_all();
+      tc_fence_after();
+      // ---- each CTA adds up and writes its share
+      const int r16 = round16(a.up_seg[0].ru), lo = pass_of(pass0).lo, hi = pass_of(pass1 - 1).hi;
+      for (int e = c * LORA_THREADS + tid; e < m * a.ucols; e += C * LORA_THREADS) {
+        const int tok = e / a.ucols, col = e - tok * a.ucols;
+        const int p = a.up_segs > 1 ? col / r16 : 0, j = col - p * r16, rank = a.up_seg[p].u0 + j;
+        const bool pad = j >= a.up_seg[p].ru;
+        if (pad ? pass0 > 0 : rank < lo || rank >= hi) continue;
+        float v = 0.f;
+        if (!pad) {
+          const int of = rank / a.down_seg[0].ru, in = rank - of * a.down_seg[0].ru;      // part and rank in it
+          v = s * cluster_sum(smem_u32(part + tok * pstride + (of * each + in / np - pass0) * np + in % np), C);
+        }
+        unsigned short* dst = a.u + (row0 + order[tok]) * a.ucols + col;
+        if (parts == 2) {
+          uint32_t q[2];
+          split<2>(v, q);
+          dst[0] = (unsigned short)q[0];
+          dst[(long long)a.T * a.ucols] = (unsigned short)q[1];
+        } else {
+          uint32_t q[3];
+          split<3>(v, q);
+#pragma unroll
+          for (int k = 0; k < 3; ++k) dst[(long long)k * a.T * a.ucols] = (unsigned short)q[k];
+        }
+      }
+      asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+      pending = true;
     }
   }
   if (pending) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-  ring_end(ring, 64);
+  ring_end(ring, DOWN_COLS);
 }
 
 // --------------------------------------------------------------------------------------------------- many rows: u onto y
@@ -1204,8 +1262,7 @@ __device__ __forceinline__ void write_grad(cg::cluster_group& cluster, const Gra
   for (int e = c * share + threadIdx.x; e < min(all, (c + 1) * share); e += LORA_THREADS) {
     const int rank = job.across ? e % ranks : e / GRAD_COLS, col = job.across ? e / ranks : e % GRAD_COLS;
     if (t.r0 + rank >= job.ru || t.col0 + col >= job.c1) continue;
-    float v = 0.f;
-    for (int k = 0; k < C; ++k) v += cluster.map_shared_rank(tile, k)[rank * GRAD_STRIDE + col];
+    const float v = cluster_sum(smem_u32(tile + rank * GRAD_STRIDE + col), C);
     const long long pos = (long long)ad * job.out_adapter + (job.across ? (long long)(t.col0 + col) * job.ld_out + t.r0 + rank
                                                                          : (long long)(job.u0 + t.r0 + rank) * job.ld_out + t.col0 + col);
     if (a.out_f32) {
@@ -1485,14 +1542,14 @@ EDL_HOST_API int edl_lora_apply(const void* x, long long ldx, const void* y, lon
     int ru = 0, cols = 0;
     for (int i = 0; i < g.down_segs; ++i) {
       ru = g.down_seg[i].ru > ru ? g.down_seg[i].ru : ru;
-      cols = g.down_seg[i].c1 - g.down_seg[i].c0 > cols ? g.down_seg[i].c1 - g.down_seg[i].c0 : cols;
+      cols += g.down_seg[i].c1 - g.down_seg[i].c0;
     }
     const int np = ru < DOWN_RANKS ? round16(ru) : DOWN_RANKS;
     // as many CTAs as run at once (two per SM), each with at least four steps of columns
     int cluster = 1;
     while (cluster < 8 && (long long)((T + DOWN_ROWS - 1) / DOWN_ROWS) * cluster * 2 <= 2 * sms && cols >= 2 * cluster * 4 * DOWN_K) cluster *= 2;
     const dim3 grid((unsigned)((long long)blocks * g.groups * cluster));
-    const int ring = RING_STAGES * down_stage(np, backward), part = DOWN_ROWS * (np + 4) * 4, down_smem = (ring > part ? ring : part) + 1024;
+    const int ring = RING_STAGES * down_stage(np, backward), part = DOWN_ROWS * (DOWN_COLS + 4) * 4, down_smem = (ring > part ? ring : part) + 1024;
     // TMA takes weights whose rows start on 16 bytes; a box of the backward pass must not reach into the next part's columns
     bool tma = !backward || (r % 8 == 0 && ldb % 8 == 0 && b_adapter % 8 == 0 && aligned(b, 16));
     for (int p = 0; backward && p + 1 < parts; ++p) tma = tma && widths[p] % DOWN_K == 0;
