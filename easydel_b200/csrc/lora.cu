@@ -957,13 +957,30 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_up_any_kernel(const __gr
   }
 }
 
+// 64 bytes of a row: two 32-byte stores where rows start on 32 bytes, so that every sector is written once.
+__device__ __forceinline__ void store_64(void* p, const uint32_t (&v)[16], bool wide) {
+  uint4* q = reinterpret_cast<uint4*>(p);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t* r = v + 8 * i;
+    if (wide) {
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(q + 2 * i), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+                   "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+    } else {
+      q[2 * i] = make_uint4(r[0], r[1], r[2], r[3]);
+      q[2 * i + 1] = make_uint4(r[4], r[5], r[6], r[7]);
+    }
+  }
+}
+
 // The same on tcgen05: 128 rows of one adapter are the M side, 64 columns at a time the N side, the ranks of both parts of u the inner index.
-// A lane loads tiles of y and of the weights ahead (TMA), a lane of the second warp issues the products into one of two
-// accumulators, and eight warps add them to y in shared memory, a row per lane, and write whole row segments out. What bounds it is the
-// traffic of y and out: a 16-byte piece costs about 30 instructions of a lane, a seventh of what `mma.sync` fragments took.
+// A lane loads tiles of y and of the weights ahead (TMA), a lane of the second warp issues the products into one of two accumulators, and
+// eight warps, a row per lane and half a tile's columns each, add them to y and write out. What bounds it is the traffic of y and out. Rows
+// of y that lanes asked for themselves, two tiles ahead, took a third longer than by TMA; rows of out that went through shared memory
+// to leave as whole lines took a fifth longer than 64 bytes from each lane.
 constexpr int UP_THREADS = 320, UP_ROWS = 128, UP_TILE = 64, UP_STAGES = 3;
-constexpr int UP_Y = UP_ROWS * UP_TILE * 2, UP_W = 64 * 128, UP_U = UP_ROWS * 128;
-constexpr int UP_SMEM = UP_STAGES * (UP_Y + UP_W) + 2 * UP_U + 1024;
+constexpr int UP_Y = UP_ROWS * UP_TILE * 2, UP_W = 64 * 128, UP_STAGE = UP_Y + UP_W, UP_U = UP_ROWS * 128;
+constexpr int UP_SMEM = UP_STAGES * UP_STAGE + 2 * UP_U + 1024;
 
 template <bool UP_T>
 __global__ void __launch_bounds__(UP_THREADS, 2) lora_up_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ CUtensorMap map_y,
@@ -974,7 +991,7 @@ __global__ void __launch_bounds__(UP_THREADS, 2) lora_up_kernel(const __grid_con
   __shared__ int s_abort;
   extern __shared__ uint8_t raw[];
   uint8_t* dyn = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  const uint32_t stages = smem_u32(dyn), su = stages + UP_STAGES * (UP_Y + UP_W);
+  const uint32_t stages = smem_u32(dyn), su = stages + UP_STAGES * UP_STAGE;
   const uint32_t full = smem_u32(s_bars), empty = full + 8 * UP_STAGES, dfull = empty + 8 * UP_STAGES, dempty = dfull + 16, ufull = dempty + 16,
                  ufree = ufull + 8;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
@@ -982,7 +999,7 @@ __global__ void __launch_bounds__(UP_THREADS, 2) lora_up_kernel(const __grid_con
   if (tid == 0) {
     for (int i = 0; i < UP_STAGES; ++i) {
       mbar_init(full + 8 * i, 1);
-      mbar_init(empty + 8 * i, 8);
+      mbar_init(empty + 8 * i, 9);      // the products and eight warps
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(dfull + 8 * i, 1);
@@ -1006,139 +1023,148 @@ __global__ void __launch_bounds__(UP_THREADS, 2) lora_up_kernel(const __grid_con
   volatile int* abort_flag = &s_abort;
   auto wait = [&](uint32_t bar, int use, int code) { mbar_wait(bar, use & 1, abort_flag, a.status, code); };
 
-  // Every role walks the same runs: a unit's tiles within one part (whose u they share). `runs` counts those with an adapter, `tiles` all tiles.
-  auto walk = [&](auto begin, auto each, auto end) {
-    int runs = 0, tiles = 0;
+  // Every role walks the same runs: a unit's tiles within one part, whose u they share. Rows without an adapter are copied by the eight
+  // warps alone.
+  struct Run {
+    int ad, m, p, n0, count, run, tile;      // first column, tiles; number of this run and of its first tile
+    const short* order;
+  };
+  auto walk = [&](auto f) {
+    Run r{};
     for (int unit = 0; unit < (units.mixed ? 0 : units.total); ++unit) {
-      const int ad = units.ad[unit], m = units.rows[unit];
-      const short* order = units.order + units.base[unit];
-      const bool line = order[m - 1] - order[0] == m - 1;      // neighbouring rows
+      r.ad = units.ad[unit];
+      r.m = units.rows[unit];
+      r.order = units.order + units.base[unit];
       int first = 0;      // of part p's tiles
-      for (int p = 0; p < a.up_segs; ++p) {
-        const int c0 = a.up_seg[p].c0, last = first + (a.up_seg[p].c1 - c0 + UP_TILE - 1) / UP_TILE;
-        const int lo = max(first, tile0), hi = min(last, tile1);
-        if (lo < hi) {
-          if (ad >= 0) begin(ad, m, order, line, p, runs);
-          for (int t = lo; t < hi; ++t, ++tiles) each(ad, m, order, line, p, c0 + (t - first) * UP_TILE, tiles);
-          if (ad >= 0) end(runs++);
-        }
+      for (r.p = 0; r.p < a.up_segs; ++r.p) {
+        const int c0 = a.up_seg[r.p].c0, last = first + (a.up_seg[r.p].c1 - c0 + UP_TILE - 1) / UP_TILE;
+        const int lo = max(first, tile0);
+        r.count = min(last, tile1) - lo;
+        r.n0 = c0 + (lo - first) * UP_TILE;
         first = last;
+        if (r.count <= 0) continue;
+        f(r);
+        if (r.ad >= 0) {
+          ++r.run;
+          r.tile += r.count;
+        }
       }
     }
   };
+  auto line = [](const Run& r) { return r.order[r.m - 1] - r.order[0] == r.m - 1; };      // neighbouring rows
   if (w == 0) {
     if (elect_one()) {
-      walk(
-          [&](int ad, int m, const short* order, bool line, int p, int run) {
-            if (run) wait(ufree, run - 1, EDL_TIMEOUT_PRODUCER);
-            if (!line) return;
-            mbar_expect_tx(ufull, 2 * UP_U);
-            for (int s = 0; s < 2; ++s) tma_load_3d(su + s * UP_U, &map_u, ufull, p * r16, (int)row0 + order[0], s);
-          },
-          [&](int ad, int m, const short* order, bool line, int p, int n0, int tile) {
-            const int at = tile % UP_STAGES, use = tile / UP_STAGES;
-            if (use) wait(empty + 8 * at, use - 1, EDL_TIMEOUT_PRODUCER);
-            const uint32_t dst = stages + at * (UP_Y + UP_W), bar = full + 8 * at;
-            const bool read = a.y && line;
-            mbar_expect_tx(bar, (read ? UP_Y : 0) + (ad < 0 ? 0 : UP_T ? r16 * 128 : UP_W));
-            if (read) tma_load_2d(dst, &map_y, bar, n0, (int)row0 + order[0]);
-            if (ad >= 0) {
-              if constexpr (UP_T) tma_load_3d(dst + UP_Y, &map_w, bar, n0, 0, ad);
-              else tma_load_3d(dst + UP_Y, &map_w, bar, 0, n0, ad);
-            }
-          },
-          [](int) {});
+      walk([&](const Run& r) {
+        if (r.ad < 0) return;
+        if (line(r)) {
+          if (r.run) wait(ufree, r.run - 1, EDL_TIMEOUT_PRODUCER);
+          mbar_expect_tx(ufull, 2 * UP_U);
+          for (int s = 0; s < 2; ++s) tma_load_3d(su + s * UP_U, &map_u, ufull, r.p * r16, (int)row0 + r.order[0], s);
+        }
+        for (int t = 0; t < r.count; ++t) {
+          const int tile = r.tile + t, at = tile % UP_STAGES, use = tile / UP_STAGES;
+          if (use) wait(empty + 8 * at, use - 1, EDL_TIMEOUT_PRODUCER);
+          const uint32_t dst = stages + at * UP_STAGE, bar = full + 8 * at;
+          const bool read = a.y && line(r);
+          mbar_expect_tx(bar, (UP_T ? r16 * 128 : UP_W) + (read ? UP_Y : 0));
+          if (read) tma_load_2d(dst, &map_y, bar, r.n0 + t * UP_TILE, (int)row0 + r.order[0]);
+          if constexpr (UP_T) tma_load_3d(dst + UP_Y, &map_w, bar, r.n0 + t * UP_TILE, 0, r.ad);
+          else tma_load_3d(dst + UP_Y, &map_w, bar, 0, r.n0 + t * UP_TILE, r.ad);
+        }
+      });
     }
     __syncwarp();
   } else if (w == 1) {
     const bool leader = elect_one();
     const uint32_t idesc = umma_idesc_bf16(UP_ROWS, UP_TILE, 0, UP_T);
-    walk([&](int, int, const short*, bool, int, int run) { wait(ufull, run, EDL_TIMEOUT_MMA); },
-         [&](int ad, int, const short*, bool, int, int, int tile) {
-           const int at = tile % UP_STAGES, buf = tile & 1;
-           wait(full + 8 * at, tile / UP_STAGES, EDL_TIMEOUT_MMA);
-           if (tile > 1) wait(dempty + 8 * buf, tile / 2 - 1, EDL_TIMEOUT_MMA);
-           tc_fence_after();
-           if (!leader) return;
-           const uint32_t src = stages + at * (UP_Y + UP_W) + UP_Y;
-           for (int s = 1; ad >= 0 && s >= 0; --s)
-             for (int k = 0; k < r16 / 16; ++k)
-               umma_f16_ss(tmem + buf * UP_TILE, umma_smem_desc_sw128(su + s * UP_U + 32 * k, 16, 1024),
-                           umma_smem_desc_sw128(src + (UP_T ? 2048 : 32) * k, UP_T ? 8192 : 16, 1024), idesc, s == 0 || k);
-           tc_commit(dfull + 8 * buf);
-         },
-         [&](int) {
-           if (leader) tc_commit(ufree);
-         });
+    walk([&](const Run& r) {
+      if (r.ad < 0) return;
+      wait(ufull, r.run, EDL_TIMEOUT_MMA);
+      for (int t = 0; t < r.count; ++t) {
+        const int tile = r.tile + t, at = tile % UP_STAGES, buf = tile & 1;
+        wait(full + 8 * at, tile / UP_STAGES, EDL_TIMEOUT_MMA);
+        if (tile > 1) wait(dempty + 8 * buf, tile / 2 - 1, EDL_TIMEOUT_MMA);
+        tc_fence_after();
+        if (leader) {
+          const uint32_t src = stages + at * UP_STAGE + UP_Y;
+          for (int s = 1; s >= 0; --s)
+            for (int k = 0; k < r16 / 16; ++k)
+              umma_f16_ss(tmem + buf * UP_TILE, umma_smem_desc_sw128(su + s * UP_U + 32 * k, 16, 1024),
+                          umma_smem_desc_sw128(src + (UP_T ? 2048 : 32) * k, UP_T ? 8192 : 16, 1024), idesc, s == 0 || k);
+          tc_commit(empty + 8 * at);
+          tc_commit(dfull + 8 * buf);
+          if (t == r.count - 1) tc_commit(ufree);
+        }
+      }
+    });
     __syncwarp();
   } else {
-    const int q = w & 3, h = (w - 2) >> 2, r = 32 * q + lane;      // this lane's row of a tile; which 32 of its columns
-    walk(
-        [&](int, int m, const short* order, bool line, int p, int run) {
-          if (line) return;
-          if (run) wait(ufree, run - 1, EDL_TIMEOUT_EPILOGUE);
-          for (int i = tid - 64; i < 2 * UP_ROWS * (r16 / 8); i += 256) {
-            const int j = i % (r16 / 8), tok = i / (r16 / 8) % UP_ROWS, s = i / (r16 / 8 * UP_ROWS);
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (tok < m) v = *reinterpret_cast<const uint4*>(a.u + ((long long)s * a.T + row0 + order[tok]) * a.ucols + p * r16 + 8 * j);
-            *reinterpret_cast<uint4*>(dyn + (su - stages) + s * UP_U + tok * 128 + 16 * (j ^ (tok & 7))) = v;
-          }
-          fence_proxy_async_smem();
-          asm volatile("bar.sync 1, 256;" ::: "memory");
-          if (tid == 64) mbar_arrive(ufull);
-        },
-        [&](int ad, int m, const short* order, bool line, int p, int n0, int tile) {
-          const int at = tile % UP_STAGES, buf = tile & 1;
-          uint8_t* box = dyn + at * (UP_Y + UP_W);
+    const int q = w & 3, h = (w - 2) >> 2, i = 32 * q + lane;      // this lane's row of a unit; which 32 columns of a tile
+    const bool wide = a.ldo % 16 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
+    walk([&](const Run& r) {
+      if (r.ad >= 0 && !line(r)) {      // u of rows that are no neighbours
+        if (r.run) wait(ufree, r.run - 1, EDL_TIMEOUT_EPILOGUE);
+        for (int e = tid - 64; e < 2 * UP_ROWS * (r16 / 8); e += 256) {
+          const int j = e % (r16 / 8), tok = e / (r16 / 8) % UP_ROWS, s = e / (r16 / 8 * UP_ROWS);
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (tok < r.m) v = *reinterpret_cast<const uint4*>(a.u + ((long long)s * a.T + row0 + r.order[tok]) * a.ucols + r.p * r16 + 8 * j);
+          *reinterpret_cast<uint4*>(dyn + UP_STAGES * UP_STAGE + s * UP_U + tok * 128 + 16 * (j ^ (tok & 7))) = v;
+        }
+        fence_proxy_async_smem();
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (tid == 64) mbar_arrive(ufull);
+      }
+      const long long row = row0 + (i < r.m ? r.order[i] : 0);
+      const int col0 = r.n0 + 32 * h, left = a.up_seg[r.p].c1 - col0;      // columns of this lane, tile after tile
+      const __nv_bfloat16* y = reinterpret_cast<const __nv_bfloat16*>(a.y) + row * a.ldy + col0;
+      __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + row * a.ldo + col0;
+      const bool boxed = a.y && r.ad >= 0 && line(r), wide_r = wide && col0 % 16 == 0;
+      for (int t = 0; t < r.count; ++t) {
+        const int tile = r.tile + t, at = tile % UP_STAGES, buf = tile & 1, have = left - t * UP_TILE;
+        uint32_t v[16];      // y, then out
+        if (boxed) {
           wait(full + 8 * at, tile / UP_STAGES, EDL_TIMEOUT_EPILOGUE);
+          const uint8_t* box = dyn + at * UP_STAGE + i * 128;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint4 x = *reinterpret_cast<const uint4*>(box + 16 * ((4 * h + e) ^ (i & 7)));
+            v[4 * e] = x.x; v[4 * e + 1] = x.y; v[4 * e + 2] = x.z; v[4 * e + 3] = x.w;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (a.y && i < r.m && have > 8 * e) x = *reinterpret_cast<const uint4*>(y + t * UP_TILE + 8 * e);
+            v[4 * e] = x.x; v[4 * e + 1] = x.y; v[4 * e + 2] = x.z; v[4 * e + 3] = x.w;
+          }
+        }
+        if (r.ad >= 0) {
+          uint32_t d[32];
           wait(dfull + 8 * buf, tile / 2, EDL_TIMEOUT_EPILOGUE);
           tc_fence_after();
-          uint32_t d[32];
           tmem_ld_32x32b_x32(tmem + (uint32_t(32 * q) << 16) + buf * UP_TILE + 32 * h, d);
-          // rows as they leave: eight rows of four pieces at a time
-          const int sub = 4 * ((lane >> 2) & 1) + (lane >> 3), piece = 4 * h + (lane & 3);
-          const bool col = n0 + 8 * piece < a.up_seg[p].c1;
-          if (a.y && !line) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int rr = 32 * q + 8 * i + sub;
-              if (rr < m && col)
-                *reinterpret_cast<uint4*>(box + rr * 128 + 16 * (piece ^ (rr & 7))) =
-                    *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.y) + (row0 + order[rr]) * a.ldy + n0 + 8 * piece);
-            }
-            __syncwarp();
-          }
           tc_wait_ld();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(dempty + 8 * buf);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint4* slot = reinterpret_cast<uint4*>(box + r * 128 + 16 * ((4 * h + i) ^ (r & 7)));
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (a.y) v = *slot;
-            if (ad >= 0) {
-              uint32_t* e = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                e[k] = pack_bf16x2(__uint_as_float(e[k] << 16) + __uint_as_float(d[8 * i + 2 * k]),
-                                   __uint_as_float(e[k] & 0xffff0000u) + __uint_as_float(d[8 * i + 2 * k + 1]));
-            }
-            *slot = v;
+          if (lane == 0) {
+            mbar_arrive(dempty + 8 * buf);
+            mbar_arrive(empty + 8 * at);
           }
-          __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int rr = 32 * q + 8 * i + sub;
-            if (rr < m && col)
-              *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(a.out) + (row0 + order[rr]) * a.ldo + n0 + 8 * piece) =
-                  *reinterpret_cast<const uint4*>(box + rr * 128 + 16 * (piece ^ (rr & 7)));
+          for (int e = 0; e < 16; ++e)
+            v[e] = pack_bf16x2(__uint_as_float(v[e] << 16) + __uint_as_float(d[2 * e]), __uint_as_float(v[e] & 0xffff0000u) + __uint_as_float(d[2 * e + 1]));
+        }
+        if (i < r.m) {
+          if (have >= 32) {
+            store_64(out + t * UP_TILE, v, wide_r);
+          } else {      // the last columns of a part
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (have > 8 * e) *reinterpret_cast<uint4*>(out + t * UP_TILE + 8 * e) = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(empty + 8 * at);
-        },
-        [](int) {});
+        }
+      }
+    });
   }
   tc_fence_before();
   __syncthreads();
@@ -1564,7 +1590,7 @@ EDL_HOST_API int edl_lora_apply(const void* x, long long ldx, const void* y, lon
                  : launch_cluster(lora_down_kernel<false>, grid, cluster, down_smem, st, "lora down launch", g, map_x, map_w, (int)tma, s, np))
       return -1;
     if (out) {
-      const int r16 = round16(g.up_seg[0].ru), columns = backward ? K : N;
+      const int r16 = round16(g.up_seg[0].ru);
       const bool tiles = r16 <= 64 && !y_f32 && (backward || (r % 8 == 0 && ldb % 8 == 0 && b_adapter % 8 == 0 && aligned(b, 16)));
       const int width = tiles ? UP_TILE : UP_COLS;
       g.groups = 0;
@@ -1577,7 +1603,7 @@ EDL_HOST_API int edl_lora_apply(const void* x, long long ldx, const void* y, lon
         if (g.splits < 1) g.splits = 1;
         g.splits = (g.groups + (g.groups + g.splits - 1) / g.splits - 1) / ((g.groups + g.splits - 1) / g.splits);
         CUtensorMap map_y{}, map_u{};
-        if (y && make_tmap_2d_16b(&map_y, y, T, columns, ldy, UP_ROWS, UP_TILE)) return -1;
+        if (y && make_tmap_2d_16b(&map_y, y, T, backward ? K : N, ldy, UP_ROWS, UP_TILE)) return -1;
         if (make_tmap_3d_16b(&map_u, u, g.ucols, T, 2, g.ucols, (uint64_t)T * g.ucols, 64, UP_ROWS, 1, 3)) return -1;
         if (backward ? make_tmap_3d_16b(&map_w, a, K, parts * r, n, lda, a_adapter, UP_TILE, r16, 1, 3)
                      : make_tmap_3d_16b(&map_w, b, r, N, n, ldb, b_adapter, 64, UP_TILE, 1, 3))
@@ -1692,8 +1718,18 @@ EDL_HOST_API int edl_lora_grads(const void* x, long long ldx, const void* dy, lo
     job.tiles = ((job.c1 - job.c0 + GRAD_COLS - 1) / GRAD_COLS) * ((job.ru + rp - 1) / rp);
     tiles += job.tiles;
   }
-  int cluster = 8;      // rows are cut into as many shares; short inputs need fewer
-  while (cluster > 1 && a.T < cluster * 32) cluster /= 2;
+  // Rows are cut over the CTAs of a cluster. Clusters have to fit the GPU's parts, which leaves about 7 of 8 places (two per SM); a
+  // turn of CTAs takes its steps of 32 rows and about as long as 6 more to start and to add up.
+  int cluster = 1;
+  const long long places = 2LL * sm_count() * 7 / 8;
+  long long best = 0;
+  for (int c = 1; c <= 8; c *= 2) {
+    const long long cost = (((long long)tiles * n * c + places - 1) / places) * (6 + (a.T + 32LL * c - 1) / (32LL * c));
+    if (c == 1 || cost < best) {
+      best = cost;
+      cluster = c;
+    }
+  }
   cudaStream_t st = (cudaStream_t)stream;
   const dim3 grid((unsigned)(tiles * cluster), (unsigned)n);
   const char* what = "lora gradient launch";
