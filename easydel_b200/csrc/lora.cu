@@ -1511,18 +1511,23 @@ bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) 
 
 using namespace edl;
 
-// x [T, K], y and out [T, N] (y null: the adapters' part alone; y == out: in place), row strides in elements. widths: columns of the
-// `parts` parts of N. a: [n][parts * r][K], b: [n][N][r] with strides. backward = 0: out = y + s (x a^T) b^T. backward = 1: x is dy [T, N],
-// out dx [T, K] (null: u alone), y null. u: s x a^T or s dy b in bf16 parts (2 for bf16 results, 3 for fp32 ones), [parts][T][columns] with
-// parts * r rounded up to 16 per part (forward) or as a whole (backward); asked for above 256 rows of bf16, else it may be null.
-// mixed: a flag per 256 rows, scratch; asked for above 256 rows of bf16 with an index. index [T] int32 or null (adapter 0 everywhere), scale
-// [n] fp32 or null (scale_all). x_f32: x and the weights are fp32 (then
-// y and out too), else bf16; y_f32: type of y and out. Indexes from n on set the status word and count as none.
-EDL_HOST_API int edl_lora_apply(const void* x, long long ldx, const void* y, long long ldy, void* out, long long ldo, const void* a,
-                                long long a_adapter, long long lda, const void* b, long long b_adapter, long long ldb,
-                                const int* index, const float* scale, float scale_all, void* u, long long u_size, int* mixed, int T,
-                                int K, int N, int n, int r, int parts, const int* widths, int x_f32, int y_f32, int backward, int* status,
-                                void* stream) {
+// Sizes of a call: strides in elements, `widths` columns of the `parts` parts of N. x_f32: x and the weights are fp32 (then y and out
+// too), else bf16; y_f32: type of y and out.
+struct edl_lora_shape {
+  long long ldx, ldy, ldo, a_adapter, lda, b_adapter, ldb;
+  int T, K, N, n, r, parts, x_f32, y_f32, backward, widths[8];
+};
+
+// x [T, K], y and out [T, N] (y null: the adapters' part alone; y == out: in place). a: [n][parts * r][K], b: [n][N][r].
+// backward = 0: out = y + s (x a^T) b^T. backward = 1: x is dy [T, N], out dx [T, K] (null: u alone), y null. u: s x a^T or s dy b
+// in bf16 parts (2 for bf16 results, 3 for fp32 ones), [parts][T][columns] with parts * r rounded up to 16 per part (forward) or as a
+// whole (backward); asked for above 256 rows of bf16, else it may be null. mixed: a flag per 256 rows, scratch; asked for above 256 rows of
+// bf16 with an index. index [T] int32 or null (adapter 0 everywhere), scale [n] fp32 or null (scale_all). Indexes from n on set the status
+// word and count as none.
+EDL_HOST_API int edl_lora_apply(const edl_lora_shape* shape, const void* x, const void* y, void* out, const void* a, const void* b,
+                                const int* index, const float* scale, float scale_all, void* u, long long u_size, int* mixed,
+                                int* status, void* stream) {
+  const auto [ldx, ldy, ldo, a_adapter, lda, b_adapter, ldb, T, K, N, n, r, parts, x_f32, y_f32, backward, widths] = *shape;
   if (T <= 0) return 0;
   if (K <= 0 || N <= 0 || n <= 0 || r <= 0 || parts < 1 || parts > LORA_SEGS || r > 512 / parts) {
     set_last_error("edl_lora_apply: needs sizes above 0, up to %d parts and parts x rank up to 512", LORA_SEGS);
@@ -1705,13 +1710,12 @@ EDL_HOST_API int edl_lora_apply(const void* x, long long ldx, const void* y, lon
 #undef EDL_LORA_F32
 }
 
-// da [n][parts * r][K] (+)= g^T x and db [n][N][r] (+)= dy^T u over each adapter's rows (either may be null). g (for da), u (for db): what
-// edl_lora_apply left of the backward and the forward call. out_f32: type of da and db; accumulate (fp32 only): add to them.
-// Adapters without rows get zeros.
-EDL_HOST_API int edl_lora_grads(const void* x, long long ldx, const void* dy, long long ldy, const void* g, const void* u,
-                                const int* index, void* da, long long da_adapter, long long ld_da, void* db, long long db_adapter,
-                                long long ld_db, int T, int K, int N, int n, int r, int parts, const int* widths, int in_f32,
-                                int out_f32, int accumulate, int* status, void* stream) {
+// da [n][parts * r][K] (+)= g^T x and db [n][N][r] (+)= dy^T u over each adapter's rows (either may be null); the strides of a and b in `shape`
+// are theirs, ldy dy's. g (for da), u (for db): what edl_lora_apply left of the backward and the forward call. out_f32: type of da and
+// db; accumulate (fp32 only): add to them. Adapters without rows get zeros.
+EDL_HOST_API int edl_lora_grads(const edl_lora_shape* shape, const void* x, const void* dy, const void* g, const void* u, const int* index,
+                                void* da, void* db, int out_f32, int accumulate, int* status, void* stream) {
+  const auto [ldx, ldy, ldo, da_adapter, ld_da, db_adapter, ld_db, T, K, N, n, r, parts, in_f32, y_f32, backward, widths] = *shape;
   if (K <= 0 || N <= 0 || n <= 0 || r <= 0 || parts < 1 || parts > LORA_SEGS || r > 512 / parts || n > 65535 || (!index && n != 1 && T > 0)) {
     set_last_error("edl_lora_grads: needs sizes above 0, up to %d parts, parts x rank up to 512, up to 65535 adapters, one without an index", LORA_SEGS);
     return -1;

@@ -12,17 +12,23 @@ each replay. Packed projections (queries / keys / values, gate / up) have one ad
 from __future__ import annotations
 
 import ctypes as C
-import functools
 
 import torch
 
 from . import _lib
 
 vp, i32, i64, f32 = _lib.vp, _lib.i32, _lib.i64, _lib.f32
-_lib.register("edl_lora_apply", i32, [vp, i64, vp, i64, vp, i64, vp, i64, i64, vp, i64, i64, vp, vp, f32, vp, i64, vp, i32, i32,
-                                      i32, i32, i32, i32, vp, i32, i32, i32, vp, vp])
-_lib.register("edl_lora_grads", i32, [vp, i64, vp, i64, vp, vp, vp, vp, i64, i64, vp, i64, i64, i32, i32, i32, i32, i32, i32, vp, i32,
-                                      i32, i32, vp, vp])
+
+
+class _Shape(C.Structure):
+    """``edl_lora_shape`` of ``csrc/lora.cu``."""
+
+    _fields_ = [(k, i64) for k in ("ldx", "ldy", "ldo", "a_adapter", "lda", "b_adapter", "ldb")] + \
+               [(k, i32) for k in ("T", "K", "N", "n", "r", "parts", "x_f32", "y_f32", "backward")] + [("widths", i32 * 8)]
+
+
+_lib.register("edl_lora_apply", i32, [vp, vp, vp, vp, vp, vp, vp, vp, f32, vp, i64, vp, vp, vp])
+_lib.register("edl_lora_grads", i32, [vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, vp, vp])
 
 MAX_RANK = 512       # ranks of all parts together
 MAX_PARTS = 8
@@ -80,30 +86,47 @@ def _check(y, x, a, b, index, scale, parts, out):
     return parts
 
 
-@functools.lru_cache(maxsize=256)
-def _widths(parts: tuple[int, ...]):
-    return (C.c_int * len(parts))(*parts)
+def _inner_columns(r: int, parts: int, backward: bool) -> int:
+    """Ranks of a row of the inner value, each part's (the backward pass: all) rounded up to 16."""
+    return -(-parts * r // 16) * 16 if backward else parts * (-(-r // 16) * 16)
 
 
-def _inner(x: torch.Tensor, r: int, parts: int, result: torch.dtype, backward: bool = False) -> torch.Tensor:
-    """Memory for the scaled inner value ``s x a^T`` (``s dy b`` of the backward pass) of rows ``x`` as bf16 parts ``[parts of a value, T, ranks]``."""
-    cols = -(-parts * r // 16) * 16 if backward else parts * (-(-r // 16) * 16)
-    return x.new_empty((3 if result == torch.float32 else 2, x.shape[0], cols), dtype=torch.bfloat16)
+class _Plan:
+    """What a call's sizes, strides and types decide: checked once, kept for the calls that follow with the same ones."""
+
+    __slots__ = ("parts", "plain", "shape", "ref", "u_parts", "u_cols", "blocks", "T", "back", "grads")
+
+    def __init__(self, x, y, out, a, b, parts, backward=False):
+        n, N, r = b.shape
+        rows = lambda t: 0 if t is None else t.stride(-2) if t.dim() > 1 and t.shape[-2] > 1 else t.shape[-1]  # noqa: E731
+        res = x if out is None else out
+        self.T = T = x.numel() // x.shape[-1]
+        self.parts = parts
+        self.shape = _Shape(rows(x), rows(y), rows(out), a.stride(0), a.stride(1), b.stride(0), b.stride(1), T, a.shape[2], N, n, r, len(parts),
+                            x.dtype == torch.float32, res.dtype == torch.float32, backward, (i32 * 8)(*parts))
+        self.ref = C.addressof(self.shape)
+        self.u_parts, self.u_cols = 3 if res.dtype == torch.float32 else 2, _inner_columns(r, len(parts), backward)
+        self.blocks = -(-T // FEW_ROWS) if T > FEW_ROWS else 0
+        self.back = self.grads = None      # the plans of the backward pass's calls, where all operands are contiguous
+
+    def inner(self, x: torch.Tensor) -> torch.Tensor:
+        """Memory for the scaled inner value (``s x a^T``, or ``s dy b`` of the backward pass) as bf16 parts ``[parts of a value, T, ranks]``."""
+        return x.new_empty((self.u_parts, self.T, self.u_cols), dtype=torch.bfloat16)
 
 
-def _apply(x, y, out, a, b, index, scale, u, parts, backward=False):
-    n, N, r = b.shape
-    T, dev = x.shape[0], x.device
-    if u is None and T > FEW_ROWS:
-        u = _inner(x, r, len(parts), x.dtype if out is None else out.dtype, backward)
-    mixed = None if index is None or T <= FEW_ROWS else index.new_empty(-(-T // FEW_ROWS))      # which blocks of rows have many adapters
-    st = scale if isinstance(scale, torch.Tensor) else None
-    _lib.call_on(dev, "edl_lora_apply", x.data_ptr(), x.stride(0), None if y is None else y.data_ptr(), 0 if y is None else y.stride(0),
-                 None if out is None else out.data_ptr(), 0 if out is None else out.stride(0), a.data_ptr(), a.stride(0), a.stride(1),
-                 b.data_ptr(), b.stride(0), b.stride(1), None if index is None else index.data_ptr(), None if st is None else st.data_ptr(),
-                 0.0 if st is not None else scale, None if u is None else u.data_ptr(), 0 if u is None else u.numel(),
-                 None if mixed is None else mixed.data_ptr(), T, a.shape[2], N, n, r, len(parts), _widths(parts), x.dtype == torch.float32, (x if out is None else out).dtype == torch.float32, backward,
-                 _lib.status_word(dev).data_ptr())
+def _apply(plan: _Plan, x, y, out, a, b, index, scale, u) -> None:
+    u_size, mixed = 0, None
+    if plan.blocks:
+        if u is None:
+            u = plan.inner(x)
+        if index is not None:
+            mixed = index.new_empty(plan.blocks)      # which blocks of rows have many adapters
+    if u is not None:
+        u_size, u = u.numel(), u.data_ptr()
+    tensor = type(scale) is not float
+    _lib.call_on(x.device, "edl_lora_apply", plan.ref, x.data_ptr(), None if y is None else y.data_ptr(), None if out is None else out.data_ptr(),
+                 a.data_ptr(), b.data_ptr(), None if index is None else index.data_ptr(), scale.data_ptr() if tensor else None,
+                 0.0 if tensor else scale, u, u_size, None if mixed is None else mixed.data_ptr(), _lib.status_word(x.device).data_ptr())
 
 
 def _grad_target(w: torch.Tensor) -> tuple[torch.Tensor, bool]:
@@ -114,47 +137,90 @@ def _grad_target(w: torch.Tensor) -> tuple[torch.Tensor, bool]:
     return mg.view(w.shape), True
 
 
+def _matrix(t: torch.Tensor) -> bool:
+    """Rows of neighbouring elements at one distance (leading dimensions, if more than one, lie one after the other)."""
+    return (t.stride(-1) == 1 or t.shape[-1] == 1) if t.dim() == 2 else t.is_contiguous()
+
+
 class _LoraAddFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, y, x, a, b, index, scale, parts):
-        x2 = _rows(x)
+    def forward(ctx, y, x, a, b, index, scale, plan):
         out = torch.empty_like(y, memory_format=torch.contiguous_format)
-        u = _inner(x2, b.shape[2], len(parts), x.dtype) if ctx.needs_input_grad[3] else None
-        _apply(x2, _rows(y), _rows(out), _weights(a), _weights(b), index, scale, u, parts)
-        ctx.save_for_backward(x, a, b, u, index, scale if isinstance(scale, torch.Tensor) else None)
-        ctx.scale, ctx.parts = scale, parts
+        ctx.x_shape, a2, b2 = x.shape, a, b
+        if not plan.plain:
+            y, x, a2, b2 = _rows(y), _rows(x), _weights(a), _weights(b)
+            plan = _Plan(x, y, out, a2, b2, plan.parts)
+        u = plan.inner(x) if ctx.needs_input_grad[3] else None
+        _apply(plan, x, y, out, a2, b2, index, scale, u)
+        ctx.scale, ctx.plan = scale if type(scale) is float else None, plan
+        ctx.save_for_backward(x, a, b, u, index, None if type(scale) is float else scale)
         return out
 
     @staticmethod
     def backward(ctx, dy):
         if torch.is_grad_enabled():
             raise NotImplementedError("adapters have no second derivatives")
-        x, a, b, u, index, st = ctx.saved_tensors
-        scale, parts = st if st is not None else ctx.scale, ctx.parts
-        need_y, need_x, need_a, need_b = ctx.needs_input_grad[:4]
-        dy2, x2 = _rows(dy), _rows(x)
-        n, N, r = b.shape
-        dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
-        g = _inner(x2, r, len(parts), x.dtype, True) if need_a else None
-        if need_x or need_a:
-            _apply(dy2, None, _rows(dx) if need_x else None, _weights(a), _weights(b), index, scale, g, parts, True)
+        x, a, b, u, index, scale = ctx.saved_tensors
+        if scale is None:
+            scale = ctx.scale
+        plan, (need_y, need_x, need_a, need_b) = ctx.plan, ctx.needs_input_grad[:4]
+        dy2 = dy if _matrix(dy) else _rows(dy)
         da, a_added = _grad_target(a) if need_a else (None, False)
         db, b_added = _grad_target(b) if need_b else (None, False)
+        dx = x.new_empty(ctx.x_shape) if need_x else None
+        g = None
+        if need_x or need_a:
+            a2, b2 = _weights(a), _weights(b)
+            usual = need_x and dy2.is_contiguous()
+            back = plan.back if usual else None
+            if back is None:
+                back = _Plan(dy2, None, dx, a2, b2, plan.parts, True)
+                if usual:
+                    plan.back = back
+            g = back.inner(x) if need_a else None
+            _apply(back, dy2, None, dx, a2, b2, index, scale, g)
         # one launch for both, unless only one of them is added to a flat buffer
         for ta, tb, added in ((da, db, a_added or b_added),) if da is None or db is None or a_added == b_added else \
                 ((da, None, a_added), (None, db, b_added)):
             if ta is None and tb is None:
                 continue
-            _lib.call_on(x.device, "edl_lora_grads", x2.data_ptr(), x2.stride(0), dy2.data_ptr(), dy2.stride(0), _lib.ptr(g), _lib.ptr(u),
-                         _lib.ptr(index), _lib.ptr(ta), 0 if ta is None else ta.stride(0), 0 if ta is None else ta.stride(1), _lib.ptr(tb),
-                         0 if tb is None else tb.stride(0), 0 if tb is None else tb.stride(1), x2.shape[0], a.shape[2], N, n, r, len(parts),
-                         _widths(parts), x.dtype == torch.float32, (ta if tb is None else tb).dtype == torch.float32, added,
+            usual = dy2.is_contiguous() and (ta is None or ta.is_contiguous()) and (tb is None or tb.is_contiguous())
+            grads = plan.grads if usual else None
+            if grads is None:
+                grads = _Plan(x, dy2, None, torch.empty_like(a, device="meta", memory_format=torch.contiguous_format) if ta is None else ta,
+                              torch.empty_like(b, device="meta", memory_format=torch.contiguous_format) if tb is None else tb, plan.parts)
+                if usual:
+                    plan.grads = grads
+            _lib.call_on(x.device, "edl_lora_grads", grads.ref, x.data_ptr(), dy2.data_ptr(), _lib.ptr(g), _lib.ptr(u), _lib.ptr(index),
+                         _lib.ptr(ta), _lib.ptr(tb), (ta if tb is None else tb).dtype == torch.float32, added,
                          _lib.status_word(x.device).data_ptr())
         if a_added:
             a.grad_added_to_main_grad = True
         if b_added:
             b.grad_added_to_main_grad = True
         return dy if need_y else None, dx, None if a_added else da, None if b_added else db, None, None, None
+
+
+_plans: dict[tuple, _Plan | None] = {}
+
+
+def _plan_of(y, x, a, b, index, scale, parts, out) -> _Plan:
+    """The plan of an inference call, by its sizes, strides, types and device."""
+    tensor = isinstance(scale, torch.Tensor)
+    key = (x.shape, x.stride(), x.dtype, x.device, y.shape, y.stride(), y.dtype, y.device, a.shape, a.stride(), a.dtype, a.device, b.shape, b.stride(),
+           b.dtype, b.device, parts, index is None or (index.shape, index.dtype, index.device, index.is_contiguous()),
+           (scale.shape, scale.dtype, scale.device, scale.is_contiguous(), scale.requires_grad) if tensor else None,
+           out is None or out is y or (out.shape, out.stride(), out.dtype, out.device))
+    plan = _plans.get(key)
+    if plan is None:
+        parts = _check(y, x, a, b, index, scale, parts, out)
+        plan = _Plan(x, y, torch.empty_like(y, device="meta", memory_format=torch.contiguous_format) if out is None else out, a, b, parts)
+        # operands whose rows have to be copied first, and results that cannot be written as rows, take the long way
+        plan.plain = x.is_cuda and all(map(_matrix, (x, y) if out is None else (x, y, out))) and a.stride(2) == 1 and b.stride(2) == 1
+        if len(_plans) >= 4096:
+            _plans.clear()
+        _plans[key] = plan
+    return plan
 
 
 def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, index: torch.Tensor | None = None,
@@ -169,27 +235,29 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     (``y`` itself for in place; inference only). An index of ``n`` or more counts as none and sets the status word that
     ``_lib.check_status`` reads.
     """
-    parts = _check(y, x, a, b, index, scale, None if parts is None else tuple(parts), out)
-    grad = torch.is_grad_enabled() and (x.requires_grad or a.requires_grad or b.requires_grad or y.requires_grad)
-    if grad and out is not None:
-        raise ValueError("out= is for inference: a gradient needs y as it was")
+    plan = _plan_of(y, x, a, b, index, scale, None if parts is None else tuple(parts), out)
+    if torch.is_grad_enabled() and (x.requires_grad or a.requires_grad or b.requires_grad or y.requires_grad):
+        if out is not None:
+            raise ValueError("out= is for inference: a gradient needs y as it was")
+        if not _lib.use_kernels(x):
+            return lora_add_reference(y, x, a, b, index, scale, parts=plan.parts)
+        if y.dtype != x.dtype:
+            raise NotImplementedError("float32 outputs beside bfloat16 rows have no backward pass")
+        return _LoraAddFn.apply(y, x, a, b, index, scale if isinstance(scale, torch.Tensor) else float(scale), plan)
     if not _lib.use_kernels(x):
-        o = lora_add_reference(y, x, a, b, index, scale, parts=parts)
+        o = lora_add_reference(y, x, a, b, index, scale, parts=plan.parts)
         return o if out is None else out.copy_(o)
     if not isinstance(scale, torch.Tensor):
         scale = float(scale)
-    if grad:
-        if y.dtype != x.dtype:
-            raise NotImplementedError("float32 outputs beside bfloat16 rows have no backward pass")
-        return _LoraAddFn.apply(y, x, a, b, index, scale, parts)
+    if plan.plain:
+        res = torch.empty_like(y, memory_format=torch.contiguous_format) if out is None else out
+        _apply(plan, x, y, res, a, b, index, scale, None)
+        return res
+    if out is not None and not _matrix(out):      # no rows with neighbouring elements to write to
+        return out.copy_(lora_add(y, x, a, b, index, scale, parts=plan.parts))
     res = torch.empty_like(y, memory_format=torch.contiguous_format) if out is None else out
-    if res.dim() == 2 and (res.stride(1) == 1 or res.shape[1] == 1):
-        o2 = res
-    elif res.is_contiguous():
-        o2 = res.view(-1, res.shape[-1])
-    else:      # no rows with neighbouring elements to write to
-        return res.copy_(lora_add(y, x, a, b, index, scale, parts=parts))
-    _apply(_rows(x), o2 if res is y else _rows(y), o2, _weights(a), _weights(b), index, scale, None, parts)
+    x2, y2, a2, b2 = _rows(x), res if res is y else _rows(y), _weights(a), _weights(b)
+    _apply(_Plan(x2, y2, res, a2, b2, plan.parts), x2, y2, res, a2, b2, index, scale, None)
     return res
 
 
