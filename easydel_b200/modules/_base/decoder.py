@@ -647,6 +647,8 @@ class DecoderModel(EasyDeLBaseModule):
                                         self.remat_policy())
         if policy and self.training and torch.is_grad_enabled() and cache_view is None:
             # recompute unit under the configured save policy (full recompute, saved dots, saved names ...)
+            if not x.requires_grad and not getattr(pending, "requires_grad", False) and any(p.requires_grad for p in layer.parameters()):
+                x = x.detach().requires_grad_()      # frozen embeddings: the unit gets its gradient through an input
             return remat.recompute_unit(lambda a, b, c, d: layer(a, b, c, d, None, None), self.remat_policy(),
                                         (x, _resolve(pending), positions, segment_ids),
                                         whole_layer=remat.runs_as_defined(layer, _LAYER_FORWARD))
