@@ -21,6 +21,7 @@ import torch
 
 from ...caching.paged import PAGE_SIZE, PagedKVCache
 from ..sampling_params import SamplingParams
+from ..token_rules import TokenRules
 from .metrics import MetricsCollector
 from .kv_manager import KVCacheCoordinator
 from .page_pool import PagePool
@@ -122,9 +123,13 @@ class eSurge:
                  sharding_axis_dims=(1, 1, 1, -1, 1), extra_eos_token_ids: tp.Sequence[int] | None = None,
                  extra_stops: str | tp.Sequence[str] | None = None, auto_cap_new_tokens: bool = True,
                  sampling_params_callback: tp.Callable | None = None, tool_parser: str | None = None,
-                 reasoning_parser: str | None = None, kv_quantization=None, **compile_options):
+                 reasoning_parser: str | None = None, kv_quantization=None, max_adapters: int = 0, max_adapter_rank: int = 16,
+                 **compile_options):
         """``async_scheduling`` / ``overlap_execution`` (either one; default on for CUDA models): step *t+1* is
         scheduled and launched before the tokens of step *t* are read back, so host work overlaps device work.
+
+        ``max_adapters``: low-rank adapters of rank up to ``max_adapter_rank`` that can be loaded at once (:meth:`load_adapter`) and named
+        by requests; the requests of a step may all name different ones.
 
         ``compile_options`` takes only the reference's ahead-of-time compilation knobs, which have nothing to
         act on here (kernels are launched eagerly or replayed from CUDA graphs); any other name is an error."""
@@ -174,7 +179,14 @@ class eSurge:
                                                    max_model_len=max_model_len,
                                                    long_prefill_token_threshold=long_prefill_token_threshold,
                                                    policy=scheduling_policy), self.kv, page_size)
-        self.runner = ModelRunner(model, self.cache, max_num_seqs, self.max_num_batched_tokens, max_model_len)
+        self.adapters = None
+        if max_adapters:
+            from ...layers.adapters import AdapterSet
+
+            self.adapters = AdapterSet(getattr(model, "language_model", model), max_adapters, max_adapter_rank)
+        self._adapter_loads = itertools.count()
+        self._adapter_keys: dict[str, str] = {}
+        self.runner = ModelRunner(model, self.cache, max_num_seqs, self.max_num_batched_tokens, max_model_len, adapters=self.adapters)
         self.metrics = MetricsCollector()
         self._tracked: dict[str, _Tracked] = {}
         self._free_slots = list(range(max_num_seqs - 1, -1, -1))
@@ -236,6 +248,8 @@ class eSurge:
         self.terminate()
         self.stop_monitoring()
         self.runner.release()
+        if self.adapters is not None:
+            self.adapters.detach()
 
     def pause(self) -> None:
         with self._work:
@@ -297,6 +311,35 @@ class eSurge:
             for m in self.kv.managers:
                 m.pool.reset_cache()
 
+    # ------------------------------------------------------------------ adapters
+    def load_adapter(self, name: str, source, scale: float | None = None) -> None:
+        """Loads an adapter that requests can name from then on (``add_request(adapter=name)``). ``source``: a PEFT directory, or tensors by name
+        (:meth:`..layers.adapters.AdapterSet.load`)."""
+        if self.adapters is None:
+            raise RuntimeError("the engine was built without room for adapters (max_adapters)")
+        with self._lock:
+            self._drain()
+            self.adapters.load(name, source, scale)
+            if self.runner.device.type == "cuda":
+                torch.cuda.synchronize(self.runner.device)      # steps may run on another stream than this thread's
+            self._adapter_keys[name] = f"{name}#{next(self._adapter_loads)}"      # pages of an earlier adapter of this name are not its own
+
+    def unload_adapter(self, name: str) -> None:
+        """Frees the slot of an adapter that no unfinished request names."""
+        with self._lock:
+            key = self._adapter_keys.get(name)
+            if self.adapters is None or key is None:
+                raise KeyError(f"no adapter {name!r}")
+            if any(r.adapter == key for r in self.scheduler.requests.values()):
+                raise RuntimeError(f"adapter {name!r} is in use")
+            self._drain()
+            self.adapters.unload(name)
+            del self._adapter_keys[name]
+
+    @property
+    def adapter_names(self) -> list[str]:
+        return list(self._adapter_keys)
+
     # ------------------------------------------------------------------ requests
     def _tokenize(self, prompt) -> tuple[list[int], str | None]:
         if isinstance(prompt, str):
@@ -318,7 +361,10 @@ class eSurge:
 
     def add_request(self, prompt, sampling_params: SamplingParams | None = None, request_id: str | None = None,
                     priority: int = 0, images: tp.Sequence[tp.Any] | None = None,
-                    videos: tp.Sequence[tp.Any] | None = None) -> str:
+                    videos: tp.Sequence[tp.Any] | None = None, adapter: str | None = None) -> str:
+        """Queues a request. ``adapter``: the name of a loaded adapter to run it with."""
+        if adapter is not None and adapter not in self._adapter_keys:
+            raise ValueError(f"adapter {adapter!r} is not loaded")
         sp = sampling_params or SamplingParams()
         if self.sampling_params_callback is not None:
             sp = self.sampling_params_callback(sp, {"prompt": prompt, "request_id": request_id}) or sp
@@ -356,9 +402,15 @@ class eSurge:
                             mm_hash=mm_hash)
         if rope is not None:
             req.rope_positions, req.rope_delta = rope
+        eos = [] if sp.ignore_eos or self.eos_token_id is None else [self.eos_token_id]
+        req.rules = TokenRules.of(sp, self.runner.vocab, [*eos, *sp.stop_token_ids])
         tr = _Tracked(req, text, IncrementalDetokenizer(self.tokenizer if sp.detokenize else None,
                                                         sp.skip_special_tokens))
         with self._work:
+            if adapter is not None:
+                if adapter not in self._adapter_keys:
+                    raise ValueError(f"adapter {adapter!r} is not loaded")
+                req.adapter, req.adapter_slot = self._adapter_keys[adapter], self.adapters.slots[adapter]
             self._tracked[rid] = tr
             self.scheduler.add_request(req)
             self.metrics.start_request(rid, len(ids))
@@ -405,6 +457,10 @@ class eSurge:
         """schedule(t) -> launch(t) -> read back and commit(t-1) -> book(t): the host work of a step (scheduling,
         batch metadata, detokenisation, stop checks) runs while the device executes the previous launch."""
         with self._lock:
+            early = 0
+            if self._inflight is not None and any(r.sampling_params.needs_history for r in self.scheduler.running):
+                prev, self._inflight = self._inflight, None      # the next mask of a grammar needs the token of the step in flight
+                early = self._commit(*prev)
             out = self.scheduler.schedule()
             for r in out.preempted:
                 self._return_slot(r)
@@ -413,7 +469,7 @@ class eSurge:
                 self._assign_slots(out)
                 handle = self.runner.launch(out)
             prev, self._inflight = self._inflight, None
-            done = self._commit(*prev) if prev is not None else 0
+            done = early + (self._commit(*prev) if prev is not None else 0)
             if handle is not None:
                 self.scheduler.advance_optimistic(out)
                 self._inflight = (out, handle, time.perf_counter())
@@ -527,9 +583,11 @@ class eSurge:
 
     def generate(self, prompts, sampling_params: SamplingParams | list[SamplingParams] | None = None,
                  request_id: str | list[str] | None = None, use_tqdm: bool = False,
-                 images: list | None = None, videos: list | None = None) -> list[RequestOutput]:
+                 images: list | None = None, videos: list | None = None,
+                 adapter: str | list[str | None] | None = None) -> list[RequestOutput]:
         """Blocking batch generation. Works with or without the background thread. ``images`` / ``videos``: the
-        images / frame stacks of the prompt (or one list per prompt), one per placeholder token."""
+        images / frame stacks of the prompt (or one list per prompt), one per placeholder token. ``adapter``: the name of a
+        loaded adapter (or one per prompt, None for none)."""
         single = isinstance(prompts, str) or (isinstance(prompts, (list, tuple)) and prompts
                                               and isinstance(prompts[0], int))
         plist = [prompts] if single else list(prompts)
@@ -540,8 +598,11 @@ class eSurge:
         else:
             imgs = [images] if single else list(images)
         vids = [None] * len(plist) if videos is None else ([videos] if single else list(videos))
-        ids = [self.add_request(p, sp, rid, images=im, videos=vd)
-               for p, sp, rid, im, vd in zip(plist, sps, rids, imgs, vids)]
+        ads = list(adapter) if isinstance(adapter, (list, tuple)) else [adapter] * len(plist)
+        if len(ads) != len(plist):
+            raise ValueError(f"{len(ads)} adapters for {len(plist)} prompts")
+        ids = [self.add_request(p, sp, rid, images=im, videos=vd, adapter=ad)
+               for p, sp, rid, im, vd, ad in zip(plist, sps, rids, imgs, vids, ads)]
         self._drive(lambda: all(self._tracked[i].finished for i in ids))
         outs = [self._snapshot(self._tracked.pop(i), True) for i in ids]
         return outs
@@ -555,9 +616,9 @@ class eSurge:
                 break
 
     def stream(self, prompt, sampling_params: SamplingParams | None = None, request_id: str | None = None,
-               images: list | None = None, videos: list | None = None) -> tp.Iterator[RequestOutput]:
+               images: list | None = None, videos: list | None = None, adapter: str | None = None) -> tp.Iterator[RequestOutput]:
         """Yields a ``RequestOutput`` whenever new tokens arrive (``delta_text`` holds the increment)."""
-        rid = self.add_request(prompt, sampling_params, request_id, images=images, videos=videos)
+        rid = self.add_request(prompt, sampling_params, request_id, images=images, videos=videos, adapter=adapter)
         tr = self._tracked[rid]
         background = self._thread is not None and self._thread.is_alive()
         try:
@@ -578,7 +639,7 @@ class eSurge:
             self._tracked.pop(rid, None)
 
     def chat(self, messages: list[dict], sampling_params: SamplingParams | None = None, tools: list | None = None,
-             stream: bool = False, chat_template: str | None = None, **template_kwargs):
+             stream: bool = False, chat_template: str | None = None, adapter: str | None = None, **template_kwargs):
         if self.tokenizer is None:
             raise ValueError("chat() needs a tokenizer with a chat template")
         images = None
@@ -590,8 +651,8 @@ class eSurge:
                                                     add_generation_prompt=True, chat_template=chat_template,
                                                     **template_kwargs)
         if stream:
-            return self.stream(prompt, sampling_params, images=images or None)
-        return self.generate(prompt, sampling_params, images=images or None)[0]
+            return self.stream(prompt, sampling_params, images=images or None, adapter=adapter)
+        return self.generate(prompt, sampling_params, images=images or None, adapter=adapter)[0]
 
     def get_metrics_summary(self) -> dict:
         m = self.metrics.summary()

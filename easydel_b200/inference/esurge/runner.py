@@ -19,12 +19,13 @@ import torch
 from ...caching.paged import PAGE_SIZE, PagedBatchMeta, PagedKVCache
 from ...ops import functional as F
 from ...ops import serving as S
+from ..token_rules import collect
 from .scheduler import SchedulerOutput
 
 
 class ModelRunner:
     def __init__(self, model, cache: PagedKVCache, max_num_seqs: int, max_num_batched_tokens: int,
-                 max_model_len: int):
+                 max_model_len: int, adapters=None):
         self.model = model
         # a vision-language wrapper is served through its language model; image rows arrive as embeddings
         self._lm = getattr(model, "language_model", model)
@@ -52,6 +53,12 @@ class ModelRunner:
         self._rope_idx = len(self._sizes) if self.rope3 else -1
         if self.rope3:
             self._sizes.append(3 * T)
+        # requests with adapters: the adapter slot of every token row
+        self.adapters = adapters
+        self._adapter_idx = len(self._sizes) if adapters is not None else -1
+        if adapters is not None:
+            self._sizes.append(T)
+        self._with_adapters = False        # the staged step has a row with an adapter
         total = sum(self._sizes)
         self._host = torch.zeros(total, dtype=torch.int32, pin_memory=pin)
         self._dev = torch.zeros(total, dtype=torch.int32, device=dev)
@@ -95,11 +102,13 @@ class ModelRunner:
             self.use_graphs = False     # these serving paths are tensor code with host-side steps: run eagerly
         self._seq_slots = torch.zeros(max_num_seqs, dtype=torch.int64, device=dev)
         self._graphs: dict[int, tuple[tp.Any, torch.Tensor]] = {}
+        self._adapter_graphs: dict[int, tuple[tp.Any, torch.Tensor]] = {}      # of steps with adapters
         # device time of replayed decode steps (CUDA events around the graph launch), read by decode_step_times()
         self.time_decode_steps = False
         self._step_events: list = []
         self._graph_pool = None
         self._warm: set[int] = set()
+        self._adapter_warm: set[int] = set()
         self._sms = torch.cuda.get_device_properties(dev).multi_processor_count if dev.type == "cuda" else 1
         self.tp_group = None
         mesh = getattr(model.config, "mesh", None)
@@ -121,6 +130,8 @@ class ModelRunner:
         """Drops the captured graphs (and with them their private memory pool). Needed before the process group
         is torn down: a graph that holds collectives keeps the communicator's resources alive."""
         self._graphs.clear()
+        self._adapter_graphs.clear()
+        self._adapter_warm.clear()
         self._graph_pool = None
         self._warm.clear()
         if self.device.type == "cuda":
@@ -159,6 +170,12 @@ class ModelRunner:
 
     def _forward(self, B: int, T: int, max_q: int, num_decode: int, mm_rows=None,
                  logit_rows: torch.Tensor | None = None) -> torch.Tensor:
+        if not self._with_adapters:
+            return self._run_backbone(B, T, max_q, num_decode, mm_rows, logit_rows)
+        with self.adapters.rows(self._dviews[self._adapter_idx][:T]):
+            return self._run_backbone(B, T, max_q, num_decode, mm_rows, logit_rows)
+
+    def _run_backbone(self, B: int, T: int, max_q: int, num_decode: int, mm_rows, logit_rows: torch.Tensor | None) -> torch.Tensor:
         """Backbone over the first ``T`` staged tokens of ``B`` sequences, LM head on each sequence's last row (or on the
         staged rows ``logit_rows``). ``mm_rows``: ``[(first staged row, features [n, hidden])]`` to write over the token
         embeddings."""
@@ -219,12 +236,13 @@ class ModelRunner:
 
     def _decode_graph(self, Bp: int) -> tuple[torch.Tensor, torch.Tensor]:
         """``(tokens, logits)`` of the greedy decode step for ``Bp`` rows, see :meth:`_decode_step_graphed`."""
-        entry = self._graphs.get(Bp)
+        graphs, warm = (self._adapter_graphs, self._adapter_warm) if self._with_adapters else (self._graphs, self._warm)
+        entry = graphs.get(Bp)
         if entry is not None:
             entry[0].replay()
             return entry[1], entry[2]
-        if Bp not in self._warm:
-            self._warm.add(Bp)
+        if Bp not in warm:
+            warm.add(Bp)
             logits = self._forward(Bp, Bp, 1, Bp)
             return S.sample(logits)[0], logits
         torch.cuda.synchronize(self.device)
@@ -234,7 +252,7 @@ class ModelRunner:
             toks = S.sample(logits)[0]
         if self._graph_pool is None:
             self._graph_pool = g.pool()
-        self._graphs[Bp] = (g, toks, logits)
+        graphs[Bp] = (g, toks, logits)
         g.replay()
         return toks, logits
 
@@ -321,7 +339,10 @@ class ModelRunner:
         cu_np[0] = 0
         any_pen = False
         any_random = False
+        any_rules = False
         mm_rows = []
+        self._with_adapters = self.adapters is not None and any(s.request.adapter_slot >= 0 for s in sched)
+        adapter_np = self._hviews[self._adapter_idx].numpy() if self._with_adapters else None
         fast = all(s.num_new_tokens == 1 and s.start >= s.request.num_prompt_tokens for s in sched)
         if fast:
             # Decode-only step: vectorised fill from the per-slot page mirror (one short Python pass per field).
@@ -337,6 +358,9 @@ class ModelRunner:
                 sp = req.sampling_params
                 any_pen |= sp.needs_penalties
                 any_random |= not sp.is_greedy
+                any_rules |= req.rules is not None and req.rules.active(len(req.output_token_ids))
+            if adapter_np is not None:
+                adapter_np[:B] = np.fromiter((s.request.adapter_slot for s in sched), dtype=np.int32, count=B)
             p = np.fromiter((s.start for s in sched), dtype=np.int32, count=B)
             ids_np[:B] = np.fromiter((s.request.output_token_ids[-1] for s in sched), dtype=np.int32, count=B)
             pos_np[:B] = p
@@ -403,13 +427,16 @@ class ModelRunner:
             cu_np[b + 1] = o
             last_np[b] = o - 1
             max_q = max(max_q, n)
+            if adapter_np is not None:
+                adapter_np[o - n:o] = req.adapter_slot
             sp = req.sampling_params
             any_pen |= sp.needs_penalties
             any_random |= not sp.is_greedy
+            any_rules |= req.rules is not None and req.rules.active(len(req.output_token_ids))
         self._spans = spans if max_q > 1 else None
         if self.num_groups > 1:
             self._fill_extra_groups(sched, B)
-        decode_only = max_q == 1 and not any_pen and not any_random
+        decode_only = max_q == 1 and not any_pen and not any_random and not any_rules
         Bp = B
         if self.use_graphs and decode_only:
             Bp = 1
@@ -427,6 +454,8 @@ class ModelRunner:
                 cu_np[B + 1:Bp + 1] = np.arange(B + 1, Bp + 1, dtype=np.int32)
                 last_np[B:Bp] = np.arange(B, Bp, dtype=np.int32)
                 slotof_np[B:Bp] = self.max_num_seqs
+                if adapter_np is not None:
+                    adapter_np[B:Bp] = -1
                 for g in range(self.num_groups - 1):
                     self._hviews[10 + 2 * g].numpy()[B:Bp] = 0
                     self._hviews[11 + 2 * g].numpy().reshape(self.max_num_seqs, MP)[B:Bp, :] = 0
@@ -439,11 +468,12 @@ class ModelRunner:
         if nfix:
             d_fixpos, d_fixslot = self._dviews[8][:nfix].long(), self._dviews[9][:nfix].long()
             self._dviews[0].index_copy_(0, d_fixpos, self._last_tokens.index_select(0, d_fixslot).to(torch.int32))
+        self._with_rules = any_rules
         return sched, B, Bp, T, max_q, decode_only, mm_rows, any_pen, any_random
 
     def _run_model(self, out, sched, B, Bp, T, max_q, decode_only, any_pen, any_random, mm_rows):
         if self.use_graphs and decode_only:
-            if self.time_decode_steps and Bp in self._graphs:
+            if self.time_decode_steps and Bp in (self._adapter_graphs if self._with_adapters else self._graphs):
                 e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
                 e0.record()
                 tokens = self._decode_step_graphed(Bp)[:B]
@@ -457,6 +487,7 @@ class ModelRunner:
             logits = self._forward(B, T, max_q, out.num_decode, mm_rows)
             t2 = time.perf_counter()
             kw = {}
+            rules = collect([s.request.rules for s in sched], [s.request for s in sched], self.device) if self._with_rules else {}
             if any_random or any_pen:
                 fh, ih = self._fhost.view(6, -1), self._ihost.view(3, -1)
                 for b, s in enumerate(sched):
@@ -472,11 +503,16 @@ class ModelRunner:
                 fd, idv = self._fdev.view(6, -1), self._idev.view(3, -1)
                 kw = dict(temperature=fd[0, :B], top_p=fd[1, :B], min_p=fd[2, :B], top_k=idv[0, :B].to(torch.int32),
                           seeds=idv[1, :B], steps=idv[2, :B].to(torch.int32))
-                if any_pen:
+                if any_pen and rules:      # one pass over the logits for penalties and rules
+                    rules.update(counts=self._ensure_counts(), presence=fd[3, :B], frequency=fd[4, :B], repetition=fd[5, :B],
+                                 count_rows=torch.tensor([s.request.slot for s in sched], dtype=torch.int32, device=self.device))
+                elif any_pen:
                     counts = self._ensure_counts()
                     slot_rows = torch.tensor([s.request.slot for s in sched], dtype=torch.int64, device=self.device)
                     kw.update(presence=fd[3, :B], frequency=fd[4, :B], repetition=fd[5, :B],
                               counts=counts.index_select(0, slot_rows))
+            if rules:
+                logits = S.adjust_logits(logits, **rules)
             tokens, _ = S.sample(logits, **kw)
             if any_pen:
                 S.count_update(self.counts, tokens, torch.tensor([s.request.slot for s in sched], dtype=torch.int32,

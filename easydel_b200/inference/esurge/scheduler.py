@@ -74,9 +74,18 @@ class EngineRequest:
     # coordinates) and the offset a generated token's rotary position has from its index; None = index everywhere
     rope_positions: tp.Any = None
     rope_delta: int = 0
+    # adapter of the request: its slot in the engine's adapter set (-1: none) and its name; the latter joins the page hashes, as images do
+    adapter_slot: int = -1
+    adapter: tp.Any = None
+    rules: tp.Any = None                  # inference.token_rules.TokenRules, or None
     # asynchronous scheduling: the request reached its length limit with a token that is still on the device;
     # it is not scheduled again and finishes when that token is committed
     finishing: bool = False
+
+    @property
+    def page_key(self) -> tp.Any:
+        """What tells pages of equal tokens apart: images and the adapter."""
+        return self.mm_hash if self.adapter is None else (self.mm_hash, "adapter", self.adapter)
 
     @property
     def all_token_ids(self) -> list[int]:
@@ -197,7 +206,7 @@ class Scheduler:
     def _admit_with_prefix(self, req: EngineRequest) -> None:
         """Shares the cached full pages that match the request's token prefix."""
         tokens = req.all_token_ids
-        req.page_hashes = hash_request_pages(tokens, self.page_size, req.mm_hash)
+        req.page_hashes = hash_request_pages(tokens, self.page_size, req.page_key)
         # never serve the whole request from cache: the last token must be recomputed to produce logits
         usable = req.page_hashes[: max(0, (len(tokens) - 1) // self.page_size)]
         n_hit = self.kv.admit_with_prefix(req, usable)
@@ -217,7 +226,7 @@ class Scheduler:
             return
         tokens = req.all_token_ids
         if len(req.page_hashes) < full:
-            req.page_hashes = hash_request_pages(tokens[: full * self.page_size], self.page_size, req.mm_hash)
+            req.page_hashes = hash_request_pages(tokens[: full * self.page_size], self.page_size, req.page_key)
         for i in range(req.num_registered_pages, full):
             self.kv.register(req, i, req.page_hashes[i])
         req.num_registered_pages = full

@@ -13,6 +13,7 @@ blocking iterators through a thread so that slow clients never stall the schedul
 from __future__ import annotations
 
 import asyncio
+import functools
 import json
 import time
 import typing as tp
@@ -68,12 +69,20 @@ class eSurgeApiServer:
 
     # ------------------------------------------------------------------ helpers
     def _engine(self, model: str | None):
+        """``(name, engine)`` that serves ``model``: an engine's name, or the name of an adapter that one of them has loaded."""
         if model in self.engines:
             return model, self.engines[model]
+        for e in self.engines.values():
+            if model is not None and model in getattr(e, "adapter_names", ()):
+                return model, e
         if model is None or len(self.engines) == 1:
             name = next(iter(self.engines))
             return name, self.engines[name]
         raise KeyError(model)
+
+    def _adapter(self, name: str) -> dict:
+        """Arguments of a request for the adapter that it names as its model."""
+        return {} if name in self.engines else {"adapter": name}
 
     def _parser(self, engine, want_tools: bool) -> DelegatingParser:
         mtype = getattr(getattr(engine, "model", None), "config", None)
@@ -154,17 +163,24 @@ class eSurgeApiServer:
                         lines.append(f'esurge_{k}{{model="{name}"}} {v}')
             return PlainTextResponse("\n".join(lines) + "\n")
 
+        @app.exception_handler(ValueError)
+        async def refused(request: Request, e: ValueError):      # what the engine does not take: a token outside the vocabulary, a prompt too long
+            return JSONResponse(status_code=400, content={"error": {"message": str(e), "type": "invalid_request_error"}})
+
         @app.get("/v1/models")
         async def models(request: Request):
             authorize(request, "/v1/models")
-            return ModelList(data=[ModelCard(id=n, max_model_len=e.max_model_len) for n, e in server.engines.items()])
+            return ModelList(data=[ModelCard(id=n, max_model_len=e.max_model_len) for k, e in server.engines.items()
+                                   for n in (k, *getattr(e, "adapter_names", ()))])
 
         @app.get("/v1/models/{model_id}")
         async def model(model_id: str, request: Request):
             authorize(request, "/v1/models")
-            if model_id not in server.engines:
+            engine = server.engines.get(model_id) or next((e for e in server.engines.values()
+                                                           if model_id in getattr(e, "adapter_names", ())), None)
+            if engine is None:
                 raise HTTPException(status_code=404, detail=f"model {model_id!r} not found")
-            return ModelCard(id=model_id, max_model_len=server.engines[model_id].max_model_len)
+            return ModelCard(id=model_id, max_model_len=engine.max_model_len)
 
         @app.post("/v1/chat/completions")
         async def chat(req: ChatCompletionRequest, request: Request):
@@ -178,7 +194,7 @@ class eSurgeApiServer:
             parser = server._parser(engine, bool(req.tools))
             if not req.stream:
                 loop = asyncio.get_running_loop()
-                out = (await loop.run_in_executor(None, engine.generate, prompt, sp))[0]
+                out = (await loop.run_in_executor(None, functools.partial(engine.generate, prompt, sp, **server._adapter(name))))[0]
                 parsed = parser.parse(out.get_text())
                 calls = [ToolCall(**c) for c in parsed["tool_calls"]] or None
                 server.auth.record_usage(rec, len(out.prompt_token_ids), out.num_generated_tokens)
@@ -194,7 +210,7 @@ class eSurgeApiServer:
                 rid = first.id
                 yield sse(first)
                 last, text, any_tools = None, "", False
-                async for out in pump(request, engine, engine.stream(prompt, sp)):
+                async for out in pump(request, engine, engine.stream(prompt, sp, **server._adapter(name))):
                     last = out
                     text += out.delta_text
                     d = parser.parse_streaming(text, final=out.finished)
@@ -229,7 +245,7 @@ class eSurgeApiServer:
                 prompts = [prompts]
             if not req.stream:
                 loop = asyncio.get_running_loop()
-                outs = await loop.run_in_executor(None, engine.generate, list(prompts), sp)
+                outs = await loop.run_in_executor(None, functools.partial(engine.generate, list(prompts), sp, **server._adapter(name)))
                 choices, usage = [], UsageInfo()
                 for i, o in enumerate(outs):
                     text = ((o.prompt or "") if req.echo else "") + o.get_text()
@@ -243,7 +259,7 @@ class eSurgeApiServer:
             async def gen():
                 last = None
                 cid = None
-                async for out in pump(request, engine, engine.stream(prompts[0], sp)):
+                async for out in pump(request, engine, engine.stream(prompts[0], sp, **server._adapter(name))):
                     last = out
                     chunk = CompletionResponse(model=name, choices=[CompletionResponseChoice(
                         text=out.delta_text, finish_reason=_finish_reason(out, False) if out.finished else None)],
@@ -292,7 +308,7 @@ class eSurgeApiServer:
                     for ev, payload in builder.start():
                         yield sse_frame(ev, payload)
                     last, text = None, ""
-                    async for out in pump(request, engine, engine.stream(prompt, sp)):
+                    async for out in pump(request, engine, engine.stream(prompt, sp, **server._adapter(name))):
                         last = out
                         text += out.delta_text
                         d = parser.parse_streaming(text, final=out.finished)
@@ -312,7 +328,7 @@ class eSurgeApiServer:
 
                 return StreamingResponse(gen(), media_type="text/event-stream")
             loop = asyncio.get_running_loop()
-            out = (await loop.run_in_executor(None, engine.generate, prompt, sp))[0]
+            out = (await loop.run_in_executor(None, functools.partial(engine.generate, prompt, sp, **server._adapter(name))))[0]
             parsed = server._parser(engine, bool(req.tools)).parse(out.get_text())
             server.auth.record_usage(rec, len(out.prompt_token_ids), out.num_generated_tokens)
             items: list[dict] = []

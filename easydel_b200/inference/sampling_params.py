@@ -65,6 +65,11 @@ class SamplingParams:
         self.stop_token_ids = list(self.stop_token_ids or [])
 
     @property
+    def needs_history(self) -> bool:
+        """Whether the tokens allowed next depend on the ones sampled so far (a grammar as a callable)."""
+        return callable(self.guided_decoding)
+
+    @property
     def is_greedy(self) -> bool:
         return self.temperature == 0.0 or self.top_k == 1
 

@@ -26,7 +26,8 @@ import typing as tp
 import torch
 from torch import nn
 
-from ..ops import functional as F
+from ..ops import _lib, functional as F
+from ..ops.adapters import MAX_RANK, lora_add
 
 
 class ParallelLinear(nn.Module):
@@ -35,6 +36,8 @@ class ParallelLinear(nn.Module):
     sp_state = None
     # activation-checkpoint name of this product (``ops.remat``): set by the block that owns the layer
     remat_name: str | None = None
+    # adapters of the requests that a serving engine runs (``layers.adapters.AdapterBank``)
+    adapters = None
 
     def __init__(self, in_features: int, out_features: int | tp.Sequence[int], bias: bool = False, *,
                  dtype: torch.dtype = torch.float32, init_std: float | None = 0.02, tp_size: int = 1,
@@ -92,7 +95,7 @@ class ParallelLinear(nn.Module):
         y = F.linear(x, self.weight if w is None else w, self.bias, name=self.remat_name)
         if self.scale is not None:
             y = y * self.scale
-        return y
+        return y if self.adapters is None else self.adapters.add(y, x)
 
     def extra_repr(self) -> str:
         return (f"in={self.in_features}, out={self.out_features}, bias={self.bias is not None}, "
@@ -167,8 +170,10 @@ class eLoRA(nn.Module):
 
     def forward(self, x: torch.Tensor, w: torch.Tensor | None = None) -> torch.Tensor:
         y = self.base(x, w)
-        z = torch.nn.functional.linear(torch.nn.functional.linear(self.dropout(x), self.lora_a), self.lora_b)
-        return y + z * self.scaling
+        if not _lib.use_kernels(x) or not x.dtype == y.dtype == self.lora_a.dtype or self.rank > MAX_RANK:
+            z = torch.nn.functional.linear(torch.nn.functional.linear(self.dropout(x), self.lora_a), self.lora_b)
+            return y + z * self.scaling
+        return lora_add(y, self.dropout(x), self.lora_a[None], self.lora_b[None], None, self.scaling)
 
     @torch.no_grad()
     def merge(self) -> ParallelLinear:

@@ -225,6 +225,8 @@ def quantized_matmul(x: torch.Tensor, q: QuantizedTensor, bias: torch.Tensor | N
 class QuantizedLinear(nn.Module):
     """Drop-in for the parallel linears after quantisation (inference only; weights are buffers)."""
 
+    adapters = None      # as on the parallel linears
+
     def __init__(self, q: QuantizedTensor, bias: torch.Tensor | None = None, source: nn.Module | None = None):
         super().__init__()
         self.fmt, self.bits, self.group = q.fmt, q.bits, q.group
@@ -256,7 +258,8 @@ class QuantizedLinear(nn.Module):
             y = quantized_matmul(x, self.tensor(), None)
             y = tp.all_reduce(y, tp_group)
             return y if self.bias is None else y + self.bias
-        return quantized_matmul(x, self.tensor(), self.bias)
+        y = quantized_matmul(x, self.tensor(), self.bias)
+        return y if self.adapters is None else self.adapters.add(y, x)
 
     def extra_repr(self) -> str:
         return f"in={self.in_features}, out={self.out_features}, fmt={self.fmt}, bits={self.bits}, group={self.group}"

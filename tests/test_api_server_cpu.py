@@ -203,3 +203,22 @@ def test_reasoning_streaming_matches_offline():
         c_all += dc
     off = ReasoningParserManager.get_reasoning_parser("qwen3")(None).extract_reasoning(text)
     assert r_all.strip("\n") == off[0] and c_all.strip("\n") == off[1]
+
+
+def test_adapters_are_models_of_the_server():
+    cfg = LlamaConfig(vocab_size=V, hidden_size=32, intermediate_size=64, num_hidden_layers=1, num_attention_heads=4, num_key_value_heads=2,
+                      max_position_embeddings=512, eos_token_id=2, initializer_range=0.3)
+    torch.manual_seed(0)
+    model = LlamaForCausalLM(cfg, dtype=torch.float32, param_dtype=torch.float32).eval()
+    eng = eSurge(model, tokenizer=Tok(), max_model_len=256, max_num_seqs=4, esurge_name="tiny", max_adapters=1, max_adapter_rank=8)
+    g = torch.Generator().manual_seed(1)
+    eng.load_adapter("mine", {"model.layers.0.mlp.down_proj.lora_a": torch.randn(8, 64, generator=g),
+                              "model.layers.0.mlp.down_proj.lora_b": torch.randn(32, 8, generator=g)})
+    client = TestClient(eSurgeApiServer(eng).app, raise_server_exceptions=False)
+    assert [m["id"] for m in client.get("/v1/models").json()["data"]] == ["tiny", "mine"]
+    assert client.get("/v1/models/mine").status_code == 200
+    ask = lambda **kw: client.post("/v1/completions", json={"prompt": "hello", "max_tokens": 6, "temperature": 0, "ignore_eos": True, **kw})  # noqa: E731
+    plain, mine = ask(model="tiny").json(), ask(model="mine").json()
+    assert mine["model"] == "mine" and mine["choices"][0]["text"] != plain["choices"][0]["text"]
+    assert ask(model="tiny", logit_bias={"40": 100000}).json()["choices"][0]["text"] == Tok().decode([40] * 6)
+    assert ask(model="tiny", logit_bias={"4000": 1}).status_code == 400
