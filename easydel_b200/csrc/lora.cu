@@ -436,8 +436,12 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const __grid_cons
             for (int j = 0; j < NT; ++j)
 #pragma unroll
               for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
-#pragma unroll(P == 1 && RT <= 2 ? 2 : 1)
-          for (int k = seg.c0 + 32 * (c * LORA_WARPS + w); k < seg.c1; k += 32 * C * LORA_WARPS) {
+          // a warp takes whole lines of 128 bytes: 64 columns (32 of fp32)
+          constexpr int HALVES = P == 1 ? 2 : 1;
+          for (int k2 = seg.c0 + 32 * HALVES * (c * LORA_WARPS + w); k2 < seg.c1; k2 += 32 * HALVES * C * LORA_WARPS)
+#pragma unroll(RT <= 2 ? HALVES : 1)
+          for (int half = 0; half < HALVES; ++half) {
+            const int k = k2 + 32 * half;
             uint32_t wa[RT][2][P][4];      // [rank tile][k16][part][register]
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
@@ -1527,7 +1531,11 @@ struct edl_lora_shape {
 EDL_HOST_API int edl_lora_apply(const edl_lora_shape* shape, const void* x, const void* y, void* out, const void* a, const void* b,
                                 const int* index, const float* scale, float scale_all, void* u, long long u_size, int* mixed,
                                 int* status, void* stream) {
-  const auto [ldx, ldy, ldo, a_adapter, lda, b_adapter, ldb, T, K, N, n, r, parts, x_f32, y_f32, backward, widths] = *shape;
+  const long long ldx = shape->ldx, ldy = shape->ldy, ldo = shape->ldo, a_adapter = shape->a_adapter, lda = shape->lda, b_adapter = shape->b_adapter,
+                  ldb = shape->ldb;
+  const int T = shape->T, K = shape->K, N = shape->N, n = shape->n, r = shape->r, parts = shape->parts, x_f32 = shape->x_f32, y_f32 = shape->y_f32,
+            backward = shape->backward;
+  const int* widths = shape->widths;
   if (T <= 0) return 0;
   if (K <= 0 || N <= 0 || n <= 0 || r <= 0 || parts < 1 || parts > LORA_SEGS || r > 512 / parts) {
     set_last_error("edl_lora_apply: needs sizes above 0, up to %d parts and parts x rank up to 512", LORA_SEGS);
@@ -1715,7 +1723,9 @@ EDL_HOST_API int edl_lora_apply(const edl_lora_shape* shape, const void* x, cons
 // db; accumulate (fp32 only): add to them. Adapters without rows get zeros.
 EDL_HOST_API int edl_lora_grads(const edl_lora_shape* shape, const void* x, const void* dy, const void* g, const void* u, const int* index,
                                 void* da, void* db, int out_f32, int accumulate, int* status, void* stream) {
-  const auto [ldx, ldy, ldo, da_adapter, ld_da, db_adapter, ld_db, T, K, N, n, r, parts, in_f32, y_f32, backward, widths] = *shape;
+  const long long ldx = shape->ldx, ldy = shape->ldy, da_adapter = shape->a_adapter, ld_da = shape->lda, db_adapter = shape->b_adapter, ld_db = shape->ldb;
+  const int T = shape->T, K = shape->K, N = shape->N, n = shape->n, r = shape->r, parts = shape->parts, in_f32 = shape->x_f32;
+  const int* widths = shape->widths;
   if (K <= 0 || N <= 0 || n <= 0 || r <= 0 || parts < 1 || parts > LORA_SEGS || r > 512 / parts || n > 65535 || (!index && n != 1 && T > 0)) {
     set_last_error("edl_lora_grads: needs sizes above 0, up to %d parts, parts x rank up to 512, up to 65535 adapters, one without an index", LORA_SEGS);
     return -1;

@@ -473,6 +473,8 @@ def adjust_logits(logits: torch.Tensor, *, counts: torch.Tensor | None = None, c
     if not logits.is_cuda:
         z = adjust_logits_reference(logits, counts, count_rows, presence, frequency, repetition, bias, mask)
         return z if out is None else out.copy_(z)
+    if counts is None and bias is None and mask is None:      # nothing to apply
+        return logits.to(torch.float32, copy=True) if out is None else out if out is logits else out.copy_(logits)
     if V > 1 and logits.stride(1) != 1:
         if out is logits:
             return out.copy_(adjust_logits(logits.contiguous(), counts=counts, count_rows=count_rows, presence=presence,
