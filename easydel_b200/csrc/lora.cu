@@ -236,16 +236,19 @@ __host__ __device__ constexpr int round16(int v) { return (v + 15) & ~15; }
 __host__ __device__ constexpr int u_stride(int cols) { return cols % 32 ? cols : cols + 16; }      // 8-byte reads without conflicts
 
 // Rows of a block in the order of their adapters, cut into units of at most `chunk` rows of one adapter.
-constexpr int UNIT_SLOTS = 2 * LORA_ROWS;
 struct RowUnits {
   int idx0, total;
   bool mixed;                                                   // rows of more than MIXED adapters
-  int key[UNIT_SLOTS];                                          // adapters by a hash of their number
-  __align__(8) uint8_t count[UNIT_SLOTS][LORA_ROWS / 32];       // rows of a slot's adapter in each warp
-  short place[UNIT_SLOTS];                                      // of its first row in `order`
   short order[LORA_ROWS], base[LORA_ROWS], rows[LORA_ROWS];     // row of a place; first place and rows of a unit
   int ad[LORA_ROWS];
   int scan[LORA_MAX_WARPS];
+};
+// What finding them takes: lies where the kernels have their stages later, two of which then fit an SM.
+constexpr int UNIT_SLOTS = 2 * LORA_ROWS;
+struct UnitTable {
+  int key[UNIT_SLOTS];                              // adapters by a hash of their number
+  uint8_t count[UNIT_SLOTS][LORA_ROWS / 32];        // rows of a slot's adapter in each warp
+  short place[UNIT_SLOTS];                          // of its first row in `order`
 };
 
 // Among many rows, a block of LORA_ROWS rows of more adapters than this (the single tokens of a step) goes to the one-launch kernel, whose
@@ -277,7 +280,8 @@ __device__ __forceinline__ int cta_scan(int v, int* scan, int& total) {
 // training batch belong to one request: those take no look-up. Else rows of one adapter find each other within their warp (`match`) and
 // across warps through a slot of a hash table, whose place decides nothing: units are numbered by their first rows.
 // 256 rows of 64 adapters: 1.4 us; 4.9 us when every row compared itself with all others.
-__device__ __forceinline__ void find_units(RowUnits& u, const LoraArgs& a, long long row0, int rows, int chunk) {
+__device__ __forceinline__ void find_units(RowUnits& u, void* scratch, const LoraArgs& a, long long row0, int rows, int chunk) {
+  UnitTable& t = *reinterpret_cast<UnitTable*>(scratch);
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   int id = -2;
   if (tid < rows) {
@@ -290,8 +294,8 @@ __device__ __forceinline__ void find_units(RowUnits& u, const LoraArgs& a, long 
     u.order[tid] = (short)tid;
 #pragma unroll
     for (int i = 0; i < UNIT_SLOTS / LORA_ROWS; ++i) {
-      u.key[tid + i * LORA_ROWS] = -3;
-      *reinterpret_cast<uint2*>(u.count[tid + i * LORA_ROWS]) = make_uint2(0, 0);
+      t.key[tid + i * LORA_ROWS] = -3;
+      *reinterpret_cast<uint2*>(t.count[tid + i * LORA_ROWS]) = make_uint2(0, 0);
     }
   }
   __syncthreads();
@@ -316,8 +320,8 @@ __device__ __forceinline__ void find_units(RowUnits& u, const LoraArgs& a, long 
     lower = __popc(same & ((1u << lane) - 1));
     if (lane == leader && id >= -1) {
       slot = (uint32_t)(id * 0x9e3779b1u) >> 23;      // the top 9 bits: UNIT_SLOTS
-      for (int found; (found = atomicCAS(&u.key[slot], -3, id)) != -3 && found != id;) slot = (slot + 1) & (UNIT_SLOTS - 1);
-      u.count[slot][w] = (uint8_t)__popc(same);
+      for (int found; (found = atomicCAS(&t.key[slot], -3, id)) != -3 && found != id;) slot = (slot + 1) & (UNIT_SLOTS - 1);
+      t.count[slot][w] = (uint8_t)__popc(same);
     }
     slot = __shfl_sync(0xffffffffu, slot, leader);
   }
@@ -325,7 +329,7 @@ __device__ __forceinline__ void find_units(RowUnits& u, const LoraArgs& a, long 
   int before = lower, count = 0;
 #pragma unroll
   for (int i = 0; i < LORA_ROWS / 32; ++i) {
-    const int v = u.count[slot][i];
+    const int v = t.count[slot][i];
     count += v;
     before += i < w ? v : 0;
   }
@@ -336,7 +340,7 @@ __device__ __forceinline__ void find_units(RowUnits& u, const LoraArgs& a, long 
   const int at = cta_scan((first ? count | nu << 10 : 0) | (any ? 1 << 20 : 0), u.scan, all);
   const int place = at & 1023, unit = at >> 10 & 1023;
   if (first) {
-    u.place[slot] = (short)place;
+    t.place[slot] = (short)place;
     for (int q = 0; q < nu; ++q) {
       u.base[unit + q] = (short)(place + q * chunk);
       u.rows[unit + q] = (short)min(chunk, count - q * chunk);
@@ -348,8 +352,8 @@ __device__ __forceinline__ void find_units(RowUnits& u, const LoraArgs& a, long 
     u.mixed = (all >> 20) > MIXED;
   }
   __syncthreads();
-  if (taken) u.order[u.place[slot] + before] = (short)tid;
-  __syncthreads();
+  if (taken) u.order[t.place[slot] + before] = (short)tid;
+  __syncthreads();      // the table makes way
 }
 
 // --------------------------------------------------------------------------------------------------- one launch, few rows
@@ -394,7 +398,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const __grid_cons
   for (int block = a.mixed ? 0 : cid / a.groups, step = a.mixed ? 1 : nblocks; block < nblocks; block += step) {
   if (a.mixed && !a.mixed[block]) continue;
   const long long row0 = (long long)block * LORA_ROWS;
-  find_units(units, a, row0, (int)min((long long)LORA_ROWS, a.T - row0), CHUNK);
+  find_units(units, dyn, a, row0, (int)min((long long)LORA_ROWS, a.T - row0), CHUNK);
   for (int unit = cid % a.groups; unit < units.total; unit += a.groups) {
     const int ad = units.ad[unit], m = units.rows[unit];
     const short* order = units.order + units.base[unit];
@@ -745,7 +749,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_down_kernel(const __grid
   const long long row0 = (long long)(cid / a.groups) * LORA_ROWS;
   const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x);
   Ring ring = ring_start(shared, dyn, down_stage(np, DOWN_T), DOWN_COLS, a.status);
-  find_units(units, a, row0, (int)min((long long)LORA_ROWS, a.T - row0), DOWN_ROWS);
+  find_units(units, dyn, a, row0, (int)min((long long)LORA_ROWS, a.T - row0), DOWN_ROWS);
   if (a.mixed && tid == 0) a.mixed[row0 / LORA_ROWS] = units.mixed;
   const uint32_t idesc = umma_idesc_bf16(128, np, 0, DOWN_T);
   // passes: `each` of a part's ranks in all parts; `at_once` of them fit tensor memory
@@ -905,7 +909,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_up_any_kernel(const __gr
   const LoraSeg seg = a.up_seg[p];
   const int n0 = seg.c0 + tile * UP_COLS + 32 * w, col = n0 + 8 * t4, r16 = round16(seg.ru), ustride = u_stride(r16);
   const bool ok = col < seg.c1;
-  find_units(units, a, row0, (int)min((long long)LORA_ROWS, a.T - row0), 16);
+  find_units(units, dyn, a, row0, (int)min((long long)LORA_ROWS, a.T - row0), 16);
   const int share = (units.total + a.splits - 1) / a.splits, unit0 = min(units.total, (int)(blockIdx.x / a.groups % a.splits) * share);
   const int total = min(units.total, unit0 + share);
   if (units.mixed || unit0 >= total) return;
@@ -1055,7 +1059,9 @@ __global__ void __launch_bounds__(UP_THREADS, 2) lora_up_kernel(const __grid_con
     tmem_relinquish();
   }
   tc_fence_before();
-  find_units(units, a, row0, (int)min((long long)LORA_ROWS, a.T - row0), UP_ROWS);
+  find_units(units, dyn, a, row0, (int)min((long long)LORA_ROWS, a.T - row0), UP_ROWS);
+  fence_proxy_async_smem();      // the table makes way for copies
+  __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
   const int r16 = round16(a.up_seg[0].ru), share = (a.groups + a.splits - 1) / a.splits;      // column tiles: all, of a CTA
@@ -1508,6 +1514,35 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_grad_kernel(const __grid
   ring_end(ring, tmem_cols);
 }
 
+// Clusters of `size` CTAs of the gradient kernel that the current device runs at once (asked for once per size).
+int grad_clusters(int size, int smem) {
+  static int known[64][9] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) dev = 0;
+  if (!known[dev][size]) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(size);
+    cfg.blockDim = dim3(LORA_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = size;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    if (shared_memory(reinterpret_cast<const void*>(lora_grad_kernel), smem, "lora gradient shared memory") ||
+        cudaOccupancyMaxActiveClusters(&clusters, lora_grad_kernel, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      clusters = 2 * sm_count() / size * 7 / 8;
+    }
+    known[dev][size] = clusters > 0 ? clusters : -1;
+  }
+  return known[dev][size];
+}
+
 bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
 
 }  // namespace
@@ -1664,7 +1699,7 @@ EDL_HOST_API int edl_lora_apply(const edl_lora_shape* shape, const void* x, cons
       } else {
         // a block that is not mixed has at most 16 + MIXED units: they are shared out where there are few CTAs, or where u takes much memory
         const int row_bytes = s * u_stride(r16) * 2, units = LORA_ROWS / 16 + MIXED;
-        auto own = [&](int splits) { return ((units + splits - 1) / splits) * 16 * row_bytes; };
+        auto own = [&](int splits) { return max((int)sizeof(UnitTable), ((units + splits - 1) / splits) * 16 * row_bytes); };
         g.splits = 1;
         while (g.splits < 8 && (own(g.splits) > 56 * 1024 || (g.splits < 4 && (long long)g.groups * blocks * g.splits < 4LL * sms))) g.splits *= 2;
         const long long ctas = (long long)g.groups * blocks * g.splits;
@@ -1692,6 +1727,7 @@ EDL_HOST_API int edl_lora_apply(const edl_lora_shape* shape, const void* x, cons
   const long long grid_blocks = g.mixed ? 1 : blocks;
   while (cluster > 2 && grid_blocks * g.groups * cluster > 4LL * sms) cluster /= 2;
   const int red = LORA_WARPS * 16 * (16 * rt + 4) * 4, su = s * 16 * u_stride(g.ucols) * 2;
+  static_assert(LORA_WARPS * 16 * 20 * 4 >= sizeof(UnitTable) && UP_SMEM >= sizeof(UnitTable), "the table of units lies in the kernels' stages");
   const int smem = ((16 * g.rtot * 4 + 15) & ~15) + (red > su ? red : su);
   const dim3 grid((unsigned)(grid_blocks * g.groups * cluster));
 #define EDL_LORA(TX, TO, RTV, BW, W) return launch_cluster(lora_kernel<TX, TO, RTV, BW, W>, grid, cluster, smem, st, "lora launch", g)
@@ -1768,14 +1804,16 @@ EDL_HOST_API int edl_lora_grads(const edl_lora_shape* shape, const void* x, cons
     job.tiles = ((job.c1 - job.c0 + GRAD_COLS - 1) / GRAD_COLS) * ((job.ru + rp - 1) / rp);
     tiles += job.tiles;
   }
-  // Rows are cut over the CTAs of a cluster. Clusters have to fit the GPU's parts, which leaves about 7 of 8 places (two per SM); a
-  // turn of CTAs takes its steps of 32 rows and about as long as 6 more to start and to add up.
+  // Rows are cut over the CTAs of a cluster, of the size that takes the least: a turn of all clusters that run at once takes its steps of 32 rows
+  // and about as long as 6 more to start and to add up.
+  const int ring_bytes = fast ? RING_STAGES * GRAD_STAGE + 1024 : 16 * GRAD_STRIDE * 4;
   int cluster = 1;
-  const long long places = 2LL * sm_count() * 7 / 8;
   long long best = 0;
-  for (int c = 1; c <= 8; c *= 2) {
-    const long long cost = (((long long)tiles * n * c + places - 1) / places) * (6 + (a.T + 32LL * c - 1) / (32LL * c));
-    if (c == 1 || cost < best) {
+  for (int c = 1; c <= 8; ++c) {
+    const int at_once = fast ? grad_clusters(c, ring_bytes) : 2 * sm_count() / c;
+    if (at_once < 1) continue;
+    const long long cost = (((long long)tiles * n + at_once - 1) / at_once) * (6 + (a.T + 32LL * c - 1) / (32LL * c));
+    if (!best || cost < best) {
       best = cost;
       cluster = c;
     }
@@ -1791,9 +1829,9 @@ EDL_HOST_API int edl_lora_grads(const edl_lora_shape* shape, const void* x, cons
     if (a.T && db && (make_tmap_2d_16b(&maps.z[1], dy, a.T, N, ldy, GRAD_ROWS, 64) ||
                       make_tmap_3d_16b(&maps.p[1], u, parts * round16(r), a.T, 2, parts * round16(r), (uint64_t)a.T * parts * round16(r), 64, GRAD_ROWS, 1, 3)))
       return -1;
-    return launch_cluster(lora_grad_kernel, grid, cluster, RING_STAGES * GRAD_STAGE + 1024, st, what, a, maps, rp);
+    return launch_cluster(lora_grad_kernel, grid, cluster, ring_bytes, st, what, a, maps, rp);
   }
-  const int smem = 16 * GRAD_STRIDE * 4;
+  const int smem = ring_bytes;
   if (in_f32) return wide ? launch_cluster(lora_grad_any_kernel<float, 3, true>, grid, cluster, smem, st, what, a)
                           : launch_cluster(lora_grad_any_kernel<float, 3, false>, grid, cluster, smem, st, what, a);
   return launch_cluster(lora_grad_any_kernel<__nv_bfloat16, 2, false>, grid, cluster, smem, st, what, a);
