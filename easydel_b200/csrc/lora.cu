@@ -1019,16 +1019,16 @@ __device__ __forceinline__ void store_64(void* p, const uint32_t (&v)[16], bool 
 
 // The same on tcgen05: 128 rows of one adapter are the M side, 64 columns at a time the N side, the ranks of both parts of u the inner index.
 // A lane loads tiles of y and of the weights ahead (TMA), a lane of the second warp issues the products into one of two accumulators, and
-// eight warps, a row per lane and half a tile's columns each, add them to y and write out. What bounds it is the traffic of y and out. Rows
-// of y that lanes asked for themselves, two tiles ahead, took a third longer than by TMA; rows of out that went through shared memory
-// to leave as whole lines took a fifth longer than 64 bytes from each lane.
+// two times four warps, a row per lane, add every other tile to y where it lies and send it out as boxes of 32 rows (TMA). What bounds it is
+// the traffic of y and out. Rows of y that lanes asked for themselves, two tiles ahead, took a third longer than by TMA.
 constexpr int UP_THREADS = 320, UP_ROWS = 128, UP_TILE = 64, UP_STAGES = 3;
 constexpr int UP_Y = UP_ROWS * UP_TILE * 2, UP_W = 64 * 128, UP_STAGE = UP_Y + UP_W, UP_U = UP_ROWS * 128;
 constexpr int UP_SMEM = UP_STAGES * UP_STAGE + 2 * UP_U + 1024;
 
 template <bool UP_T>
 __global__ void __launch_bounds__(UP_THREADS, 2) lora_up_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ CUtensorMap map_y,
-                                                               const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_u) {
+                                                               const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_u,
+                                                               const __grid_constant__ CUtensorMap map_out) {
   __shared__ RowUnits units;
   __shared__ uint64_t s_bars[2 * UP_STAGES + 6];
   __shared__ uint32_t s_tmem;
@@ -1043,11 +1043,11 @@ __global__ void __launch_bounds__(UP_THREADS, 2) lora_up_kernel(const __grid_con
   if (tid == 0) {
     for (int i = 0; i < UP_STAGES; ++i) {
       mbar_init(full + 8 * i, 1);
-      mbar_init(empty + 8 * i, 9);      // the products and eight warps
+      mbar_init(empty + 8 * i, 5);      // the products and four warps
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(dfull + 8 * i, 1);
-      mbar_init(dempty + 8 * i, 8);
+      mbar_init(dempty + 8 * i, 4);
     }
     mbar_init(ufull, 1);
     mbar_init(ufree, 1);
@@ -1145,7 +1145,7 @@ __global__ void __launch_bounds__(UP_THREADS, 2) lora_up_kernel(const __grid_con
     });
     __syncwarp();
   } else {
-    const int q = w & 3, h = (w - 2) >> 2, i = 32 * q + lane;      // this lane's row of a unit; which 32 columns of a tile
+    const int q = w & 3, half = (w - 2) >> 2, i = 32 * q + lane;      // this lane's row of a unit; its four warps take every other tile
     const bool wide = a.ldo % 16 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
     walk([&](const Run& r) {
       if (r.ad >= 0 && !line(r)) {      // u of rows that are no neighbours
@@ -1160,58 +1160,72 @@ __global__ void __launch_bounds__(UP_THREADS, 2) lora_up_kernel(const __grid_con
         asm volatile("bar.sync 1, 256;" ::: "memory");
         if (tid == 64) mbar_arrive(ufull);
       }
+      const bool neighbours = line(r), boxed = a.y && r.ad >= 0 && neighbours;
       const long long row = row0 + (i < r.m ? r.order[i] : 0);
-      const int col0 = r.n0 + 32 * h, left = a.up_seg[r.p].c1 - col0;      // columns of this lane, tile after tile
-      const __nv_bfloat16* y = reinterpret_cast<const __nv_bfloat16*>(a.y) + row * a.ldy + col0;
-      __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + row * a.ldo + col0;
-      const bool boxed = a.y && r.ad >= 0 && line(r), wide_r = wide && col0 % 16 == 0;
-      for (int t = 0; t < r.count; ++t) {
-        const int tile = r.tile + t, at = tile % UP_STAGES, buf = tile & 1, have = left - t * UP_TILE;
-        uint32_t v[16];      // y, then out
-        if (boxed) {
+      const __nv_bfloat16* y = reinterpret_cast<const __nv_bfloat16*>(a.y) + row * a.ldy;
+      __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + row * a.ldo;
+      for (int t = (r.tile ^ half) & 1; t < r.count; t += 2) {
+        const int tile = r.tile + t, at = tile % UP_STAGES, n0 = r.n0 + t * UP_TILE, left = a.up_seg[r.p].c1 - n0;
+        uint8_t* box = dyn + at * UP_STAGE + i * 128;
+        // 32 whole rows of a whole tile leave as one box from where y lay; others from registers
+        const bool whole = r.ad >= 0 && neighbours && 32 * q + 32 <= r.m && left >= UP_TILE;
+        if (r.ad >= 0) {
           wait(full + 8 * at, tile / UP_STAGES, EDL_TIMEOUT_EPILOGUE);
-          const uint8_t* box = dyn + at * UP_STAGE + i * 128;
+          wait(dfull + 8 * half, tile / 2, EDL_TIMEOUT_EPILOGUE);
+          tc_fence_after();
+        }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint4 x = *reinterpret_cast<const uint4*>(box + 16 * ((4 * h + e) ^ (i & 7)));
-            v[4 * e] = x.x; v[4 * e + 1] = x.y; v[4 * e + 2] = x.z; v[4 * e + 3] = x.w;
-          }
-        } else {
+        for (int h = 0; h < 2; ++h) {
+          const int have = left - 32 * h;
+          uint32_t v[16];      // y, then out
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             uint4 x = make_uint4(0, 0, 0, 0);
-            if (a.y && i < r.m && have > 8 * e) x = *reinterpret_cast<const uint4*>(y + t * UP_TILE + 8 * e);
+            if (boxed) x = *reinterpret_cast<const uint4*>(box + 16 * ((4 * h + e) ^ (i & 7)));
+            else if (a.y && i < r.m && have > 8 * e) x = *reinterpret_cast<const uint4*>(y + n0 + 32 * h + 8 * e);
             v[4 * e] = x.x; v[4 * e + 1] = x.y; v[4 * e + 2] = x.z; v[4 * e + 3] = x.w;
+          }
+          if (r.ad >= 0) {
+            uint32_t d[32];
+            tmem_ld_32x32b_x32(tmem + (uint32_t(32 * q) << 16) + half * UP_TILE + 32 * h, d);
+            tc_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              v[e] = pack_bf16x2(__uint_as_float(v[e] << 16) + __uint_as_float(d[2 * e]), __uint_as_float(v[e] & 0xffff0000u) + __uint_as_float(d[2 * e + 1]));
+          }
+          if (whole) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              *reinterpret_cast<uint4*>(box + 16 * ((4 * h + e) ^ (i & 7))) = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+          } else if (i < r.m) {
+            if (have >= 32) {
+              store_64(out + n0 + 32 * h, v, wide && (n0 & 15) == 0);
+            } else {      // the last columns of a part
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (have > 8 * e) *reinterpret_cast<uint4*>(out + n0 + 32 * h + 8 * e) = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+            }
           }
         }
         if (r.ad >= 0) {
-          uint32_t d[32];
-          wait(dfull + 8 * buf, tile / 2, EDL_TIMEOUT_EPILOGUE);
-          tc_fence_after();
-          tmem_ld_32x32b_x32(tmem + (uint32_t(32 * q) << 16) + buf * UP_TILE + 32 * h, d);
-          tc_wait_ld();
           tc_fence_before();
+          if (whole) fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            mbar_arrive(dempty + 8 * buf);
+            mbar_arrive(dempty + 8 * half);
+            if (whole) {
+              tma_store_2d(&map_out, smem_u32(dyn + at * UP_STAGE + 32 * q * 128), n0, (int)row0 + r.order[0] + 32 * q);
+              tma_store_commit();
+              tma_store_wait_read<0>();
+            }
             mbar_arrive(empty + 8 * at);
           }
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            v[e] = pack_bf16x2(__uint_as_float(v[e] << 16) + __uint_as_float(d[2 * e]), __uint_as_float(v[e] & 0xffff0000u) + __uint_as_float(d[2 * e + 1]));
-        }
-        if (i < r.m) {
-          if (have >= 32) {
-            store_64(out + t * UP_TILE, v, wide_r);
-          } else {      // the last columns of a part
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (have > 8 * e) *reinterpret_cast<uint4*>(out + t * UP_TILE + 8 * e) = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
-          }
+          __syncwarp();
         }
       }
     });
   }
+  tma_store_wait<0>();
   tc_fence_before();
   __syncthreads();
   if (w == 1) tmem_dealloc(tmem, 2 * UP_TILE);
@@ -1686,15 +1700,16 @@ EDL_HOST_API int edl_lora_apply(const edl_lora_shape* shape, const void* x, cons
         g.splits = ctas < g.groups / 4 ? ctas : g.groups / 4;
         if (g.splits < 1) g.splits = 1;
         g.splits = (g.groups + (g.groups + g.splits - 1) / g.splits - 1) / ((g.groups + g.splits - 1) / g.splits);
-        CUtensorMap map_y{}, map_u{};
+        CUtensorMap map_y{}, map_u{}, map_out{};
+        if (make_tmap_2d_16b(&map_out, out, T, backward ? K : N, ldo, 32, UP_TILE)) return -1;
         if (y && make_tmap_2d_16b(&map_y, y, T, backward ? K : N, ldy, UP_ROWS, UP_TILE)) return -1;
         if (make_tmap_3d_16b(&map_u, u, g.ucols, T, 2, g.ucols, (uint64_t)T * g.ucols, 64, UP_ROWS, 1, 3)) return -1;
         if (backward ? make_tmap_3d_16b(&map_w, a, K, parts * r, n, lda, a_adapter, UP_TILE, r16, 1, 3)
                      : make_tmap_3d_16b(&map_w, b, r, N, n, ldb, b_adapter, 64, UP_TILE, 1, 3))
           return -1;
         const dim3 up((unsigned)((long long)blocks * g.splits));
-        if (backward ? launch_sized(lora_up_kernel<true>, up, UP_THREADS, 1, UP_SMEM, st, "lora up launch", g, map_y, map_w, map_u)
-                     : launch_sized(lora_up_kernel<false>, up, UP_THREADS, 1, UP_SMEM, st, "lora up launch", g, map_y, map_w, map_u))
+        if (backward ? launch_sized(lora_up_kernel<true>, up, UP_THREADS, 1, UP_SMEM, st, "lora up launch", g, map_y, map_w, map_u, map_out)
+                     : launch_sized(lora_up_kernel<false>, up, UP_THREADS, 1, UP_SMEM, st, "lora up launch", g, map_y, map_w, map_u, map_out))
           return -1;
       } else {
         // a block that is not mixed has at most 16 + MIXED units: they are shared out where there are few CTAs, or where u takes much memory
