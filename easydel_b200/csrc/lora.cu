@@ -178,6 +178,22 @@ __device__ __forceinline__ float cluster_sum(uint32_t addr, int C) {
   return sum;
 }
 
+__device__ __forceinline__ void cluster_sum4(uint32_t addr, int C, float (&sum)[4]) {      // four neighbours
+  float v[8][4];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[k][i] = 0.f;
+    if (k < C)
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[k][0]), "=f"(v[k][1]), "=f"(v[k][2]), "=f"(v[k][3])
+                   : "r"(mapa_shared(addr, k)) : "memory");
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] += v[k][i];
+}
+
 // ---------------------------------------------------------------------------------------------------------- which rows
 struct LoraSeg {
   int c0, c1;       // columns of the matrix this side works on
@@ -859,28 +875,35 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_down_kernel(const __grid
       tc_fence_after();
       // ---- each CTA adds up and writes its share
       const int r16 = round16(a.up_seg[0].ru), lo = pass_of(pass0).lo, hi = pass_of(pass1 - 1).hi;
-      for (int e = c * LORA_THREADS + tid; e < m * a.ucols; e += C * LORA_THREADS) {
-        const int tok = e / a.ucols, col = e - tok * a.ucols;
+      // (four ranks at a time: r is a multiple of 4 here, so they belong to one part and one pass)
+      const int quads = a.ucols / 4;
+      for (int e = c * LORA_THREADS + tid; e < m * quads; e += C * LORA_THREADS) {
+        const int tok = e / quads, col = 4 * (e - tok * quads);
         const int p = a.up_segs > 1 ? col / r16 : 0, j = col - p * r16, rank = a.up_seg[p].u0 + j;
         const bool pad = j >= a.up_seg[p].ru;
         if (pad ? pass0 > 0 : rank < lo || rank >= hi) continue;
-        float v = 0.f;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
         if (!pad) {
-          const int of = rank / a.down_seg[0].ru, in = rank - of * a.down_seg[0].ru;      // part and rank in it
-          v = s * cluster_sum(smem_u32(part + tok * pstride + (of * each + in / np - pass0) * np + in % np), C);
+          const int of = a.down_segs > 1 ? rank / a.down_seg[0].ru : 0, in = rank - of * a.down_seg[0].ru;      // part and rank in it
+          cluster_sum4(smem_u32(part + tok * pstride + (of * each - pass0) * np + in), C, v);
         }
         unsigned short* dst = a.u + (row0 + order[tok]) * a.ucols + col;
-        if (parts == 2) {
-          uint32_t q[2];
-          split<2>(v, q);
-          dst[0] = (unsigned short)q[0];
-          dst[(long long)a.T * a.ucols] = (unsigned short)q[1];
-        } else {
-          uint32_t q[3];
-          split<3>(v, q);
+        uint32_t q[4][3];
 #pragma unroll
-          for (int k = 0; k < 3; ++k) dst[(long long)k * a.T * a.ucols] = (unsigned short)q[k];
+        for (int i = 0; i < 4; ++i) {
+          v[i] = pad ? 0.f : v[i] * s;
+          if (parts == 2) {
+            uint32_t two[2];
+            split<2>(v[i], two);
+            q[i][0] = two[0];
+            q[i][1] = two[1];
+          } else {
+            split<3>(v[i], q[i]);
+          }
         }
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+          if (k < parts) *reinterpret_cast<uint2*>(dst + (long long)k * a.T * a.ucols) = make_uint2(q[0][k] | q[1][k] << 16, q[2][k] | q[3][k] << 16);
       }
       asm volatile("barrier.cluster.arrive.release;" ::: "memory");
       pending = true;
@@ -1662,7 +1685,9 @@ EDL_HOST_API int edl_lora_apply(const edl_lora_shape* shape, const void* x, cons
       return -1;
     }
     g.mixed = may_mix ? mixed : nullptr;
+    // a block has two units, one more for each end of a request within it; a third cluster takes most of those
     g.groups = groups_of(DOWN_ROWS);
+    if (g.groups > 3) g.groups = 3;
     int ru = 0, cols = 0;
     for (int i = 0; i < g.down_segs; ++i) {
       ru = g.down_seg[i].ru > ru ? g.down_seg[i].ru : ru;
@@ -1671,7 +1696,7 @@ EDL_HOST_API int edl_lora_apply(const edl_lora_shape* shape, const void* x, cons
     const int np = ru < DOWN_RANKS ? round16(ru) : DOWN_RANKS;
     // as many CTAs as run at once (two per SM), each with at least four steps of columns
     int cluster = 1;
-    while (cluster < 8 && (long long)((T + DOWN_ROWS - 1) / DOWN_ROWS) * cluster * 2 <= 2 * sms && cols >= 2 * cluster * 4 * DOWN_K) cluster *= 2;
+    while (cluster < 8 && (long long)blocks * g.groups * cluster * 2 <= 2 * sms && cols >= 2 * cluster * 4 * DOWN_K) cluster *= 2;
     const dim3 grid((unsigned)((long long)blocks * g.groups * cluster));
     const int ring = RING_STAGES * down_stage(np, backward), part = DOWN_ROWS * (DOWN_COLS + 4) * 4, down_smem = (ring > part ? ring : part) + 1024;
     // TMA takes weights whose rows start on 16 bytes; a box of the backward pass must not reach into the next part's columns
