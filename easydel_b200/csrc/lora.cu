@@ -414,7 +414,8 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const __grid_cons
   for (int block = a.mixed ? 0 : cid / a.groups, step = a.mixed ? 1 : nblocks; block < nblocks; block += step) {
   if (a.mixed && !a.mixed[block]) continue;
   const long long row0 = (long long)block * LORA_ROWS;
-  find_units(units, dyn, a, row0, (int)min((long long)LORA_ROWS, a.T - row0), CHUNK);
+  // (not where `part` lies: other CTAs may still read that of the last unit)
+  find_units(units, second, a, row0, (int)min((long long)LORA_ROWS, a.T - row0), CHUNK);
   for (int unit = cid % a.groups; unit < units.total; unit += a.groups) {
     const int ad = units.ad[unit], m = units.rows[unit];
     const short* order = units.order + units.base[unit];
@@ -1748,11 +1749,11 @@ EDL_HOST_API int edl_lora_apply(const edl_lora_shape* shape, const void* x, cons
           return -1;
         }
         const int kc = r16 / 16;
-#define EDL_LORA_UP(TO, BW)                                                                                                          \
-  (kc == 1   ? launch_cluster(lora_up_any_kernel<TO, 1, BW>, dim3((unsigned)ctas), 1, own(g.splits), st, "lora up launch", g)        \
-   : kc == 2 ? launch_cluster(lora_up_any_kernel<TO, 2, BW>, dim3((unsigned)ctas), 1, own(g.splits), st, "lora up launch", g)        \
-             : launch_cluster(lora_up_any_kernel<TO, 4, BW>, dim3((unsigned)ctas), 1, own(g.splits), st, "lora up launch", g))
-        if (backward ? EDL_LORA_UP(__nv_bfloat16, true) : y_f32 ? EDL_LORA_UP(float, false) : EDL_LORA_UP(__nv_bfloat16, false)) return -1;
+#define EDL_LORA_UP_OF(TO, KC, BW) launch_cluster(lora_up_any_kernel<TO, KC, BW>, dim3((unsigned)ctas), 1, own(g.splits), st, "lora up launch", g)
+#define EDL_LORA_UP(TO) (kc == 1 ? EDL_LORA_UP_OF(TO, 1, false) : kc == 2 ? EDL_LORA_UP_OF(TO, 2, false) : EDL_LORA_UP_OF(TO, 4, false))
+        // (the backward pass comes here with more than 64 ranks alone)
+        if (backward ? EDL_LORA_UP_OF(__nv_bfloat16, 4, true) : y_f32 ? EDL_LORA_UP(float) : EDL_LORA_UP(__nv_bfloat16)) return -1;
+#undef EDL_LORA_UP_OF
 #undef EDL_LORA_UP
       }
     }

@@ -32,18 +32,30 @@ _lib.register("edl_lora_grads", i32, [vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, 
 
 MAX_RANK = 512       # ranks of all parts together
 MAX_PARTS = 8
+MAX_TRAINED = 65535  # adapters of a call with gradients
 FEW_ROWS = 256       # up to here the inner value stays in shared memory
+
+
+def _matrix(t: torch.Tensor) -> bool:
+    """Rows of neighbouring elements at one distance, apart from each other (leading dimensions, if more than one, lie one after the other)."""
+    return (t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1) if t.dim() == 2 else t.is_contiguous()
+
+
+def _stack(t: torch.Tensor) -> bool:
+    """Matrices ``[n, rows, width]`` of such rows, apart from each other (a stack that is one matrix repeated is none)."""
+    return (t.stride(2) == 1 or t.shape[2] == 1) and (t.stride(1) >= t.shape[2] or t.shape[1] == 1) and \
+        (t.stride(0) >= t.stride(1) * (t.shape[1] - 1) + t.shape[2] or t.shape[0] == 1)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` as rows ``[T, width]`` with neighbouring elements side by side: a view where it has such a layout."""
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
-    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+    return t if _matrix(t) else t.contiguous()
 
 
 def _weights(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
+    return t if _stack(t) else t.contiguous()
 
 
 def _check(y, x, a, b, index, scale, parts, out):
@@ -98,11 +110,13 @@ class _Plan:
 
     def __init__(self, x, y, out, a, b, parts, backward=False):
         n, N, r = b.shape
+        # (strides along dimensions of one element mean nothing)
         rows = lambda t: 0 if t is None else t.stride(-2) if t.dim() > 1 and t.shape[-2] > 1 else t.shape[-1]  # noqa: E731
+        each = lambda t: t.stride(0) if t.shape[0] > 1 else rows(t) * t.shape[1]  # noqa: E731
         res = x if out is None else out
         self.T = T = x.numel() // x.shape[-1]
         self.parts = parts
-        self.shape = _Shape(rows(x), rows(y), rows(out), a.stride(0), a.stride(1), b.stride(0), b.stride(1), T, a.shape[2], N, n, r, len(parts),
+        self.shape = _Shape(rows(x), rows(y), rows(out), each(a), rows(a), each(b), rows(b), T, a.shape[2], N, n, r, len(parts),
                             x.dtype == torch.float32, res.dtype == torch.float32, backward, (i32 * 8)(*parts))
         self.ref = C.addressof(self.shape)
         self.u_parts, self.u_cols = 3 if res.dtype == torch.float32 else 2, _inner_columns(r, len(parts), backward)
@@ -135,11 +149,6 @@ def _grad_target(w: torch.Tensor) -> tuple[torch.Tensor, bool]:
     if mg is None:
         return torch.empty_like(w, memory_format=torch.contiguous_format), False
     return mg.view(w.shape), True
-
-
-def _matrix(t: torch.Tensor) -> bool:
-    """Rows of neighbouring elements at one distance (leading dimensions, if more than one, lie one after the other)."""
-    return (t.stride(-1) == 1 or t.shape[-1] == 1) if t.dim() == 2 else t.is_contiguous()
 
 
 class _LoraAddFn(torch.autograd.Function):
@@ -216,7 +225,7 @@ def _plan_of(y, x, a, b, index, scale, parts, out) -> _Plan:
         parts = _check(y, x, a, b, index, scale, parts, out)
         plan = _Plan(x, y, torch.empty_like(y, device="meta", memory_format=torch.contiguous_format) if out is None else out, a, b, parts)
         # operands whose rows have to be copied first, and results that cannot be written as rows, take the long way
-        plan.plain = x.is_cuda and all(map(_matrix, (x, y) if out is None else (x, y, out))) and a.stride(2) == 1 and b.stride(2) == 1
+        plan.plain = x.is_cuda and all(map(_matrix, (x, y) if out is None else (x, y, out))) and _stack(a) and _stack(b)
         if len(_plans) >= 4096:
             _plans.clear()
         _plans[key] = plan
@@ -232,7 +241,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     rows); ``a [n, P * r, K]``, ``b [n, N, r]``: the adapters' weights, of x's type; ``index``: int32, an adapter per row, negative
     for none (None: one adapter for all rows); ``scale``: a number, or float32 ``[n]``; ``parts``: widths of the P parts of a
     packed output, whose ranks follow one another in ``a``. Adapters of a smaller rank are padded with zeros. ``out``: where to write
-    (``y`` itself for in place; inference only). An index of ``n`` or more counts as none and sets the status word that
+    (``y`` itself for in place, else apart from all inputs; inference only; its rows do not overlap). An index of ``n`` or more counts as none and sets the status word that
     ``_lib.check_status`` reads.
     """
     plan = _plan_of(y, x, a, b, index, scale, None if parts is None else tuple(parts), out)
@@ -243,6 +252,8 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
             return lora_add_reference(y, x, a, b, index, scale, parts=plan.parts)
         if y.dtype != x.dtype:
             raise NotImplementedError("float32 outputs beside bfloat16 rows have no backward pass")
+        if b.shape[0] > MAX_TRAINED:
+            raise ValueError(f"{b.shape[0]} adapters; gradients take at most {MAX_TRAINED}")
         return _LoraAddFn.apply(y, x, a, b, index, scale if isinstance(scale, torch.Tensor) else float(scale), plan)
     if not _lib.use_kernels(x):
         o = lora_add_reference(y, x, a, b, index, scale, parts=plan.parts)

@@ -2,7 +2,7 @@
 
 import pytest
 import torch
-from adapter_cases import check, exact, make
+from adapter_cases import bound, check, exact, make
 
 pytestmark = pytest.mark.gpu
 BF, F32 = torch.bfloat16, torch.float32
@@ -255,4 +255,83 @@ def test_refuses_gradients_of_float32_outputs_beside_bf16_rows():
     c["y"] = c["y"].float()
     c["x"].requires_grad_()
     with pytest.raises(NotImplementedError):
+        _call(c)
+
+
+@pytest.mark.parametrize("T", [40, 600])
+def test_broadcast_inputs_and_gradients(T):
+    from easydel_b200.ops import adapters
+
+    # one row for all, one first matrix for all adapters, and a gradient that is one row repeated
+    c = make(T, 64, (32, 16), 8, 3, BF, "cuda")
+    c["x"], c["a"], c["dy"] = c["x"][:1].expand(T, 64), c["a"][:1].expand(3, -1, -1), c["dy"][:1].expand(T, -1)
+    val, mag = exact(c, grads=True)
+    check(_call(c), val["out"], mag["out"], 64)
+    x, a, b = (c[k].detach().requires_grad_() for k in ("x", "a", "b"))
+    shared = a[:1].detach().clone().requires_grad_()
+    out = adapters.lora_add(c["y"], x, shared.expand(3, -1, -1), b, c["index"], c["scale"], parts=c["parts"])
+    (out * c["dy"][0]).sum(0).backward(torch.ones(48, device="cuda", dtype=BF))
+    check(x.grad, val["dx"], mag["dx"], 48, "dx")
+    check(b.grad, val["db"], mag["db"], T + 64, "db")
+    # the adapters' gradients are rounded, then their sum is
+    want, size = val["da"].sum(0, keepdim=True), mag["da"].sum(0, keepdim=True)
+    assert ((shared.grad.double().cpu() - want).abs() <= bound(BF, want, size, T + 48) + 2.0 ** -8 * size).all()
+    out = adapters.lora_add(c["y"], x, a.detach(), b, c["index"], c["scale"], parts=c["parts"])
+    x.grad = None
+    out.backward(c["dy"])      # strides (0, 1)
+    check(x.grad, val["dx"], mag["dx"], 48, "dx")
+
+
+def test_many_blocks_of_many_adapters_repeat():
+    # more blocks than a cluster takes turns for, all of them single tokens of many adapters
+    c = make(256 * 90 + 17, 64, (64,), 16, 40, BF, "cuda", "mixed")
+    want, mag = exact(c)
+    got = _call(c)
+    check(got, want, mag, 64)
+    for _ in range(20):
+        assert torch.equal(got, _call(c))
+
+
+@pytest.mark.parametrize("n", [4, 9, 70])
+def test_gradients_of_blocks_of_many_adapters(n):
+    c = make(1300, 128, (64, 32), 16, n, BF, "cuda", "mixed")
+    c["index"][256:700] = 1      # among them blocks of one
+    _gradients(c, *exact(c, grads=True))
+
+
+@pytest.mark.parametrize("r", [8, 24])
+def test_training_step_captured_and_replayed(r):
+    from easydel_b200.ops import adapters
+
+    c = make(600, 128, (96, 32), r, 3, BF, "cuda", "runs")
+    grad = {k: torch.zeros(c[k].shape, device="cuda", dtype=BF) for k in ("x", "a", "b")}
+
+    def step():
+        leaf = {k: c[k].detach().requires_grad_() for k in ("x", "a", "b")}
+        out = adapters.lora_add(c["y"], leaf["x"], leaf["a"], leaf["b"], c["index"], c["scale"], parts=c["parts"])
+        for k, g in zip(leaf, torch.autograd.grad(out, list(leaf.values()), c["dy"])):
+            grad[k].copy_(g)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for fill in (None, 2, -1):
+        if fill is not None:
+            c["index"].fill_(fill)
+        c["dy"].mul_(-1)
+        graph.replay()
+        val, mag = exact(c, grads=True)
+        for k, length in (("x", 128), ("a", 728), ("b", 728)):
+            check(grad[k], val["d" + k], mag["d" + k], length, "d" + k)
+
+
+def test_refuses_gradients_of_too_many_adapters():
+    c = make(4, 8, (8,), 1, 65536, BF, "cuda", "3")
+    _call(c)
+    c["x"].requires_grad_()
+    with pytest.raises(ValueError, match="65535"):
         _call(c)
