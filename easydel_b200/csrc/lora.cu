@@ -163,6 +163,11 @@ __device__ __forceinline__ void mma_parts(float (&d)[4], const uint32_t (&a)[PA]
       if (o - i >= 0 && o - i < PB) mma_bf16(d, a[i][0], a[i][1], a[i][2], a[i][3], b[o - i][0], b[o - i][1]);
 }
 
+// A kernel that was launched to start early waits here until the one before it, and with that all before, has ended and its results are there;
+// the one before says from where on the next may take the SMs that its blocks leave.
+__device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
 // Sum of the values at `addr` (shared memory) of the CTAs of a cluster, in rank order; all are asked for before the first is used.
@@ -767,6 +772,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_down_kernel(const __grid
   const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x);
   Ring ring = ring_start(shared, dyn, down_stage(np, DOWN_T), DOWN_COLS, a.status);
   find_units(units, dyn, a, row0, (int)min((long long)LORA_ROWS, a.T - row0), DOWN_ROWS);
+  let_next_start();
   if (a.mixed && tid == 0) a.mixed[row0 / LORA_ROWS] = units.mixed;
   const uint32_t idesc = umma_idesc_bf16(128, np, 0, DOWN_T);
   // passes: `each` of a part's ranks in all parts; `at_once` of them fit tensor memory
@@ -1085,6 +1091,8 @@ __global__ void __launch_bounds__(UP_THREADS, 2) lora_up_kernel(const __grid_con
   tc_fence_before();
   find_units(units, dyn, a, row0, (int)min((long long)LORA_ROWS, a.T - row0), UP_ROWS);
   fence_proxy_async_smem();      // the table makes way for copies
+  wait_for_last();
+  let_next_start();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
@@ -1281,27 +1289,30 @@ int shared_memory(const void* kernel, int bytes, const char* what) {
   return 0;
 }
 
+// `early`: the kernel may start while the one before it ends (it waits by itself, see `wait_for_last`).
 template <typename... E, typename... A>
-int launch_sized(void (*k)(E...), dim3 grid, int threads, int cluster, int smem, cudaStream_t stream, const char* what, const A&... args) {
+int launch_sized(void (*k)(E...), dim3 grid, int threads, int cluster, bool early, int smem, cudaStream_t stream, const char* what, const A&... args) {
   if (smem > 40 * 1024 && shared_memory(reinterpret_cast<const void*>(k), smem, what)) return -1;      // 48 KB with the static part
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = cluster;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = early ? 2 : 1;
   return check_cuda(cudaLaunchKernelEx(&cfg, k, args...), what);
 }
 
 template <typename... E, typename... A>
 int launch_cluster(void (*k)(E...), dim3 grid, int cluster, int smem, cudaStream_t stream, const char* what, const A&... args) {
-  return launch_sized(k, grid, LORA_THREADS, cluster, smem, stream, what, args...);
+  return launch_sized(k, grid, LORA_THREADS, cluster, false, smem, stream, what, args...);
 }
 
 // ------------------------------------------------------------------------------------------------------------- gradients
@@ -1493,6 +1504,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_grad_kernel(const __grid
   const int tmem_cols = 4 * rp;
   Ring ring = ring_start(shared, dyn, GRAD_STAGE, tmem_cols, a.status);
   const uint32_t idesc = umma_idesc_bf16(128, rp, 1, 1);
+  wait_for_last();
   bool any = false;
   for (long long at = t.lo; at < t.hi; at += GRAD_LIST) {
     const int found = list_rows(a, ad, at, (int)min((long long)GRAD_LIST, t.hi - at), s_rows, s_scan);
@@ -1734,8 +1746,8 @@ EDL_HOST_API int edl_lora_apply(const edl_lora_shape* shape, const void* x, cons
                      : make_tmap_3d_16b(&map_w, b, r, N, n, ldb, b_adapter, 64, UP_TILE, 1, 3))
           return -1;
         const dim3 up((unsigned)((long long)blocks * g.splits));
-        if (backward ? launch_sized(lora_up_kernel<true>, up, UP_THREADS, 1, UP_SMEM, st, "lora up launch", g, map_y, map_w, map_u, map_out)
-                     : launch_sized(lora_up_kernel<false>, up, UP_THREADS, 1, UP_SMEM, st, "lora up launch", g, map_y, map_w, map_u, map_out))
+        if (backward ? launch_sized(lora_up_kernel<true>, up, UP_THREADS, 1, true, UP_SMEM, st, "lora up launch", g, map_y, map_w, map_u, map_out)
+                     : launch_sized(lora_up_kernel<false>, up, UP_THREADS, 1, true, UP_SMEM, st, "lora up launch", g, map_y, map_w, map_u, map_out))
           return -1;
       } else {
         // a block that is not mixed has at most 16 + MIXED units: they are shared out where there are few CTAs, or where u takes much memory
@@ -1870,7 +1882,7 @@ EDL_HOST_API int edl_lora_grads(const edl_lora_shape* shape, const void* x, cons
     if (a.T && db && (make_tmap_2d_16b(&maps.z[1], dy, a.T, N, ldy, GRAD_ROWS, 64) ||
                       make_tmap_3d_16b(&maps.p[1], u, parts * round16(r), a.T, 2, parts * round16(r), (uint64_t)a.T * parts * round16(r), 64, GRAD_ROWS, 1, 3)))
       return -1;
-    return launch_cluster(lora_grad_kernel, grid, cluster, ring_bytes, st, what, a, maps, rp);
+    return launch_sized(lora_grad_kernel, grid, LORA_THREADS, cluster, true, ring_bytes, st, what, a, maps, rp);
   }
   const int smem = ring_bytes;
   if (in_f32) return wide ? launch_cluster(lora_grad_any_kernel<float, 3, true>, grid, cluster, smem, st, what, a)
