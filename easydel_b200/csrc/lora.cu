@@ -1503,11 +1503,14 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_grad_kernel(const __grid
   const int r16 = round16(job.ru) - t.r0;      // ranks that p has from r0 on
   const int tmem_cols = 4 * rp;
   Ring ring = ring_start(shared, dyn, GRAD_STAGE, tmem_cols, a.status);
-  const uint32_t idesc = umma_idesc_bf16(128, rp, 1, 1);
+  // both parts of p in one product where they fill their boxes
+  const int merged = rp == 64 ? 2 : 1;
+  const uint32_t idesc = umma_idesc_bf16(128, merged * rp, 1, 1);
   wait_for_last();
   bool any = false;
-  for (long long at = t.lo; at < t.hi; at += GRAD_LIST) {
-    const int found = list_rows(a, ad, at, (int)min((long long)GRAD_LIST, t.hi - at), s_rows, s_scan);
+  const int at_once = a.index ? GRAD_LIST : a.T;      // without a list the ring runs dry only once
+  for (long long at = t.lo; at < t.hi; at += at_once) {
+    const int found = list_rows(a, ad, at, (int)min((long long)at_once, t.hi - at), s_rows, s_scan);
     auto row_of = [&](int k) -> long long { return k < found ? (a.index ? (long long)s_rows[k] : at + k) : 0; };
     auto fill = [&](uint32_t dst, int step) {
 #pragma unroll
@@ -1529,8 +1532,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_grad_kernel(const __grid
       for (int q = 0; q < GRAD_ROWS / 16; ++q)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int s = 0; s < 2; ++s)
+          for (int s = 0; s < 2; s += merged)
             umma_f16_ss(ring.tmem + rp * (2 * h + s), umma_smem_desc_sw128(src + 2 * h * GRAD_BOX + 2048 * q, GRAD_BOX, 1024),
                         umma_smem_desc_sw128(src + GRAD_Z + s * GRAD_BOX + 2048 * q, GRAD_BOX, 1024), idesc, !start || step || q);
     };
