@@ -1374,23 +1374,41 @@ __device__ __forceinline__ GradTile grad_tile(const GradArgs& a, int tile, int r
   return t;
 }
 
-// Adds up the CTAs' tiles [ranks][GRAD_STRIDE] through each other's shared memory, in order; each writes its share.
+// Adds up the CTAs' tiles [ranks][GRAD_STRIDE] through each other's shared memory, in order; each writes its share, four columns of a rank at a
+// time (one by one it took 15 us longer for 72 tiles of 64 ranks).
 __device__ __forceinline__ void write_grad(cg::cluster_group& cluster, const GradArgs& a, const GradTile& t, float* tile, int ranks, int ad) {
   const int C = cluster.num_blocks(), c = cluster.block_rank();
   const GradJob& job = t.job;
   cluster_sync_all();
-  const int all = ranks * GRAD_COLS, share = (all + C - 1) / C;
+  constexpr int QUADS = GRAD_COLS / 4;
+  const int all = ranks * QUADS, share = (all + C - 1) / C;
   for (int e = c * share + threadIdx.x; e < min(all, (c + 1) * share); e += LORA_THREADS) {
-    const int rank = job.across ? e % ranks : e / GRAD_COLS, col = job.across ? e / ranks : e % GRAD_COLS;
-    if (t.r0 + rank >= job.ru || t.col0 + col >= job.c1) continue;
-    const float v = cluster_sum(smem_u32(tile + rank * GRAD_STRIDE + col), C);
+    const int rank = job.across ? e % ranks : e / QUADS, col = 4 * (job.across ? e / ranks : e % QUADS), have = job.c1 - t.col0 - col;
+    if (t.r0 + rank >= job.ru || have <= 0) continue;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    cluster_sum4(smem_u32(tile + rank * GRAD_STRIDE + col), C, v);
+    const long long next = job.across ? job.ld_out : 1;      // from one of the four to the next
     const long long pos = (long long)ad * job.out_adapter + (job.across ? (long long)(t.col0 + col) * job.ld_out + t.r0 + rank
                                                                          : (long long)(job.u0 + t.r0 + rank) * job.ld_out + t.col0 + col);
     if (a.out_f32) {
       float* o = reinterpret_cast<float*>(job.out) + pos;
-      *o = a.accumulate ? *o + v : v;
+      if (!job.across && have >= 4 && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
+        float4 b = a.accumulate ? *reinterpret_cast<const float4*>(o) : make_float4(0.f, 0.f, 0.f, 0.f);
+        *reinterpret_cast<float4*>(o) = make_float4(b.x + v[0], b.y + v[1], b.z + v[2], b.w + v[3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < have) o[i * next] = a.accumulate ? o[i * next] + v[i] : v[i];
+      }
     } else {
-      reinterpret_cast<__nv_bfloat16*>(job.out)[pos] = __float2bfloat16_rn(v);
+      __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(job.out) + pos;
+      if (!job.across && have >= 4 && (reinterpret_cast<uintptr_t>(o) & 7) == 0) {
+        *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < have) o[i * next] = __float2bfloat16_rn(v[i]);
+      }
     }
   }
   cluster_sync_all();      // no CTA leaves while its tile is read
