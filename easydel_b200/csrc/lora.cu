@@ -1830,17 +1830,17 @@ EDL_HOST_API int edl_lora_apply(const edl_lora_shape* shape, const void* x, cons
 // da [n][parts * r][K] (+)= g^T x and db [n][N][r] (+)= dy^T u over each adapter's rows (either may be null); the strides of a and b in `shape`
 // are theirs, ldy dy's. g (for da), u (for db): what edl_lora_apply left of the backward and the forward call. out_f32: type of da and
 // db; accumulate (fp32 only): add to them. Adapters without rows get zeros.
-EDL_HOST_API int edl_lora_grads(const edl_lora_shape* shape, const void* x, const void* dy, const void* g, const void* u, const int* index,
+static int lora_grads(const edl_lora_shape* shape, const void* x, const void* dy, const void* g, const void* u, const int* index,
                                 void* da, void* db, int out_f32, int accumulate, int* status, void* stream) {
   const long long ldx = shape->ldx, ldy = shape->ldy, da_adapter = shape->a_adapter, ld_da = shape->lda, db_adapter = shape->b_adapter, ld_db = shape->ldb;
   const int T = shape->T, K = shape->K, N = shape->N, n = shape->n, r = shape->r, parts = shape->parts, in_f32 = shape->x_f32;
   const int* widths = shape->widths;
   if (K <= 0 || N <= 0 || n <= 0 || r <= 0 || parts < 1 || parts > LORA_SEGS || r > 512 / parts || n > 65535 || (!index && n != 1 && T > 0)) {
-    set_last_error("edl_lora_grads: needs sizes above 0, up to %d parts, parts x rank up to 512, up to 65535 adapters, one without an index", LORA_SEGS);
+    set_last_error("edl_lora_backward: needs sizes above 0, up to %d parts, parts x rank up to 512, up to 65535 adapters, one without an index", LORA_SEGS);
     return -1;
   }
   if ((in_f32 && !out_f32) || (accumulate && !out_f32)) {
-    set_last_error("edl_lora_grads: fp32 inputs give fp32 gradients, and only those are accumulated into");
+    set_last_error("edl_lora_backward: fp32 inputs give fp32 gradients, and only those are accumulated into");
     return -1;
   }
   GradArgs a{};
@@ -1862,7 +1862,7 @@ EDL_HOST_API int edl_lora_grads(const edl_lora_shape* shape, const void* x, cons
       wide = wide && widths[p] % 8 == 0;
     }
     if (c0 != N) {
-      set_last_error("edl_lora_grads: the parts have %d columns, the output %d", c0, N);
+      set_last_error("edl_lora_backward: the parts have %d columns, the output %d", c0, N);
       return -1;
     }
     wide = wide && ldy % va == 0 && aligned(dy, 16);
@@ -1908,4 +1908,12 @@ EDL_HOST_API int edl_lora_grads(const edl_lora_shape* shape, const void* x, cons
   if (in_f32) return wide ? launch_cluster(lora_grad_any_kernel<float, 3, true>, grid, cluster, smem, st, what, a)
                           : launch_cluster(lora_grad_any_kernel<float, 3, false>, grid, cluster, smem, st, what, a);
   return launch_cluster(lora_grad_any_kernel<__nv_bfloat16, 2, false>, grid, cluster, smem, st, what, a);
+}
+
+// The backward pass: edl_lora_apply's backward form (`back` null: not wanted, or done by an earlier call), then the gradients of the weights.
+EDL_HOST_API int edl_lora_backward(const edl_lora_shape* back, const edl_lora_shape* shape, const void* x, const void* dy, const void* a, const void* b,
+                                   const int* index, const float* scale, float scale_all, void* g, long long g_size, int* mixed, void* dx,
+                                   const void* u, void* da, void* db, int out_f32, int accumulate, int* status, void* stream) {
+  if (back && edl_lora_apply(back, dy, nullptr, dx, a, b, index, scale, scale_all, g, g_size, mixed, status, stream)) return -1;
+  return da || db ? lora_grads(shape, x, dy, g, u, index, da, db, out_f32, accumulate, status, stream) : 0;
 }

@@ -28,7 +28,7 @@ class _Shape(C.Structure):
 
 
 _lib.register("edl_lora_apply", i32, [vp, vp, vp, vp, vp, vp, vp, vp, f32, vp, i64, vp, vp, vp])
-_lib.register("edl_lora_grads", i32, [vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, vp, vp])
+_lib.register("edl_lora_backward", i32, [vp, vp, vp, vp, vp, vp, vp, vp, f32, vp, i64, vp, vp, vp, vp, vp, i32, i32, vp, vp])
 
 MAX_RANK = 512       # ranks of all parts together
 MAX_PARTS = 8
@@ -121,6 +121,7 @@ class _Plan:
         self.ref = C.addressof(self.shape)
         self.u_parts, self.u_cols = 3 if res.dtype == torch.float32 else 2, _inner_columns(r, len(parts), backward)
         self.blocks = -(-T // FEW_ROWS) if T > FEW_ROWS else 0
+        self.plain = False      # all operands, as the caller has them, are rows that kernels read
         self.back = self.grads = None      # the plans of the backward pass's calls, where all operands are contiguous
 
     def inner(self, x: torch.Tensor) -> torch.Tensor:
@@ -173,36 +174,47 @@ class _LoraAddFn(torch.autograd.Function):
         if scale is None:
             scale = ctx.scale
         plan, (need_y, need_x, need_a, need_b) = ctx.plan, ctx.needs_input_grad[:4]
-        dy2 = dy if _matrix(dy) else _rows(dy)
+        dy2 = dy if dy.is_contiguous() or _matrix(dy) else _rows(dy)
         da, a_added = _grad_target(a) if need_a else (None, False)
         db, b_added = _grad_target(b) if need_b else (None, False)
-        dx = x.new_empty(ctx.x_shape) if need_x else None
-        g = None
+        dx = g = back = mixed = None
+        g_size = 0
         if need_x or need_a:
-            a2, b2 = _weights(a), _weights(b)
+            a2, b2 = (a, b) if plan.plain else (_weights(a), _weights(b))
+            if need_x:
+                dx = torch.empty_like(x) if x.shape == ctx.x_shape and x.is_contiguous() else x.new_empty(ctx.x_shape)
             usual = need_x and dy2.is_contiguous()
             back = plan.back if usual else None
             if back is None:
                 back = _Plan(dy2, None, dx, a2, b2, plan.parts, True)
                 if usual:
                     plan.back = back
-            g = back.inner(x) if need_a else None
-            _apply(back, dy2, None, dx, a2, b2, index, scale, g)
-        # one launch for both, unless only one of them is added to a flat buffer
+            if need_a or back.blocks:
+                g = back.inner(x)
+                g_size = g.numel()
+            if back.blocks and index is not None:
+                mixed = index.new_empty(back.blocks)
+        else:
+            a2 = b2 = None
+        # one call for all, unless only one of the weights' gradients is added to a flat buffer
         for ta, tb, added in ((da, db, a_added or b_added),) if da is None or db is None or a_added == b_added else \
                 ((da, None, a_added), (None, db, b_added)):
-            if ta is None and tb is None:
+            out = ta if tb is None else tb
+            if back is None and out is None:
                 continue
             usual = dy2.is_contiguous() and (ta is None or ta.is_contiguous()) and (tb is None or tb.is_contiguous())
             grads = plan.grads if usual else None
-            if grads is None:
+            if grads is None and out is not None:
                 grads = _Plan(x, dy2, None, torch.empty_like(a, device="meta", memory_format=torch.contiguous_format) if ta is None else ta,
                               torch.empty_like(b, device="meta", memory_format=torch.contiguous_format) if tb is None else tb, plan.parts)
                 if usual:
                     plan.grads = grads
-            _lib.call_on(x.device, "edl_lora_grads", grads.ref, x.data_ptr(), dy2.data_ptr(), _lib.ptr(g), _lib.ptr(u), _lib.ptr(index),
-                         _lib.ptr(ta), _lib.ptr(tb), (ta if tb is None else tb).dtype == torch.float32, added,
-                         _lib.status_word(x.device).data_ptr())
+            tensor = type(scale) is not float
+            _lib.call_on(x.device, "edl_lora_backward", None if back is None else back.ref, None if grads is None else grads.ref, x.data_ptr(),
+                         dy2.data_ptr(), _lib.ptr(a2), _lib.ptr(b2), _lib.ptr(index), scale.data_ptr() if tensor else None,
+                         0.0 if tensor else scale, _lib.ptr(g), g_size, _lib.ptr(mixed), _lib.ptr(dx), _lib.ptr(u), _lib.ptr(ta), _lib.ptr(tb),
+                         out is not None and out.dtype == torch.float32, added, _lib.status_word(x.device).data_ptr())
+            back = None
         if a_added:
             a.grad_added_to_main_grad = True
         if b_added:
