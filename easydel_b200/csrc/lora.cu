@@ -567,17 +567,13 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const __grid_cons
     const T* wu = reinterpret_cast<const T*>(a.up) + (long long)(ad < 0 ? 0 : ad) * a.up_adapter;
     for (int grp = g0 + w; a.out && grp < g1; grp += 2 * LORA_WARPS) {
       int2 at[2];      // first column, part
-      float acc[2][4][4], yv[2][2][8];
+      float acc[2][4][4];
       long long row[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) row[h] = 8 * h + g < m ? row0 + order[8 * h + g] : -1;
 #pragma unroll
       for (int d = 0; d < 2; ++d) {
         at[d] = grp + d * LORA_WARPS < g1 ? column_of(grp + d * LORA_WARPS) : make_int2(0, -1);
-        const int col = at[d].x + 8 * t4, ok = at[d].y < 0 ? 0 : a.up_seg[at[d].y].c1 - col;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          load_row<TY, WIDE>(reinterpret_cast<const TY*>(a.y) + row[h] * a.ldy + col, a.y && row[h] >= 0 ? ok : 0, yv[d][h]);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -612,8 +608,9 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const __grid_cons
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float v[8];
+          load_row<TY, WIDE>(reinterpret_cast<const TY*>(a.y) + row[h] * a.ldy + col, a.y && row[h] >= 0 ? ok : 0, v);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = yv[d][h][e] + acc[d][e >> 1][2 * h + (e & 1)];
+          for (int e = 0; e < 8; ++e) v[e] += acc[d][e >> 1][2 * h + (e & 1)];
           store_row<TY, WIDE>(reinterpret_cast<TY*>(a.out) + row[h] * a.ldo + col, row[h] >= 0 ? ok : 0, v);
         }
       }
