@@ -168,8 +168,6 @@ __device__ __forceinline__ void mma_parts(float (&d)[4], const uint32_t (&a)[PA]
 __device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
-
 // Sum of the values at `addr` (shared memory) of the CTAs of a cluster, in rank order; all are asked for before the first is used.
 __device__ __forceinline__ float cluster_sum(uint32_t addr, int C) {
   float v[8], sum = 0.f;
@@ -426,20 +424,6 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const __grid_cons
     const short* order = units.order + units.base[unit];
 
     if (ad >= 0) {
-      // ---- the weights and y of the second product start towards L2
-      if (a.out && g1 > g0) {
-        const int n0 = column_of(g0).x, n1 = min(column_of(g1 - 1).x + 32, a.up_seg[a.up_segs - 1].c1);
-        const T* wu = reinterpret_cast<const T*>(a.up) + (long long)ad * a.up_adapter;
-        constexpr int LINE = 128 / (int)sizeof(T);
-        if constexpr (!DOWN_T) {
-          for (long long i = n0 * a.ld_up + tid * LINE; i < n1 * a.ld_up; i += LORA_THREADS * LINE) prefetch_l2(wu + i);
-        } else {
-          const int lines = (n1 - n0 + LINE - 1) / LINE;
-          for (int i = tid; i < lines * a.up_seg[0].ru; i += LORA_THREADS) prefetch_l2(wu + (long long)(i / lines) * a.ld_up + n0 + i % lines * LINE);
-        }
-        if (a.y && n0 + tid * 64 < n1)
-          for (int i = 0; i < m; ++i) prefetch_l2(reinterpret_cast<const TY*>(a.y) + (row0 + order[i]) * a.ldy + n0 + tid * 64);
-      }
       // ---- this CTA's share of u: ranks are the rows of the product, tokens its columns
       const T* wd = reinterpret_cast<const T*>(a.down) + (long long)ad * a.down_adapter;
       const T* xr[NT];
