@@ -272,7 +272,8 @@ struct UnitTable {
 
 // Among many rows, a block of LORA_ROWS rows of more adapters than this (the single tokens of a step) goes to the one-launch kernel, whose
 // clusters take a few rows of an adapter each; the streaming kernels take the others. Every kernel of a call decides so for itself.
-// 3900 rows, 256 of them single tokens of 64 adapters: see the end of edl_lora_apply.
+// 3900 rows, 4096 columns to 4096, rank 16, 256 of them single tokens of 16 (64) adapters: 56 (67) us; 169 (531) where the streaming kernels took
+// all of them. Where there is nothing to take, the third launch costs 8 us.
 constexpr int MIXED = 4;
 
 // Exclusive sum over the CTA's threads; `total` gets the sum of all.
@@ -298,7 +299,7 @@ __device__ __forceinline__ int cta_scan(int v, int* scan, int& total) {
 // All threads of the CTA. Rows without an adapter form units (adapter -1) where they have to be copied. Most blocks of a prompt or a
 // training batch belong to one request: those take no look-up. Else rows of one adapter find each other within their warp (`match`) and
 // across warps through a slot of a hash table, whose place decides nothing: units are numbered by their first rows.
-// 256 rows of 64 adapters: 1.4 us; 4.9 us when every row compared itself with all others.
+// 256 rows of 64 adapters: 2.7 us from the launch on; 4.9 us when every row compared itself with all others.
 __device__ __forceinline__ void find_units(RowUnits& u, void* scratch, const LoraArgs& a, long long row0, int rows, int chunk) {
   UnitTable& t = *reinterpret_cast<UnitTable*>(scratch);
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
@@ -1601,6 +1602,11 @@ bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) 
 
 using namespace edl;
 
+// Rows that one launch takes: up to 512, or 256 of a wide output that all belong to one adapter, whose weights are read again for every 16 rows.
+// 4096 columns to 4096, rank 16: 512 rows of one adapter take 16.4 us against 25.6 in two launches, of eight 18.5 against 42, 768 rows 22-25
+// against 42. To 28672 columns: 512 rows of one adapter 43 against 34, of eight 46 against 50.
+static bool few_rows(int T, int cols, bool index) { return T <= 256 || (T <= 512 && (index || cols <= 8192)); }
+
 // Sizes of a call: strides in elements, `widths` columns of the `parts` parts of N. x_f32: x and the weights are fp32 (then y and out
 // too), else bf16; y_f32: type of y and out.
 struct edl_lora_shape {
@@ -1611,8 +1617,8 @@ struct edl_lora_shape {
 // x [T, K], y and out [T, N] (y null: the adapters' part alone; y == out: in place). a: [n][parts * r][K], b: [n][N][r].
 // backward = 0: out = y + s (x a^T) b^T. backward = 1: x is dy [T, N], out dx [T, K] (null: u alone), y null. u: s x a^T or s dy b
 // in bf16 parts (2 for bf16 results, 3 for fp32 ones), [parts][T][columns] with parts * r rounded up to 16 per part (forward) or as a
-// whole (backward); asked for above 256 rows of bf16, else it may be null. mixed: a flag per 256 rows, scratch; asked for above 256 rows of
-// bf16 with an index. index [T] int32 or null (adapter 0 everywhere), scale [n] fp32 or null (scale_all). Indexes from n on set the status
+// whole (backward); asked for with many rows (see `few_rows`) of bf16, else it may be null. mixed: a flag per 256 rows, scratch; asked for
+// with many rows of bf16 and an index. index [T] int32 or null (adapter 0 everywhere), scale [n] fp32 or null (scale_all). Indexes from n on set the status
 // word and count as none.
 EDL_HOST_API int edl_lora_apply(const edl_lora_shape* shape, const void* x, const void* y, void* out, const void* a, const void* b,
                                 const int* index, const float* scale, float scale_all, void* u, long long u_size, int* mixed,
@@ -1688,18 +1694,19 @@ EDL_HOST_API int edl_lora_apply(const edl_lora_shape* shape, const void* x, cons
     return groups > in_block ? in_block : groups;
   };
 
-  if (wide && !x_f32 && T > LORA_ROWS) {
+  if (wide && !x_f32 && !few_rows(T, backward ? K : N, index)) {
     if (!u) {
-      set_last_error("edl_lora_apply: more than %d rows need u", LORA_ROWS);
+      set_last_error("edl_lora_apply: %d rows need u", T);
       return -1;
     }
     const bool may_mix = index && n + 1 > MIXED;      // rows without an adapter count as one
     if (may_mix && !mixed) {
-      set_last_error("edl_lora_apply: more than %d rows of %d adapters need a flag per block of rows", LORA_ROWS, n);
+      set_last_error("edl_lora_apply: %d rows of %d adapters need a flag per block of rows", T, n);
       return -1;
     }
     g.mixed = may_mix ? mixed : nullptr;
-    // a block has two units, one more for each end of a request within it; a third cluster takes most of those
+    // a block has two units, one more for each end of a request within it; a third cluster takes most of those (six, most of them idle,
+    // took 4 us longer for 3900 rows)
     g.groups = groups_of(DOWN_ROWS);
     if (g.groups > 3) g.groups = 3;
     int ru = 0, cols = 0;
@@ -1734,7 +1741,8 @@ EDL_HOST_API int edl_lora_apply(const edl_lora_shape* shape, const void* x, cons
       for (int i = 0; i < g.up_segs; ++i) g.groups += (g.up_seg[i].c1 - g.up_seg[i].c0 + width - 1) / width;
       if (tiles) {
         // a block's columns are cut into as many CTAs as run at once (two per SM), or three times that where blocks may have more
-        // units than others, of at least four tiles
+        // units than others, of at least four tiles. 28672 columns, 3900 rows of 8 requests: 128 us, 164 without the three times; 4096
+        // columns, 8192 rows without an index: 52 us, 56 with them.
         const int ctas = (index ? 6 : 2) * sms / blocks;
         g.splits = ctas < g.groups / 4 ? ctas : g.groups / 4;
         if (g.splits < 1) g.splits = 1;

@@ -33,7 +33,7 @@ _lib.register("edl_lora_backward", i32, [vp, vp, vp, vp, vp, vp, vp, vp, f32, vp
 MAX_RANK = 512       # ranks of all parts together
 MAX_PARTS = 8
 MAX_TRAINED = 65535  # adapters of a call with gradients
-FEW_ROWS = 256       # up to here the inner value stays in shared memory
+BLOCK = 256          # rows that are looked through for their adapters together
 
 
 def _matrix(t: torch.Tensor) -> bool:
@@ -103,12 +103,17 @@ def _inner_columns(r: int, parts: int, backward: bool) -> int:
     return -(-parts * r // 16) * 16 if backward else parts * (-(-r // 16) * 16)
 
 
+def _few_rows(T: int, cols: int, index: bool) -> bool:
+    """``few_rows`` of ``csrc/lora.cu``: the inner value stays in shared memory."""
+    return T <= 256 or T <= 512 and (index or cols <= 8192)
+
+
 class _Plan:
     """What a call's sizes, strides and types decide: checked once, kept for the calls that follow with the same ones."""
 
     __slots__ = ("parts", "plain", "shape", "ref", "u_parts", "u_cols", "blocks", "T", "back", "grads")
 
-    def __init__(self, x, y, out, a, b, parts, backward=False):
+    def __init__(self, x, y, out, a, b, parts, index, backward=False):
         n, N, r = b.shape
         # (strides along dimensions of one element mean nothing)
         rows = lambda t: 0 if t is None else t.stride(-2) if t.dim() > 1 and t.shape[-2] > 1 else t.shape[-1]  # noqa: E731
@@ -120,7 +125,7 @@ class _Plan:
                             x.dtype == torch.float32, res.dtype == torch.float32, backward, (i32 * 8)(*parts))
         self.ref = C.addressof(self.shape)
         self.u_parts, self.u_cols = 3 if res.dtype == torch.float32 else 2, _inner_columns(r, len(parts), backward)
-        self.blocks = -(-T // FEW_ROWS) if T > FEW_ROWS else 0
+        self.blocks = 0 if _few_rows(T, a.shape[2] if backward else N, index is not None) else -(-T // BLOCK)
         self.plain = False      # all operands, as the caller has them, are rows that kernels read
         self.back = self.grads = None      # the plans of the backward pass's calls, where all operands are contiguous
 
@@ -159,7 +164,7 @@ class _LoraAddFn(torch.autograd.Function):
         ctx.x_shape, a2, b2 = x.shape, a, b
         if not plan.plain:
             y, x, a2, b2 = _rows(y), _rows(x), _weights(a), _weights(b)
-            plan = _Plan(x, y, out, a2, b2, plan.parts)
+            plan = _Plan(x, y, out, a2, b2, plan.parts, index)
         u = plan.inner(x) if ctx.needs_input_grad[3] else None
         _apply(plan, x, y, out, a2, b2, index, scale, u)
         ctx.scale, ctx.plan = scale if type(scale) is float else None, plan
@@ -186,7 +191,7 @@ class _LoraAddFn(torch.autograd.Function):
             usual = need_x and dy2.is_contiguous()
             back = plan.back if usual else None
             if back is None:
-                back = _Plan(dy2, None, dx, a2, b2, plan.parts, True)
+                back = _Plan(dy2, None, dx, a2, b2, plan.parts, index, True)
                 if usual:
                     plan.back = back
             if need_a or back.blocks:
@@ -206,7 +211,7 @@ class _LoraAddFn(torch.autograd.Function):
             grads = plan.grads if usual else None
             if grads is None and out is not None:
                 grads = _Plan(x, dy2, None, torch.empty_like(a, device="meta", memory_format=torch.contiguous_format) if ta is None else ta,
-                              torch.empty_like(b, device="meta", memory_format=torch.contiguous_format) if tb is None else tb, plan.parts)
+                              torch.empty_like(b, device="meta", memory_format=torch.contiguous_format) if tb is None else tb, plan.parts, index)
                 if usual:
                     plan.grads = grads
             tensor = type(scale) is not float
@@ -235,7 +240,7 @@ def _plan_of(y, x, a, b, index, scale, parts, out) -> _Plan:
     plan = _plans.get(key)
     if plan is None:
         parts = _check(y, x, a, b, index, scale, parts, out)
-        plan = _Plan(x, y, torch.empty_like(y, device="meta", memory_format=torch.contiguous_format) if out is None else out, a, b, parts)
+        plan = _Plan(x, y, torch.empty_like(y, device="meta", memory_format=torch.contiguous_format) if out is None else out, a, b, parts, index)
         # operands whose rows have to be copied first, and results that cannot be written as rows, take the long way
         plan.plain = x.is_cuda and all(map(_matrix, (x, y) if out is None else (x, y, out))) and _stack(a) and _stack(b)
         if len(_plans) >= 4096:
@@ -280,7 +285,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
         return out.copy_(lora_add(y, x, a, b, index, scale, parts=plan.parts))
     res = torch.empty_like(y, memory_format=torch.contiguous_format) if out is None else out
     x2, y2, a2, b2 = _rows(x), res if res is y else _rows(y), _weights(a), _weights(b)
-    _apply(_Plan(x2, y2, res, a2, b2, plan.parts), x2, y2, res, a2, b2, index, scale, None)
+    _apply(_Plan(x2, y2, res, a2, b2, plan.parts, index), x2, y2, res, a2, b2, index, scale, None)
     return res
 
 

@@ -335,3 +335,53 @@ def test_refuses_gradients_of_too_many_adapters():
     c["x"].requires_grad_()
     with pytest.raises(ValueError, match="65535"):
         _call(c)
+
+
+@pytest.mark.parametrize("T", [512, 513, 900])
+@pytest.mark.parametrize("index", ["none", "runs", "bare", "2"])
+def test_index_patterns_of_many_rows(index, T):
+    test_index_patterns(index, T)
+
+
+@pytest.mark.parametrize("r,parts", [(128, (64,)), (256, (64, 32)), (512, (40,)), (100, (16,) * 5), (64, (8,) * 8), (12, (24, 16))])
+def test_high_and_odd_ranks_of_many_rows(r, parts):
+    test_high_ranks(600, r, parts)
+
+
+def test_float32_output_beside_many_bf16_rows():
+    for T, r, parts in ((600, 16, (64, 32)), (900, 72, (96,)), (900, 4, (40,))):
+        c = make(T, 320, parts, r, 3, BF, "cuda")
+        c["y"] = c["y"].float() * 1.0001
+        want, mag = exact(c)
+        check(_call(c), want, mag, 320)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_strides_and_alignment_of_many_rows(dtype):
+    test_strides_and_alignment(dtype, 700)
+
+
+def test_values_that_are_not_finite_stay_with_their_row_and_adapter_among_many():
+    test_values_that_are_not_finite_stay_with_their_row_and_adapter(700)
+
+
+@pytest.mark.parametrize("T", [256, 257, 512, 513])
+@pytest.mark.parametrize("index", ["none", "runs"])
+def test_wide_outputs_on_both_sides_of_the_forms(T, index):
+    c = make(T, 64, (8200,), 16, 1 if index == "none" else 3, BF, "cuda", index)
+    want, mag = exact(c)
+    check(_call(c), want, mag, 64)
+    c = make(T, 8200, (64,), 16, 1 if index == "none" else 3, BF, "cuda", index)      # the backward pass is the wide one
+    _gradients(c, *exact(c, grads=True))
+
+
+def test_frozen_rows_of_a_wide_input():
+    from easydel_b200.ops import adapters
+
+    for K, N in ((8200, 64), (64, 8200)):
+        c = make(300, K, (N,), 16, 1, BF, "cuda", "none")
+        val, mag = exact(c, grads=True)
+        a, b = (c[k].detach().requires_grad_() for k in ("a", "b"))
+        adapters.lora_add(c["y"], c["x"], a, b, None, c["scale"]).backward(c["dy"])
+        check(a.grad, val["da"], mag["da"], 300 + N, "da")
+        check(b.grad, val["db"], mag["db"], 300 + K, "db")
