@@ -384,6 +384,12 @@ __device__ __forceinline__ void find_units(RowUnits& u, void* scratch, const Lor
 // takes eight neighbouring elements with one 16-byte load and calls them the four register pairs of two m16n8k16 products; the same
 // holds for output columns. Weights that are needed across their rows (the backward pass) are turned in registers (`movmatrix`).
 // DOWN_T: the weights of the first product lie [columns][ranks] (B in the backward pass) and those of the second [ranks][columns].
+//
+// One row, 4096 columns to 4096, rank 16: 8 us (start 1.3, contraction 1.8, cluster 0.7, u 0.8, expansion 2); 48 rows of 32 adapters to 6144
+// columns in three parts: 16 us; 256 rows of 64 adapters, 14336 to 4096, rank 32: 33 us, 2.5 TB/s of 83 MB (all cold). What bounds the last: an SM
+// has two CTAs or one (252 of 296 places), a warp's loads of a step follow the last step's products, and the expansion reads its weights
+// after the cluster has met. Weights copied ahead into rings in shared memory, or asked for before the cluster met, gained nothing.
+// 4096 rows of fp32, 4096 to 4096: 108 us, bound by the nine products of parts.
 template <typename T, typename TY, int RT, bool DOWN_T, bool WIDE>
 __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const __grid_constant__ LoraArgs a) {
   constexpr int NT = 2, CHUNK = 8 * NT;
@@ -741,6 +747,8 @@ __device__ __forceinline__ void ring_end(Ring& r, int tmem_cols) {
 // u of up to 128 rows of one adapter (the M side; ranks are the N side): columns in steps of 64 through the ring, cut over the CTAs of a
 // cluster where there are few rows. Passes (up to 64 ranks of a part) run one after the other into columns of their own of tensor memory,
 // up to 128 at a time, before the CTAs' sums are added, in a fixed order.
+// 8192 rows: 4096 columns, rank 16: 22 us, 67 MB at 3.0 TB/s; 14336 columns, rank 64: 57 us, 4.1 TB/s. It is bound by the stream of x while that
+// lasts (15 of the 22 us); the rest is its start and the sums' way through the cluster.
 constexpr int DOWN_ROWS = 128, DOWN_K = 64, DOWN_X = DOWN_ROWS * DOWN_K * 2, DOWN_RANKS = 64, DOWN_COLS = 128;
 __host__ __device__ constexpr int down_stage(int np, bool down_t) { return DOWN_X + (down_t ? DOWN_K : np) * 128; }
 
@@ -913,7 +921,8 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_down_kernel(const __grid
 // What no TMA box fits or tensor memory holds (fp32 outputs, ranks that are no multiple of 8 or above 64), on `mma.sync`. A CTA takes 256
 // columns of one part (32 per warp) of some of a block's units of 16 rows. The rows' u goes to shared memory once, the weights of
 // a warp's columns stay in registers for all rows of an adapter (up to 16 KC ranks); what remains per 16 rows is to read y, asked for
-// two turns ahead, and to write out.
+// two turns ahead, and to write out. 4096 rows, 4096 columns: rank 12 27 us (67 MB at 2.4 TB/s), fp32 rank 16 35 us (134 MB at 3.8 TB/s): traffic;
+// rank 128 72 us: `mma.sync`, 20 clocks a product and scheduler, and weights that are read again for every 16 rows.
 constexpr int UP_COLS = 32 * LORA_WARPS;
 template <typename TY, int KC, bool UP_T>
 __global__ void __launch_bounds__(LORA_THREADS, 2) lora_up_any_kernel(const __grid_constant__ LoraArgs a) {
@@ -1040,6 +1049,8 @@ __device__ __forceinline__ void store_64(void* p, const uint32_t (&v)[16], bool 
 // A lane loads tiles of y and of the weights ahead (TMA), a lane of the second warp issues the products into one of two accumulators, and
 // two times four warps, a row per lane, add every other tile to y where it lies and send it out as boxes of 32 rows (TMA). What bounds it is
 // the traffic of y and out. Rows of y that lanes asked for themselves, two tiles ahead, took a third longer than by TMA.
+// 8192 rows, 4096 columns: 27 us, 134 MB at 5.0 TB/s; 3900 rows of 8 requests, 28672 columns: 95 us, 447 MB at 4.7 TB/s; without y (the backward
+// pass), 14336 columns: 59 us, 235 MB at 4.0 TB/s.
 constexpr int UP_THREADS = 320, UP_ROWS = 128, UP_TILE = 64, UP_STAGES = 3;
 constexpr int UP_Y = UP_ROWS * UP_TILE * 2, UP_W = 64 * 128, UP_STAGE = UP_Y + UP_W, UP_U = UP_ROWS * 128;
 constexpr int UP_SMEM = UP_STAGES * UP_STAGE + 2 * UP_U + 1024;
@@ -1405,7 +1416,8 @@ __device__ __forceinline__ void write_grad(cg::cluster_group& cluster, const Gra
 
 // out[rank, col] (+)= sum over the adapter's rows t of p[t, rank] z[t, col]: ranks x 256 columns per cluster, the rows cut over its CTAs.
 // This form takes rows of any alignment and fp32 ones: 16 ranks at a time, operands along their rows from global memory, turned in registers.
-// Warps 0-3 and 4-7 take every other 16 rows.
+// Warps 0-3 and 4-7 take every other 16 rows. 1000 rows, 1023 and 1021 columns, rank 5: 12 us; 4096 rows of fp32, 4096 and 4096 columns, rank 16:
+// 139 us, bound by its products of parts.
 template <typename T, int S, bool WIDE>
 __global__ void __launch_bounds__(LORA_THREADS, 1) lora_grad_any_kernel(const __grid_constant__ GradArgs a) {
   constexpr int P = PARTS<T>;
@@ -1488,7 +1500,9 @@ __global__ void __launch_bounds__(LORA_THREADS, 1) lora_grad_any_kernel(const __
 }
 
 // The same for bf16 rows that 16-byte copies fit: 32 rows at a time through the ring. z's columns are the M side (128 at a time), both parts of
-// p side by side the N side, and the rows the inner index of the products; both operands lie along M and N.
+// p side by side the N side, and the rows the inner index of the products; both operands lie along M and N. 8192 rows: 4096 and 4096 columns,
+// rank 16: 35 us, 134 MB at 3.8 TB/s; 14336 and 4096 columns, rank 64: 72 us, 302 MB at 4.2 TB/s. Its stream bounds it: without the products
+// both take 4 us less, without the reads of p 2 us less.
 constexpr int GRAD_ROWS = 32, GRAD_Z = GRAD_ROWS * GRAD_COLS * 2, GRAD_BOX = GRAD_ROWS * 128, GRAD_STAGE = GRAD_Z + 2 * GRAD_BOX;
 struct GradMaps {
   CUtensorMap z[2], p[2];      // of dA's and dB's inputs
