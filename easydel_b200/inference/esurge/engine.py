@@ -508,6 +508,11 @@ class eSurge:
                 continue
             tok = sampled[rid]
             req = s.request
+            if req.rules is not None and req.rules.error is not None:      # its grammar failed: the step's token means nothing
+                self.scheduler.finish_request(req, RequestStatus.FINISHED_ABORTED)
+                del req.output_token_ids[-1:]
+                fin[rid] = req
+                continue
             if len(req.output_token_ids) == 1:
                 self.metrics.record_first_token(rid)
             delta = tr.detok.push([tok])
@@ -537,7 +542,7 @@ class eSurge:
             self.metrics.finish_request(rid, len(req.output_token_ids))
             if tr is not None:
                 tr.finished = True
-                tr.finish_reason = req.status.value
+                tr.finish_reason = req.status.value if req.rules is None or req.rules.error is None else f"error: {req.rules.error!r}"
                 tr.event.set()
 
     def _loop(self) -> None:

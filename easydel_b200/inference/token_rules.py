@@ -5,7 +5,7 @@
 
 A grammar is a callable in ``SamplingParams.guided_decoding``: ``f(prompt_token_ids, output_token_ids)`` returns the tokens allowed next (ids,
 or packed int32 words with bit ``t % 32`` of word ``t // 32`` for token t), or None where everything is. Requests with one are read back after
-every step, since the next mask needs the token.
+every step, since the next mask needs the token. One that raises, or allows nothing, ends its own request with that error.
 """
 
 from __future__ import annotations
@@ -48,6 +48,7 @@ class TokenRules:
         self.allowed = None if sp.allowed_token_ids is None else pack_tokens(sp.allowed_token_ids, vocab)
         if self.allowed is not None and not self.allowed.any():
             raise ValueError("allowed_token_ids is empty")
+        self.error: Exception | None = None      # of the grammar
 
     @classmethod
     def of(cls, sp, vocab: int, end_tokens: tp.Sequence[int]) -> "TokenRules | None":
@@ -63,8 +64,15 @@ class TokenRules:
 
     def mask(self, prompt: list[int], output: list[int]) -> np.ndarray | None:
         m = self.allowed
-        if self.grammar is None:
+        if self.grammar is None or self.error is not None:
             return m
+        try:
+            return self._grammar_mask(m, prompt, output)
+        except Exception as e:  # the user's code: other requests of the step go on
+            self.error = e
+            return m
+
+    def _grammar_mask(self, m: np.ndarray | None, prompt: list[int], output: list[int]) -> np.ndarray | None:
         g = self.grammar(prompt, output)
         if g is None:
             return m
@@ -74,7 +82,10 @@ class TokenRules:
             g = np.ascontiguousarray(g)
         else:
             g = pack_tokens((int(t) for t in g), self.vocab)
-        return g if m is None else m & g
+        g = g if m is None else m & g
+        if not g.any():
+            raise ValueError("the grammar allows no token")
+        return g
 
 
 def collect(rules: tp.Sequence["TokenRules | None"], requests: tp.Sequence, device) -> dict[str, tuple]:

@@ -390,7 +390,7 @@ def sample_reference(logits, *, temperature=None, top_k=None, top_p=None, min_p=
     for r in range(R_):
         t = float(temperature[r]) if temperature is not None else 0.0
         k = int(top_k[r]) if top_k is not None else 0
-        if t <= 0 or k == 1:
+        if t <= 0 or k == 1 or bool((z[r] == -float("inf")).all()):      # (or nothing is allowed: token 0, as the kernel's)
             i = int(torch.argmax(z[r]))
             out[r] = i
             lps[r] = torch.log_softmax(z[r], -1)[i]

@@ -219,3 +219,33 @@ def test_layout_of_rules():
 def test_refusals_of_rules(kw):
     with pytest.raises(ValueError):
         _engine(_model()).add_request(PROMPTS[0], SamplingParams(**kw))
+
+
+@pytest.mark.parametrize("asynchronous", [False, True])
+@pytest.mark.parametrize("last", [2, 5])
+def test_a_grammar_that_fails_ends_its_own_request(asynchronous, last):
+    def raises(prompt, output):
+        if len(output) == last:
+            raise KeyError("state")
+        return [30]
+
+    def dead_end(prompt, output):
+        return [31] if len(output) < last else []
+
+    def outside(prompt, output):
+        return [32] if len(output) < last else [200]
+
+    mk = lambda g: SamplingParams(max_tokens=6, temperature=0.0, ignore_eos=True, guided_decoding=g)  # noqa: E731
+    eng = _engine(_model(), asynchronous)
+    outs = [o.outputs[0] for o in eng.generate(PROMPTS[:4], [mk(raises), mk(dead_end), mk(outside), mk(None)])]
+    for o, t, what in zip(outs, (30, 31, 32), ("KeyError", "no token", "vocabulary")):
+        assert o.token_ids == [t] * last and o.finish_reason.startswith("error") and what in o.finish_reason
+    assert outs[3].token_ids == _engine(_model()).generate(PROMPTS[3], mk(None))[0].outputs[0].token_ids
+    assert not eng.scheduler.has_unfinished() and len(eng._free_slots) == eng.runner.max_num_seqs
+
+
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+def test_rules_that_leave_nothing_still_give_a_token(temperature):
+    sp = SamplingParams(max_tokens=3, temperature=temperature, allowed_token_ids=[7], logit_bias={7: -float("inf")}, ignore_eos=True)
+    o = _engine(_model()).generate(PROMPTS[0], sp)[0].outputs[0]
+    assert len(o.token_ids) == 3 and all(0 <= t < 200 for t in o.token_ids)

@@ -139,3 +139,20 @@ def test_requests_without_an_adapter_are_served_as_by_an_engine_without_room_for
         outs.append([o.outputs[0].token_ids for o in eng.generate([[5, 6, 7], list(range(200))], SamplingParams(max_tokens=10, temperature=0.0, ignore_eos=True))])
         eng.close()
     assert outs[0] == outs[1]
+
+
+@pytest.mark.parametrize("vocab", [100, 50257])
+def test_rows_that_rules_leave_nothing_still_give_a_token(vocab):
+    from easydel_b200.ops import serving as S
+
+    z = torch.randn(5, vocab, device="cuda")
+    bits = torch.zeros(1, (vocab + 31) // 32, dtype=torch.int32, device="cuda")
+    rows = torch.tensor([-1, 0, -1, 0, -1], dtype=torch.int32, device="cuda")
+    z = S.adjust_logits(z, mask=(bits, rows))
+    assert (z[1] == -float("inf")).all() and torch.isfinite(z[0]).all()
+    for t in (0.0, 0.8):
+        kw = {} if not t else dict(temperature=torch.full((5,), t, device="cuda"), top_p=torch.full((5,), 0.9, device="cuda"),
+                                   min_p=torch.zeros(5, device="cuda"), top_k=torch.zeros(5, dtype=torch.int32, device="cuda"),
+                                   seeds=torch.arange(5, device="cuda"), steps=torch.zeros(5, dtype=torch.int32, device="cuda"))
+        tokens, _ = S.sample(z, **kw)
+        assert ((tokens >= 0) & (tokens < vocab)).all()
