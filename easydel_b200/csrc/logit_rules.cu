@@ -12,13 +12,14 @@
 // forbidden tokens skip those steps.
 //
 // One row of 32000: 3.2 us, 7 rows of 50257 with counts: 5 us (launch and one round of loads); 64 rows of 128256, half of them with counts and
-// half with masks: 20 us, 66 MB at 3.3 TB/s (three rounds of CTAs of unlike work); 256 fp32 rows of 151936: 75 us, 436 MB at 5.8 TB/s.
+// half with masks: 20 us, 66 MB at 3.3 TB/s (rounds of CTAs of unlike work, each of which waits for its mask, then its values, then its
+// biases; biases asked for before the values took registers and were no faster); 256 fp32 rows of 151936: 75 us, 436 MB at 5.8 TB/s.
 #include "common.cuh"
 
 namespace edl {
 namespace {
 
-constexpr int RULE_THREADS = 256;
+constexpr int RULE_THREADS = 128;      // 256: 64 x 128256 bf16 21.1 us (20.3), 256 x 151936 fp32 76.3 us (75)
 
 struct RuleArgs {
   const void* logits;
@@ -48,7 +49,7 @@ __device__ __forceinline__ float to_float(T v) {
 }
 
 // WIDE: a thread's eight values are neighbours that start on 16 bytes, in rows of any length (`shift` values of a row's first group belong
-// to the row before it); else they lie 256 apart, so that rows of any alignment are read in whole lines.
+// to the row before it); else they lie a CTA's threads apart, so that rows of any alignment are read in whole lines.
 template <typename T, typename TO, bool WIDE, int GROUPS>
 __global__ void __launch_bounds__(RULE_THREADS) rules_kernel(const RuleArgs a) {
   constexpr int SLICE = RULE_THREADS * GROUPS * 8;
@@ -244,9 +245,9 @@ EDL_HOST_API int edl_adjust_logits(const void* logits, int in_f32, long long ld,
   auto odd = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; };
   // rows of both sides start at the same place within a group of eight
   const bool wide = ld % 8 == ldo % 8 && !odd(logits) && !odd(out);
-  // two groups per thread while that leaves four CTAs per SM, else one (and one where values lie apart, which takes more registers):
-  // 256 x 151936 fp32 79 us with two, 85 with one; 1 x 32000 bf16 2.5 us with two, 2.2 with one
-  const int groups = wide && (long long)R * ((V + 4095) / 4096) >= 4LL * sm_count() ? 2 : 1, slice = RULE_THREADS * groups * 8;
+  // two groups per thread while that leaves eight CTAs per SM, else one (and one where values lie apart, which takes more registers):
+  // 256 x 151936 fp32 79 us with two, 85 with one; 1 x 32000 bf16 2.5 us with two, 2.2 with one (both in CTAs of 256)
+  const int groups = wide && (long long)R * ((V + 2047) / 2048) >= 8LL * sm_count() ? 2 : 1, slice = RULE_THREADS * groups * 8;
   RuleArgs a{logits, out, ld, ldo, V, (int)(((long long)V + (wide ? 7 : 0) + slice - 1) / slice), counts, ld_counts, count_rows, slots, presence, frequency,
              repetition, bias_ptr, bias_ids, bias_values, bias_n, (const uint32_t*)bits, ld_bits, bits ? mask_rows : nullptr, masks, status};
   const long long ctas = (long long)R * a.slices;
