@@ -385,3 +385,85 @@ def test_frozen_rows_of_a_wide_input():
         adapters.lora_add(c["y"], c["x"], a, b, None, c["scale"]).backward(c["dy"])
         check(a.grad, val["da"], mag["da"], 300 + N, "da")
         check(b.grad, val["db"], mag["db"], 300 + K, "db")
+
+
+def test_many_rows_captured_and_replayed_with_other_indexes():
+    from easydel_b200.ops import adapters
+
+    c = make(1500, 128, (96, 32), 16, 12, BF, "cuda", "mixed")
+    out = torch.empty_like(c["y"])
+    call = lambda: adapters.lora_add(c["y"], c["x"], c["a"], c["b"], c["index"], c["scale"], parts=c["parts"], out=out)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    rows = torch.arange(1500, device="cuda")
+    for index in (rows * 0 + 11, rows * 12 // 1500, rows % 12 - 1, rows * 0 - 1, torch.where(rows < 256, rows % 12, 3)):
+        c["index"].copy_(index)
+        graph.replay()
+        want, mag = exact(c)
+        check(out, want, mag, 128)
+
+
+def test_many_rows_on_two_streams_and_in_two_threads():
+    import threading
+
+    from easydel_b200.ops import adapters
+
+    cs = [make(900 + 100 * i, 256, (128,), 16, 6, BF, "cuda", ("mixed", "runs")[i], seed=i) for i in range(2)]
+    torch.cuda.synchronize()
+    outs, grads, errors = [[], []], [[], []], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    leaf = {k: cs[i][k].detach().requires_grad_() for k in ("x", "a", "b")}
+                    o = adapters.lora_add(cs[i]["y"], leaf["x"], leaf["a"], leaf["b"], cs[i]["index"], cs[i]["scale"])
+                    grads[i].append(torch.autograd.grad(o, list(leaf.values()), cs[i]["dy"]))
+                    outs[i].append(o.detach())
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # shown by the assertion below
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for c, o, g in zip(cs, outs, grads):
+        val, mag = exact(c, grads=True)
+        for t, (dx, da, db) in zip(o, g):
+            assert torch.equal(t, o[0]) and torch.equal(dx, g[0][0]) and torch.equal(da, g[0][1]) and torch.equal(db, g[0][2])
+        check(o[0], val["out"], mag["out"], 256)
+        check(g[0][0], val["dx"], mag["dx"], 128)
+        check(g[0][1], val["da"], mag["da"], 1100)
+        check(g[0][2], val["db"], mag["db"], 1300)
+
+
+@pytest.mark.parametrize("K,N", [(14336, 64), (64, 14336)])
+def test_offsets_beyond_32_bits(K, N):
+    from easydel_b200.ops import adapters
+
+    T, last = 160000, 300      # 2.3e9 elements; the last rows have an adapter of their own
+    g = torch.Generator(device="cuda").manual_seed(0)
+    rn = lambda *s: torch.randn(s, generator=g, device="cuda", dtype=BF)  # noqa: E731
+    x, y, dy = rn(T, K), rn(T, N), rn(T, N)
+    a, b = rn(2, 8, K) * K ** -0.5, rn(2, N, 8) * 8 ** -0.5
+    index = torch.zeros(T, dtype=torch.int32, device="cuda")
+    index[-last:] = 1
+    leaf = [t.requires_grad_() for t in (x, a, b)]
+    out = adapters.lora_add(y, *leaf, index, 0.5)
+    dx, da, db = torch.autograd.grad(out, leaf, dy)
+    c = dict(x=x.detach()[-last:], y=y[-last:], a=a.detach()[1:], b=b.detach()[1:], index=None, scale=0.5, parts=(N,), dy=dy[-last:])
+    val, mag = exact(c, grads=True)
+    check(out.detach()[-last:], val["out"], mag["out"], K, "out")
+    check(dx[-last:], val["dx"], mag["dx"], N, "dx")
+    check(da[1:], val["da"], mag["da"], last + N, "da")
+    check(db[1:], val["db"], mag["db"], last + K, "db")
+    c = dict(c, x=x.detach()[:last], y=y[:last], a=a.detach()[:1], b=b.detach()[:1], dy=dy[:last])
+    val, mag = exact(c, grads=True)
+    check(out.detach()[:last], val["out"], mag["out"], K, "out")
+    check(dx[:last], val["dx"], mag["dx"], N, "dx")
