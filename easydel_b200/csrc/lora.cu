@@ -1804,7 +1804,8 @@ EDL_HOST_API int edl_lora_apply(const edl_lora_shape* shape, const void* x, cons
   }
 
   const int ranks = backward ? r : parts * r;      // that one pass over x can take
-  const int rt = !wide || x_f32 || ranks <= 16 ? 1 : ranks <= 32 ? 2 : 4;
+  // (fp32 takes 32 at a time at most: 3000 rows, 2816 to 1024, rank 64 127 us, 147 with 16 at a time; 64 of three parts do not fit registers)
+  const int rt = !wide || ranks <= 16 ? 1 : ranks <= 32 || x_f32 ? 2 : 4;
   // clusters of eight while they all fit the GPU twice, then smaller ones
   int cluster = 8;
   g.groups = g.mixed ? 2 * sms / cluster : groups_of(16);
@@ -1825,6 +1826,7 @@ EDL_HOST_API int edl_lora_apply(const edl_lora_shape* shape, const void* x, cons
 #define EDL_LORA_F32(BW)                               \
   {                                                    \
     if (!wide) EDL_LORA(float, float, 1, BW, false);   \
+    if (rt == 2) EDL_LORA(float, float, 2, BW, true);  \
     EDL_LORA(float, float, 1, BW, true);               \
   }
   if (x_f32) {
