@@ -138,9 +138,11 @@ def stream_ptr() -> int:
 
 def call_on(device: torch.device, name: str, *args) -> None:
     """:func:`call` on ``device``'s current stream, which is the launcher's last argument, whichever device is the current one."""
-    if _device_index is not None and device.index == _device_index():
-        call(name, *args, stream_ptr())
-        return
+    if _device_index is not None and _raw_stream is not None:
+        current = _device_index()
+        if device.index == current:
+            call(name, *args, _raw_stream(current))
+            return
     with torch.cuda.device(device):
         call(name, *args, stream_ptr())
 
@@ -151,7 +153,7 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def status_word(device: torch.device | int | None = None) -> torch.Tensor:
     """Per-device int32 word that kernels set when a bounded wait runs out."""
-    idx = torch.cuda.current_device() if device is None else torch.device(device).index or 0
+    idx = torch.cuda.current_device() if device is None else (device if isinstance(device, torch.device) else torch.device(device)).index or 0
     t = _status.get(idx)
     if t is None:
         t = torch.zeros(1, dtype=torch.int32, device=f"cuda:{idx}")

@@ -272,15 +272,15 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
         if b.shape[0] > MAX_TRAINED:
             raise ValueError(f"{b.shape[0]} adapters; gradients take at most {MAX_TRAINED}")
         return _LoraAddFn.apply(y, x, a, b, index, scale if isinstance(scale, torch.Tensor) else float(scale), plan)
+    if plan.plain:
+        res = torch.empty_like(y, memory_format=torch.contiguous_format) if out is None else out
+        _apply(plan, x, y, res, a, b, index, scale if isinstance(scale, torch.Tensor) else float(scale), None)
+        return res
     if not _lib.use_kernels(x):
         o = lora_add_reference(y, x, a, b, index, scale, parts=plan.parts)
         return o if out is None else out.copy_(o)
     if not isinstance(scale, torch.Tensor):
         scale = float(scale)
-    if plan.plain:
-        res = torch.empty_like(y, memory_format=torch.contiguous_format) if out is None else out
-        _apply(plan, x, y, res, a, b, index, scale, None)
-        return res
     if out is not None and not _matrix(out):      # no rows with neighbouring elements to write to
         return out.copy_(lora_add(y, x, a, b, index, scale, parts=plan.parts))
     res = torch.empty_like(y, memory_format=torch.contiguous_format) if out is None else out
