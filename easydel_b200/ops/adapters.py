@@ -4,7 +4,7 @@ Every row of a batch may bring an adapter of its own. The shared projection runs
 
     ``out[t, c] = y[t, c] + scale[i] * (x[t] @ a[i, p].T) @ b[i, c]``,  ``i = index[t]``, ``p`` the part of the output that ``c`` is in
 
-in one launch, whatever the rows' order: which rows go together is found on the device, so a captured graph follows the indexes of
+in one launch (two or three for more than a few hundred rows), whatever the rows' order: which rows go together is found on the device, so a captured graph follows the indexes of
 each replay. Packed projections (queries / keys / values, gate / up) have one adapter per part, stored together. Differentiable in
 ``y``, ``x``, ``a`` and ``b``. CPU tensors run the plain form.
 """
@@ -259,7 +259,8 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     for none (None: one adapter for all rows); ``scale``: a number, or float32 ``[n]``; ``parts``: widths of the P parts of a
     packed output, whose ranks follow one another in ``a``. Adapters of a smaller rank are padded with zeros. ``out``: where to write
     (``y`` itself for in place, else apart from all inputs; inference only; its rows do not overlap). An index of ``n`` or more counts as none and sets the status word that
-    ``_lib.check_status`` reads.
+    ``_lib.check_status`` reads. A row with infinities gives values that are not finite in that row alone; there are no second
+    derivatives.
     """
     plan = _plan_of(y, x, a, b, index, scale, None if parts is None else tuple(parts), out)
     if torch.is_grad_enabled() and (x.requires_grad or a.requires_grad or b.requires_grad or y.requires_grad):
