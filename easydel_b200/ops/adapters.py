@@ -236,7 +236,7 @@ def _plan_of(y, x, a, b, index, scale, parts, out) -> _Plan:
     key = (x.shape, x.stride(), x.dtype, x.device, y.shape, y.stride(), y.dtype, y.device, a.shape, a.stride(), a.dtype, a.device, b.shape, b.stride(),
            b.dtype, b.device, parts, index is None or (index.shape, index.dtype, index.device, index.is_contiguous()),
            (scale.shape, scale.dtype, scale.device, scale.is_contiguous(), scale.requires_grad) if tensor else None,
-           out is None or out is y or (out.shape, out.stride(), out.dtype, out.device))
+           0 if out is None else 1 if out is y else (out.shape, out.stride(), out.dtype, out.device))      # new rows lie side by side, y's need not
     plan = _plans.get(key)
     if plan is None:
         parts = _check(y, x, a, b, index, scale, parts, out)
