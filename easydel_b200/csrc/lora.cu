@@ -1060,14 +1060,14 @@ __global__ void __launch_bounds__(UP_THREADS, 2) lora_up_kernel(const __grid_con
                                                                const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_u,
                                                                const __grid_constant__ CUtensorMap map_out) {
   __shared__ RowUnits units;
-  __shared__ uint64_t s_bars[2 * UP_STAGES + 6];
+  __shared__ uint64_t s_bars[2 * UP_STAGES + 7];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   extern __shared__ uint8_t raw[];
   uint8_t* dyn = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   const uint32_t stages = smem_u32(dyn), su = stages + UP_STAGES * UP_STAGE;
   const uint32_t full = smem_u32(s_bars), empty = full + 8 * UP_STAGES, dfull = empty + 8 * UP_STAGES, dempty = dfull + 16, ufull = dempty + 16,
-                 ufree = ufull + 8;
+                 ufree = ufull + 8, ugo = ufree + 8;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const long long row0 = (long long)(blockIdx.x / a.splits) * LORA_ROWS;
   if (tid == 0) {
@@ -1081,6 +1081,7 @@ __global__ void __launch_bounds__(UP_THREADS, 2) lora_up_kernel(const __grid_con
     }
     mbar_init(ufull, 1);
     mbar_init(ufree, 1);
+    mbar_init(ugo, 1);
     s_abort = 0;
     fence_mbar_init();
   }
@@ -1102,7 +1103,9 @@ __global__ void __launch_bounds__(UP_THREADS, 2) lora_up_kernel(const __grid_con
   auto wait = [&](uint32_t bar, int use, int code) { mbar_wait(bar, use & 1, abort_flag, a.status, code); };
 
   // Every role walks the same runs: a unit's tiles within one part, whose u they share. Rows without an adapter are copied by the eight
-  // warps alone.
+  // warps alone. A wait by parity tells a phase from its neighbours alone, so whoever waits on a barrier waits for each of its phases: the lane
+  // that loads is the only one that waits until the last run's products have read their u (`ufree`, a phase per run; the next one's products need
+  // weights that it has not asked for yet), and passes that on to the eight warps where they bring u themselves (`ugo`, a phase per such run).
   struct Run {
     int ad, m, p, n0, count, run, tile;      // first column, tiles; number of this run and of its first tile
     const short* order;
@@ -1134,10 +1137,12 @@ __global__ void __launch_bounds__(UP_THREADS, 2) lora_up_kernel(const __grid_con
     if (elect_one()) {
       walk([&](const Run& r) {
         if (r.ad < 0) return;
+        if (r.run) wait(ufree, r.run - 1, EDL_TIMEOUT_PRODUCER);
         if (line(r)) {
-          if (r.run) wait(ufree, r.run - 1, EDL_TIMEOUT_PRODUCER);
           mbar_expect_tx(ufull, 2 * UP_U);
           for (int s = 0; s < 2; ++s) tma_load_3d(su + s * UP_U, &map_u, ufull, r.p * r16, (int)row0 + r.order[0], s);
+        } else {
+          mbar_arrive(ugo);
         }
         for (int t = 0; t < r.count; ++t) {
           const int tile = r.tile + t, at = tile % UP_STAGES, use = tile / UP_STAGES;
@@ -1179,9 +1184,10 @@ __global__ void __launch_bounds__(UP_THREADS, 2) lora_up_kernel(const __grid_con
   } else {
     const int q = w & 3, half = (w - 2) >> 2, i = 32 * q + lane;      // this lane's row of a unit; its four warps take every other tile
     const bool wide = a.ldo % 16 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
+    int gathered = 0;
     walk([&](const Run& r) {
       if (r.ad >= 0 && !line(r)) {      // u of rows that are no neighbours
-        if (r.run) wait(ufree, r.run - 1, EDL_TIMEOUT_EPILOGUE);
+        wait(ugo, gathered++, EDL_TIMEOUT_EPILOGUE);
         for (int e = tid - 64; e < 2 * UP_ROWS * (r16 / 8); e += 256) {
           const int j = e % (r16 / 8), tok = e / (r16 / 8) % UP_ROWS, s = e / (r16 / 8 * UP_ROWS);
           uint4 v = make_uint4(0, 0, 0, 0);

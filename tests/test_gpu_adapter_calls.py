@@ -39,3 +39,76 @@ def test_new_results_and_results_in_place_of_one_strided_y(order, dtype, T, monk
             got = _call(dict(c, x=c["x"].detach().requires_grad_()))
             check(got.detach(), want, mag, 64, how)
         assert (wide[:, 32:] == 7.0).all(), how
+
+
+# blocks of 256 rows: rows of an adapter side by side, and rows of others that lie apart between them, one after the other in every order
+def _layouts(T):
+    t, row = torch.arange(T), torch.arange(T) % 256
+    pair = torch.where(t % 2 == 0, 1, -1)
+    return {
+        "line, apart, line": torch.where(row < 60, 0, torch.where(row < 160, pair, 2)),
+        "apart, apart, line": torch.where(row < 100, t % 2, 2),
+        "apart, line, apart, line": torch.where(row < 40, torch.where(t % 2 == 0, 0, -1), torch.where(row < 90, 1, torch.where(row < 140, 2, torch.where(row == 200, 0, -1)))),
+        "line, apart, apart": torch.where(row < 70, 2, t % 2),
+        "line, line, apart, line in turns of blocks": torch.where(t // 256 % 2 == 0, torch.where(row < 128, 0, torch.where(row < 250, t % 2 + 1, 0)), row // 100),
+    }
+
+
+def _close(got, want, mag, length, what):
+    """`check` with operands that stay where they are."""
+    from adapter_cases import bound
+
+    off, top = (got.double() - want).abs(), bound(got.dtype, want, mag, length)
+    bad = ~(off <= top)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} values off, first row {int(bad.any(1).nonzero()[0])}"
+
+
+def _exact(x, y, a, b, index, scale, parts, dy=None):
+    """out and its magnitudes, or dx and its: 64 bits, on the device."""
+    r, n = b.shape[2], b.shape[0]
+    x, a, b = x.double(), a.double(), b.double()
+    val = y.double().clone() if dy is None else torch.zeros_like(x)
+    mag = val.abs()
+    for i in range(n):
+        at, c0 = (index == i).nonzero()[:, 0], 0
+        for p, w in enumerate(parts):
+            A, B = a[i, p * r:(p + 1) * r], b[i, c0:c0 + w]
+            for m, f in ((val, lambda t: t), (mag, torch.abs)):
+                s = f(scale[i].double())
+                if dy is None:
+                    m[at, c0:c0 + w] += s * (f(x[at]) @ f(A).t()) @ f(B).t()
+                else:
+                    m[at] += s * (f(dy[at, c0:c0 + w].double()) @ f(B)) @ f(A)
+            c0 += w
+    return val, mag
+
+
+@pytest.mark.parametrize("rank", [8, 16, 64])
+@pytest.mark.parametrize("T,parts", [(600, (64,)), (1500, (128,)), (1500, (1344,)), (3900, (896, 128, 128)), (2100, (14336, 14336))])
+def test_rows_side_by_side_and_apart_in_one_block(T, parts, rank):
+    for name, index in _layouts(T).items():
+        c = make(T, 64, parts, rank, 3, BF, "cuda", "bare", seed=T + rank)
+        c["index"] = index.to(torch.int32).cuda()
+        want, mag = _exact(c["x"], c["y"], c["a"], c["b"], c["index"], c["scale"], parts)
+        got = _call(c)
+        _close(got, want, mag, 64, name)
+        for _ in range(4):
+            assert torch.equal(got, _call(c)), name
+        y = c["y"].clone()
+        assert torch.equal(_call(dict(c, y=y), out=y), got), name
+
+
+@pytest.mark.parametrize("rank", [8, 16, 64])
+@pytest.mark.parametrize("T,K", [(600, 64), (1500, 128), (1500, 1344), (3900, 1152), (2100, 28672)])
+def test_gradients_of_rows_side_by_side_and_apart_in_one_block(T, K, rank):
+    for name, index in _layouts(T).items():
+        c = make(T, K, (64,), rank, 3, BF, "cuda", "bare", seed=T + rank)
+        c["index"] = index.to(torch.int32).cuda()
+        want, mag = _exact(c["x"], c["y"], c["a"], c["b"], c["index"], c["scale"], c["parts"], c["dy"])
+        first = None
+        for _ in range(4):
+            x = c["x"].detach().requires_grad_()
+            _call(dict(c, x=x)).backward(c["dy"])
+            first = x.grad if first is None else first
+            assert torch.equal(first, x.grad), name
+        _close(first, want, mag, 64, name)
