@@ -16,6 +16,8 @@
 // it keeps 16 (24) bits; fp32 operands enter as three bf16 parts each.
 #include <cooperative_groups.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace edl {
@@ -1269,36 +1271,31 @@ __global__ void __launch_bounds__(UP_THREADS, 2) lora_up_kernel(const __grid_con
   if (w == 1) tmem_dealloc(tmem, 2 * UP_TILE);
 }
 
-// Raises a kernel's limit of dynamic shared memory on the current device, once.
-int shared_memory(const void* kernel, int bytes, const char* what) {
-  struct Limit {
+// Raises a kernel's limit of dynamic shared memory on the current device, once per thread. The limit belongs to all threads and a call may lower it, so
+// it is always the most that the device allows beside the kernel's static part, whatever this launch takes.
+int shared_memory(const void* kernel, const char* what) {
+  struct Known {
     const void* kernel;
-    int dev, bytes;
+    int dev;
   };
-  static thread_local Limit known[64] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  Limit* free_slot = nullptr;
-  for (Limit& l : known) {
-    if (l.kernel == kernel && l.dev == dev) {
-      if (l.bytes >= bytes) return 0;
-      free_slot = &l;
-      break;
-    }
-    if (!l.kernel) {
-      free_slot = &l;
-      break;
-    }
-  }
-  if (check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), what)) return -1;
-  if (free_slot) *free_slot = Limit{kernel, dev, bytes};
+  static thread_local Known known[64] = {};
+  int dev = 0, most = 0;
+  if (check_cuda(cudaGetDevice(&dev), what)) return -1;
+  Known* slot = known;
+  for (; slot < known + 64 && slot->kernel; ++slot)
+    if (slot->kernel == kernel && slot->dev == dev) return 0;
+  cudaFuncAttributes attr{};
+  if (check_cuda(cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev), what) || check_cuda(cudaFuncGetAttributes(&attr, kernel), what) ||
+      check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most - (int)attr.sharedSizeBytes), what))
+    return -1;
+  if (slot < known + 64) *slot = Known{kernel, dev};
   return 0;
 }
 
 // `early`: the kernel may start while the one before it ends (it waits by itself, see `wait_for_last`).
 template <typename... E, typename... A>
 int launch_sized(void (*k)(E...), dim3 grid, int threads, int cluster, bool early, int smem, cudaStream_t stream, const char* what, const A&... args) {
-  if (smem > 40 * 1024 && shared_memory(reinterpret_cast<const void*>(k), smem, what)) return -1;      // 48 KB with the static part
+  if (smem > 40 * 1024 && shared_memory(reinterpret_cast<const void*>(k), what)) return -1;      // 48 KB with the static part
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
@@ -1596,7 +1593,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_grad_kernel(const __grid
 // Clusters of `size` CTAs of the gradient kernel that the current device runs at once (asked for once per size): the runtime counts one CTA to an
 // SM, two fit.
 int grad_clusters(int size, int smem) {
-  static int known[64][9] = {};
+  static std::atomic<int> known[64][9] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) dev = 0;
@@ -1613,7 +1610,7 @@ int grad_clusters(int size, int smem) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int clusters = 0;
-    if (shared_memory(reinterpret_cast<const void*>(lora_grad_kernel), smem, "lora gradient shared memory") ||
+    if (shared_memory(reinterpret_cast<const void*>(lora_grad_kernel), "lora gradient shared memory") ||
         cudaOccupancyMaxActiveClusters(&clusters, lora_grad_kernel, &cfg) != cudaSuccess) {
       cudaGetLastError();
       clusters = sm_count() / size * 7 / 8;

@@ -112,3 +112,34 @@ def test_gradients_of_rows_side_by_side_and_apart_in_one_block(T, K, rank):
             first = x.grad if first is None else first
             assert torch.equal(first, x.grad), name
         _close(first, want, mag, 64, name)
+
+
+@pytest.mark.parametrize("T", [40, 600])
+def test_threads_in_turn_with_ranks_that_take_unlike_shared_memory(T):
+    import threading
+
+    # the limit of a kernel's shared memory belongs to the process: a thread with a low rank must not lower it under one with a high rank
+    cs = [make(T, 64, (64,) * 3, r, 3, BF if T > 256 else F32, "cuda", "runs", seed=r) for r in (64, 16, 64, 8)]
+    turn, errors, outs = threading.Barrier(4), [], [[] for _ in cs]
+
+    def work(i):
+        for at in range(12):
+            turn.wait()
+            if at % 4 == i or at >= 8:
+                try:
+                    outs[i].append(_call(cs[i]))
+                except RuntimeError as e:  # shown by the assertion below
+                    errors.append(e)
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for c, o in zip(cs, outs):
+        want, mag = exact(c)
+        for got in o:
+            check(got, want, mag, 64)
