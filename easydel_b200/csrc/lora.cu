@@ -12,8 +12,11 @@
 // Which rows go together is found by each CTA from the indexes of its rows, so a captured graph follows the indexes of the step and nothing
 // is sorted, counted or copied by the host.
 //
-// Precision: sums are fp32. u enters the second product (and the gradients) as two bf16 parts, three where the result is fp32, so
-// it keeps 16 (24) bits; fp32 operands enter as three bf16 parts each.
+// Precision: sums are fp32. u enters the second product (and the gradients) as two bf16 parts, off by 2^-16 of it at most, which a bf16 result does
+// not show but in single roundings; three where the result is fp32, which hold all of it. fp32 operands enter as three bf16 parts each. The tensor
+// cores cut their sums off, so fp32 results take the products of 16 columns, ranks or rows at a time from them and add those up outside, where
+// sums are rounded: 4096 to 4096 columns, rank 16, off by 1.3e-7 of the result (2.0e-6 in the accumulators; fp32 library products 1.1e-6). Only fp32
+// results beside many bf16 rows do not (14336 columns, rank 64: 2e-6; the second product would take 7 % longer).
 #include <cooperative_groups.h>
 
 #include <atomic>
@@ -35,32 +38,30 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_bf16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t turn(uint32_t v) {      // 8 x 8 transpose over the warp
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
   return d;
 }
 
-// v as the sum of `S` bf16 values (upper halves), each cut off towards zero, so that nothing overflows and the remainder is
-// exact. Values that are not finite keep to the first part.
+// Two values as sums of `S` bf16 values each, in packed pairs, rounded to nearest: a remainder is exact and at most 2^-8 of what it remains of.
+// Three parts hold an fp32 value's 24 bits, two are off by 2^-16 of it at most. (Parts cut off towards zero are off by twice that, and all remainders
+// then have the value's sign: products of the lower parts, which `mma_parts` leaves out, add up instead of cancelling.) What would round to
+// infinity stays finite in the first part; an infinity has infinite or undefined later parts. Two at a time take one conversion per part:
+// 4096 rows of fp32, 4096 columns to 4096, rank 16: 79 us, 108 value by value.
 template <int S>
-__device__ __forceinline__ void split(float v, uint32_t (&p)[S]) {
-  const uint32_t u = __float_as_uint(v);
-  if ((u & 0x7f800000u) == 0x7f800000u) {
-    p[0] = (u & 0x7fffffu) ? 0x7fc0u : u >> 16;
-#pragma unroll
-    for (int s = 1; s < S; ++s) p[s] = 0;
-    return;
-  }
+__device__ __forceinline__ void split(float lo, float hi, uint32_t (&p)[S]) {
 #pragma unroll
   for (int s = 0; s < S; ++s) {
-    if (s + 1 < S) {
-      const uint32_t h = __float_as_uint(v) & 0xffff0000u;
-      p[s] = h >> 16;
-      v -= __uint_as_float(h);
-    } else {
-      p[s] = __bfloat16_as_ushort(__float2bfloat16_rn(v));
-    }
+    if (s == 0) asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(p[s]) : "f"(hi), "f"(lo));
+    else p[s] = pack_bf16x2(lo, hi);
+    lo -= __uint_as_float(p[s] << 16);
+    hi -= __uint_as_float(p[s] & 0xffff0000u);
   }
 }
 
@@ -103,11 +104,10 @@ __device__ __forceinline__ void load_pairs(const T* p, int valid, uint32_t (&q)[
     }
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
-      uint32_t a[3], b[3];
-      split<3>(f[2 * i], a);
-      split<3>(f[2 * i + 1], b);
+      uint32_t v[3];
+      split<3>(f[2 * i], f[2 * i + 1], v);
 #pragma unroll
-      for (int s = 0; s < 3; ++s) q[s][i] = a[s] | (b[s] << 16);
+      for (int s = 0; s < 3; ++s) q[s][i] = v[s];
     }
   }
 }
@@ -154,15 +154,28 @@ __device__ __forceinline__ void store_row(TY* dst, int ok, const float (&f)[8]) 
   }
 }
 
-// d += a b over the parts of both operands whose product is above the rounding of fp32 (part i has the bits from 8 i on).
-template <int PA, int PB>
+// d += a b over the parts of both operands whose product is above the rounding of fp32: the second part is at most 2^-8 of its value, the third 2^-17,
+// so what is left out of nine products is at most 2^-24 of theirs, of either sign.
+// Where `F32` results need sums that are rounded, the products are added up by themselves first.
+template <bool F32, int PA, int PB>
 __device__ __forceinline__ void mma_parts(float (&d)[4], const uint32_t (&a)[PA][4], const uint32_t (&b)[PB][2]) {
   constexpr int TOP = PA > PB ? PA : PB;
+  float few[4];
+  bool first = F32;
 #pragma unroll
   for (int o = TOP - 1; o >= 0; --o)      // small products first
 #pragma unroll
-    for (int i = 0; i < PA; ++i)
-      if (o - i >= 0 && o - i < PB) mma_bf16(d, a[i][0], a[i][1], a[i][2], a[i][3], b[o - i][0], b[o - i][1]);
+    for (int i = 0; i < PA; ++i) {
+      if (o - i < 0 || o - i >= PB) continue;
+      if (!F32) mma_bf16(d, a[i][0], a[i][1], a[i][2], a[i][3], b[o - i][0], b[o - i][1]);
+      else if (first) mma_bf16_first(few, a[i][0], a[i][1], a[i][2], a[i][3], b[o - i][0], b[o - i][1]);
+      else mma_bf16(few, a[i][0], a[i][1], a[i][2], a[i][3], b[o - i][0], b[o - i][1]);
+      first = false;
+    }
+  if constexpr (F32) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) d[e] += few[e];
+  }
 }
 
 // A kernel that was launched to start early waits here until the one before it, and with that all before, has ended and its results are there;
@@ -391,7 +404,8 @@ __device__ __forceinline__ void find_units(RowUnits& u, void* scratch, const Lor
 // columns in three parts: 16 us; 256 rows of 64 adapters, 14336 to 4096, rank 32: 33 us, 2.5 TB/s of 83 MB (all cold). What bounds the last: an SM
 // has two CTAs or one (252 of 296 places), a warp's loads of a step follow the last step's products, and the expansion reads its weights
 // after the cluster has met. Weights copied ahead into rings in shared memory, or asked for before the cluster met, gained nothing.
-// 4096 rows of fp32, 4096 to 4096: 108 us, bound by the nine products of parts.
+// 4096 rows of fp32, 4096 to 4096: 79 us against 31 of traffic: the weights are read and cut into their parts again for every 16 rows, and every
+// element of x is cut in registers, between loads that wait for the products of the step before.
 template <typename T, typename TY, int RT, bool DOWN_T, bool WIDE>
 __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const __grid_constant__ LoraArgs a) {
   constexpr int NT = 2, CHUNK = 8 * NT;
@@ -512,8 +526,8 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const __grid_cons
               }
 #pragma unroll
               for (int i = 0; i < RT; ++i) {
-                mma_parts<P, P>(acc[i][j], wa[i][0], b[0]);
-                mma_parts<P, P>(acc[i][j], wa[i][1], b[1]);
+                mma_parts<S == 3, P, P>(acc[i][j], wa[i][0], b[0]);
+                mma_parts<S == 3, P, P>(acc[i][j], wa[i][1], b[1]);
               }
             }
           }
@@ -551,7 +565,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const __grid_cons
         float v = 0.f;
         if (tok < m && rank < a.up_seg[p].ru) v = cluster_sum(smem_u32(part + tok * pstride + a.up_seg[p].u0 + rank), C) * s;
         uint32_t parts[S];
-        split<S>(v, parts);
+        split<S>(v, 0.f, parts);
 #pragma unroll
         for (int k = 0; k < S; ++k) {
           su[(k * CHUNK + tok) * ustride + col] = (unsigned short)parts[k];
@@ -597,7 +611,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const __grid_cons
                 ua[s][2 + h] = v.y;
               }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) mma_parts<S, P>(acc[d][j], ua, wb[d][j]);
+            for (int j = 0; j < 4; ++j) mma_parts<S == 3, S, P>(acc[d][j], ua, wb[d][j]);
           }
         }
       }
@@ -894,22 +908,23 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_down_kernel(const __grid
           cluster_sum4(smem_u32(part + tok * pstride + (of * each - pass0) * np + in), C, v);
         }
         unsigned short* dst = a.u + (row0 + order[tok]) * a.ucols + col;
-        uint32_t q[4][3];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[i] = pad ? 0.f : v[i] * s;
+        for (int i = 0; i < 4; ++i) v[i] = pad ? 0.f : v[i] * s;
+        uint32_t q[2][3];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
           if (parts == 2) {
             uint32_t two[2];
-            split<2>(v[i], two);
-            q[i][0] = two[0];
-            q[i][1] = two[1];
+            split<2>(v[2 * h], v[2 * h + 1], two);
+            q[h][0] = two[0];
+            q[h][1] = two[1];
           } else {
-            split<3>(v[i], q[i]);
+            split<3>(v[2 * h], v[2 * h + 1], q[h]);
           }
         }
 #pragma unroll
         for (int k = 0; k < 3; ++k)
-          if (k < parts) *reinterpret_cast<uint2*>(dst + (long long)k * a.T * a.ucols) = make_uint2(q[0][k] | q[1][k] << 16, q[2][k] | q[3][k] << 16);
+          if (k < parts) *reinterpret_cast<uint2*>(dst + (long long)k * a.T * a.ucols) = make_uint2(q[0][k], q[1][k]);
       }
       asm volatile("barrier.cluster.arrive.release;" ::: "memory");
       pending = true;
@@ -1013,7 +1028,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_up_any_kernel(const __gr
             ua[s][2] = v0.y; ua[s][3] = v1.y;
           }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) mma_parts<S, 1>(acc[j], ua, wb[i][j]);
+          for (int j = 0; j < 4; ++j) mma_parts<false, S, 1>(acc[j], ua, wb[i][j]);
         }
       }
     }
@@ -1476,16 +1491,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 1) lora_grad_any_kernel(const __
             pa[s][h + 2 * k] = turn(v);
           }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if constexpr (S == 3) {      // the tensor cores cut sums off: 32-bit results take a few products at a time and round the sum
-          float few[4] = {0.f, 0.f, 0.f, 0.f};
-          mma_parts<S, P>(few, pa, zb[j]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[j][e] += few[e];
-        } else {
-          mma_parts<S, P>(acc[j], pa, zb[j]);
-        }
-      }
+      for (int j = 0; j < 8; ++j) mma_parts<S == 3, S, P>(acc[j], pa, zb[j]);
     }
     if (a.index) __syncthreads();
   }
