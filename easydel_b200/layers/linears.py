@@ -27,7 +27,7 @@ import torch
 from torch import nn
 
 from ..ops import _lib, functional as F
-from ..ops.adapters import MAX_RANK, lora_add
+from ..ops.adapters import lora_add, pays
 
 
 class ParallelLinear(nn.Module):
@@ -170,7 +170,7 @@ class eLoRA(nn.Module):
 
     def forward(self, x: torch.Tensor, w: torch.Tensor | None = None) -> torch.Tensor:
         y = self.base(x, w)
-        if not _lib.use_kernels(x) or not x.dtype == y.dtype == self.lora_a.dtype or self.rank > MAX_RANK:
+        if not _lib.use_kernels(x) or not x.dtype == y.dtype == self.lora_a.dtype or not pays(x, self.lora_b):
             z = torch.nn.functional.linear(torch.nn.functional.linear(self.dropout(x), self.lora_a), self.lora_b)
             return y + z * self.scaling
         return lora_add(y, self.dropout(x), self.lora_a[None], self.lora_b[None], None, self.scaling)

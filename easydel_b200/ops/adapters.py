@@ -108,6 +108,19 @@ def _few_rows(T: int, cols: int, index: bool) -> bool:
     return T <= 256 or T <= 512 and (index or cols <= 8192)
 
 
+def pays(x: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether one adapter ``b [out, r]`` for all rows of ``x`` is faster by these kernels than by two library products and a sum.
+
+    They have streaming forms for bfloat16 ranks up to 64 whose sizes 16-byte loads fit (8192 rows, 14336 columns to 4096, forward and backward: rank
+    64 225 us, 275 by products; rank 128 709, 287), and cut float32 operands into parts for every 16 ranks (8192 rows, 14336 columns to 1024: rank
+    32 1098 us, 982; to 4096: rank 16 790, 1222). Ranks or widths that those loads do not fit pay while the rows are few (512 rows, rank 14: 140
+    us, 169; 8192 rows: 444, 329), of float32 with many rows too (rank 5 514 us, 697; rank 1 500, 383; rank 30 786, 731)."""
+    rank, many, f32 = b.shape[1], x.numel() // x.shape[-1] > 512, x.dtype == torch.float32
+    if rank % 4 == 0 and x.shape[-1] % 8 == 0 and b.shape[0] % 8 == 0:
+        return rank <= (64 if not f32 else 16 if many else 32)
+    return rank <= 16 and (not many or f32 and rank >= 4)
+
+
 class _Plan:
     """What a call's sizes, strides and types decide: checked once, kept for the calls that follow with the same ones."""
 
