@@ -5,7 +5,8 @@
 
 A grammar is a callable in ``SamplingParams.guided_decoding``: ``f(prompt_token_ids, output_token_ids)`` returns the tokens allowed next (ids,
 or packed int32 words with bit ``t % 32`` of word ``t // 32`` for token t), or None where everything is. Requests with one are read back after
-every step, since the next mask needs the token. One that raises, or allows nothing, ends its own request with that error.
+every step, since the next mask needs the token. One that raises, or allows nothing that ``allowed_token_ids``, ``min_tokens`` and biases of minus
+infinity leave, ends its own request with that error. (Where those alone leave nothing, every token is forbidden and the sampler gives token 0.)
 """
 
 from __future__ import annotations
@@ -48,6 +49,7 @@ class TokenRules:
         self.allowed = None if sp.allowed_token_ids is None else pack_tokens(sp.allowed_token_ids, vocab)
         if self.allowed is not None and not self.allowed.any():
             raise ValueError("allowed_token_ids is empty")
+        self._tokens = pack_tokens(range(vocab), vocab) if self.grammar is not None else None      # the last word's other bits name none
         self.error: Exception | None = None      # of the grammar
 
     @classmethod
@@ -79,12 +81,15 @@ class TokenRules:
         if isinstance(g, torch.Tensor):
             g = g.cpu().numpy()
         if isinstance(g, np.ndarray) and g.dtype == np.int32 and g.ndim == 1 and g.size == (self.vocab + 31) // 32:
-            g = np.ascontiguousarray(g)
+            g = g & self._tokens
         else:
             g = pack_tokens((int(t) for t in g), self.vocab)
         g = g if m is None else m & g
-        if not g.any():
-            raise ValueError("the grammar allows no token")
+        ids, values = self.entries(len(output))
+        left, gone = g.view(np.uint32).copy(), ids[values == -np.inf].astype(np.int64)
+        np.bitwise_and.at(left, gone // 32, ~(np.uint32(1) << (gone % 32).astype(np.uint32)))
+        if not left.any():
+            raise ValueError("the grammar allows no token" + (" that the request's other rules leave" if g.any() else ""))
         return g
 
 
