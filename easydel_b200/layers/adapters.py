@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import contextlib
 import json
+import math
 import os
 import re
 import threading
@@ -137,15 +138,24 @@ class AdapterSet:
         if not self._free:
             raise RuntimeError(f"all {self.count} adapter slots are taken: unload one, or make more")
         tensors, config = (source, {}) if isinstance(source, tp.Mapping) else _read(source)
-        todo = [(bank, part, a, b, _scale(config, path, a.shape[0]) if scale is None else scale)
-                for path, bank, part, a, b in self._match(tensors)]       # everything is checked before anything is written
+        # everything is checked before anything is written. A bank has one factor per adapter: parts with factors of their own have them in b
+        todo: dict[int, list] = {}
+        for path, bank, part, a, b in self._match(tensors):
+            s = float(_scale(config, path, a.shape[0]) if scale is None else scale)
+            if not math.isfinite(s):
+                raise ValueError(f"{path!r}: its factor is {s}")
+            todo.setdefault(id(bank), []).append((bank, part, a, b, s))
         slot = self._free.pop()
-        for bank in self.banks.values():
-            bank.clear(slot)
-        for bank, part, a, b, s in todo:
-            if part is not None and float(s) != float(todo[0][4]):        # ranks of their own per module: the factor goes into b
-                b, s = b.float() * (s / todo[0][4]), todo[0][4]
-            bank.put(slot, part, a, b, s)
+        try:
+            for bank in self.banks.values():
+                bank.clear(slot)
+            for puts in todo.values():
+                same = all(s == puts[0][4] for *_, s in puts)
+                for bank, part, a, b, s in puts:
+                    bank.put(slot, part, a, b if same else b.float() * s, s if same else 1.0)
+        except BaseException:
+            self._free.append(slot)
+            raise
         self.slots[name] = slot
         return slot
 
