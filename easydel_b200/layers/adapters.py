@@ -170,9 +170,13 @@ class AdapterSet:
             m = re.fullmatch(r"(?:base_model\.model\.)?(.+?)\.(?:lora_(A|B)(?:\.[^.]+)?\.weight|lora_(a|b))", key)
             if m is None:
                 raise ValueError(f"{key!r} is no adapter weight")
-            pairs.setdefault(m[1], {})[(m[2] or m[3]).lower()] = t
+            pair, letter = pairs.setdefault(m[1], {}), (m[2] or m[3]).lower()
+            if letter in pair:
+                raise ValueError(f"{m[1]!r} has its weight {letter} twice")
+            pair[letter] = t
         if not pairs:
             raise ValueError("no adapter weights")
+        taken: dict[int, list[int | None]] = {}      # parts of a bank (None: all)
         for path, w in pairs.items():
             owner, _, leaf = path.rpartition(".")
             merged = next((k for k, parts in MERGED.items() if leaf in parts), None)
@@ -188,6 +192,10 @@ class AdapterSet:
                 raise ValueError(f"{path!r}: adapter weights {tuple(a.shape)} and {tuple(b.shape)} do not fit a projection of {bank.a.shape[2]} to {out}")
             if a.shape[0] > self.rank:
                 raise ValueError(f"{path!r}: rank {a.shape[0]}; there is room for {self.rank}")
+            others = taken.setdefault(id(bank), [])
+            if others and (part is None or None in others or part in others):
+                raise ValueError(f"{path!r} is adapted twice, by itself and as a part of a merged projection")
+            others.append(part)
             yield path, bank, part, a, b
 
 

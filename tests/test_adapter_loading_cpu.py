@@ -66,3 +66,14 @@ def test_factors_that_are_no_numbers_are_refused(scale):
     with pytest.raises(ValueError, match="factor"):
         aset.load("x", _pair("mlp.down_proj", 48, 32, 4), scale)
     assert aset._free == [0]
+
+
+def test_a_projection_that_is_named_twice_is_refused():
+    q, qkv = _pair("self_attn.q_proj", 32, 32, 4), _pair("self_attn.qkv_proj", 32, 64, 4)
+    aset = _set()
+    for both in ({**q, **qkv}, {**qkv, **q}, {**q, **{f"base_model.model.{k}": v for k, v in q.items()}},
+                 {**q, **{k.replace("lora_A.weight", "lora_A.default.weight"): v for k, v in q.items()}}):
+        with pytest.raises(ValueError, match="twice"):
+            aset.load("x", both)
+        assert aset._free == [0]
+    aset.load("x", qkv)
