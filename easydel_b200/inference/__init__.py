@@ -1,3 +1,3 @@
-from .sampling_params import BeamSearchParams, JitableSamplingParams, SamplingParams
+from .sampling_params import BeamSearchParams, InvalidRequest, JitableSamplingParams, SamplingParams
 
-__all__ = ["SamplingParams", "JitableSamplingParams", "BeamSearchParams"]
+__all__ = ["SamplingParams", "InvalidRequest", "JitableSamplingParams", "BeamSearchParams"]

@@ -20,7 +20,7 @@ from dataclasses import dataclass, field
 import torch
 
 from ...caching.paged import PAGE_SIZE, PagedKVCache
-from ..sampling_params import SamplingParams
+from ..sampling_params import InvalidRequest, SamplingParams
 from ..token_rules import TokenRules
 from .metrics import MetricsCollector
 from .kv_manager import KVCacheCoordinator
@@ -344,7 +344,7 @@ class eSurge:
     def _tokenize(self, prompt) -> tuple[list[int], str | None]:
         if isinstance(prompt, str):
             if self.tokenizer is None:
-                raise ValueError("string prompts need a tokenizer")
+                raise InvalidRequest("string prompts need a tokenizer")
             return list(self.tokenizer(prompt, add_special_tokens=True)["input_ids"]), prompt
         if isinstance(prompt, dict) and "prompt_token_ids" in prompt:
             return list(prompt["prompt_token_ids"]), prompt.get("prompt")
@@ -364,7 +364,7 @@ class eSurge:
                     videos: tp.Sequence[tp.Any] | None = None, adapter: str | None = None) -> str:
         """Queues a request. ``adapter``: the name of a loaded adapter to run it with."""
         if adapter is not None and adapter not in self._adapter_keys:
-            raise ValueError(f"adapter {adapter!r} is not loaded")
+            raise InvalidRequest(f"adapter {adapter!r} is not loaded")
         sp = sampling_params or SamplingParams()
         if self.sampling_params_callback is not None:
             sp = self.sampling_params_callback(sp, {"prompt": prompt, "request_id": request_id}) or sp
@@ -373,20 +373,20 @@ class eSurge:
                           stop=list(dict.fromkeys([*(sp.stop or []), *self.extra_stops])))
         ids, text = self._tokenize(prompt)
         if not ids:
-            raise ValueError("empty prompt")
+            raise InvalidRequest("empty prompt")
         mm_embeds, mm_hash, rope = [], None, None
         if images or videos:
             if self.multimodal is None:
-                raise ValueError("this model has no vision tower: images cannot be served")
+                raise InvalidRequest("this model has no vision tower: images cannot be served")
             ids, mm_embeds, mm_hash, rope = self.multimodal.prepare(ids, images, videos, with_rope=True)
             if len(ids) > self.max_model_len - self.reserve_tokens:
-                raise ValueError(f"prompt with images has {len(ids)} tokens; max_model_len is {self.max_model_len}")
+                raise InvalidRequest(f"prompt with images has {len(ids)} tokens; max_model_len is {self.max_model_len}")
         limit = self.max_model_len - self.reserve_tokens
         want = len(ids) + (sp.max_tokens or 0)
         if len(ids) > limit or want > self.max_model_len:
             if len(ids) > limit:
                 if not self.auto_truncate_prompt:
-                    raise ValueError(f"prompt has {len(ids)} tokens; max_model_len is {self.max_model_len}")
+                    raise InvalidRequest(f"prompt has {len(ids)} tokens; max_model_len is {self.max_model_len}")
                 rope = None     # a truncated prompt keeps consecutive positions
                 keep = limit
                 if self.truncate_mode == "left":
@@ -409,7 +409,7 @@ class eSurge:
         with self._work:
             if adapter is not None:
                 if adapter not in self._adapter_keys:
-                    raise ValueError(f"adapter {adapter!r} is not loaded")
+                    raise InvalidRequest(f"adapter {adapter!r} is not loaded")
                 req.adapter, req.adapter_slot = self._adapter_keys[adapter], self.adapters.slots[adapter]
             self._tracked[rid] = tr
             self.scheduler.add_request(req)

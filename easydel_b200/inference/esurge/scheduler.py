@@ -19,7 +19,7 @@ import time
 import typing as tp
 from dataclasses import dataclass, field
 
-from ..sampling_params import SamplingParams
+from ..sampling_params import InvalidRequest, SamplingParams
 from .kv_manager import KVCacheCoordinator
 from .page_pool import PagePool, hash_request_pages
 
@@ -153,7 +153,7 @@ class Scheduler:
     # ------------------------------------------------------------------ queue management
     def add_request(self, req: EngineRequest) -> None:
         if req.num_prompt_tokens >= self.config.max_model_len:
-            raise ValueError(f"prompt of {req.num_prompt_tokens} tokens does not fit max_model_len "
+            raise InvalidRequest(f"prompt of {req.num_prompt_tokens} tokens does not fit max_model_len "
                              f"{self.config.max_model_len}")
         self.requests[req.request_id] = req
         req.status = RequestStatus.WAITING

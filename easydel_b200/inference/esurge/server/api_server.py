@@ -27,6 +27,7 @@ from ...openai_api_modules import (ChatCompletionRequest, ChatCompletionResponse
                                    ModelCard, ModelList, ResponsesRequest, ResponsesResponse, ToolCall,
                                    ToolExecuteRequest, UsageInfo, sse)
 from ...reasoning import DelegatingParser, ReasoningParserManager, detect_reasoning_parser
+from ...sampling_params import InvalidRequest
 from ...stream_protocol import ResponsesStreamBuilder, sse_frame
 from ...tools import ToolParserManager, detect_tool_parser
 
@@ -163,8 +164,8 @@ class eSurgeApiServer:
                         lines.append(f'esurge_{k}{{model="{name}"}} {v}')
             return PlainTextResponse("\n".join(lines) + "\n")
 
-        @app.exception_handler(ValueError)
-        async def refused(request: Request, e: ValueError):      # what the engine does not take: a token outside the vocabulary, a prompt too long
+        @app.exception_handler(InvalidRequest)
+        async def refused(request: Request, e: InvalidRequest):      # what the engine does not take: a token outside the vocabulary, a prompt too long
             return JSONResponse(status_code=400, content={"error": {"message": str(e), "type": "invalid_request_error"}})
 
         @app.get("/v1/models")

@@ -92,7 +92,7 @@ class _SamplingFields(_Open):
     stop_token_ids: list[int] | None = None
 
     def to_sampling_params(self, default_max_tokens: int = 256):
-        from .sampling_params import SamplingParams
+        from .sampling_params import InvalidRequest, SamplingParams
 
         mt = self.max_completion_tokens or self.max_tokens or default_max_tokens
         kw = dict(max_tokens=mt, n=self.n, stop=self.stop, seed=self.seed)
@@ -102,7 +102,10 @@ class _SamplingFields(_Open):
             if v is not None:
                 kw[k] = v
         if self.logit_bias:
-            kw["logit_bias"] = {int(k): float(v) for k, v in self.logit_bias.items()}
+            try:
+                kw["logit_bias"] = {int(k): float(v) for k, v in self.logit_bias.items()}
+            except (TypeError, ValueError):
+                raise InvalidRequest("logit_bias maps token ids to numbers") from None
         return SamplingParams(**kw)
 
 

@@ -6,6 +6,10 @@ import typing as tp
 from dataclasses import dataclass, field
 
 
+class InvalidRequest(ValueError):
+    """What a request asks for cannot be had: its own fault, which a server answers as such."""
+
+
 @dataclass
 class SamplingParams:
     n: int = 1
@@ -38,27 +42,27 @@ class SamplingParams:
 
     def __post_init__(self):
         if self.n < 1:
-            raise ValueError("n must be at least 1")
+            raise InvalidRequest("n must be at least 1")
         if self.best_of is not None and self.best_of < self.n:
-            raise ValueError("best_of must be >= n")
+            raise InvalidRequest("best_of must be >= n")
         if self.temperature < 0:
-            raise ValueError("temperature must be non-negative")
+            raise InvalidRequest("temperature must be non-negative")
         if not 0.0 < self.top_p <= 1.0:
-            raise ValueError("top_p must be in (0, 1]")
+            raise InvalidRequest("top_p must be in (0, 1]")
         if not 0.0 <= self.min_p <= 1.0:
-            raise ValueError("min_p must be in [0, 1]")
+            raise InvalidRequest("min_p must be in [0, 1]")
         if self.top_k < -1:
-            raise ValueError("top_k must be -1 (disabled), 0 (disabled) or positive")
+            raise InvalidRequest("top_k must be -1 (disabled), 0 (disabled) or positive")
         if self.top_k == -1:
             self.top_k = 0
         if self.repetition_penalty <= 0:
-            raise ValueError("repetition_penalty must be positive")
+            raise InvalidRequest("repetition_penalty must be positive")
         if not -2.0 <= self.presence_penalty <= 2.0 or not -2.0 <= self.frequency_penalty <= 2.0:
-            raise ValueError("presence / frequency penalties must be in [-2, 2]")
+            raise InvalidRequest("presence / frequency penalties must be in [-2, 2]")
         if self.max_tokens is not None and self.max_tokens < 1:
-            raise ValueError("max_tokens must be at least 1")
+            raise InvalidRequest("max_tokens must be at least 1")
         if self.min_tokens < 0 or (self.max_tokens is not None and self.min_tokens > self.max_tokens):
-            raise ValueError("min_tokens must be in [0, max_tokens]")
+            raise InvalidRequest("min_tokens must be in [0, max_tokens]")
         if isinstance(self.stop, str):
             self.stop = [self.stop]
         self.stop = list(self.stop or [])

@@ -16,6 +16,8 @@ import typing as tp
 import numpy as np
 import torch
 
+from .sampling_params import InvalidRequest
+
 _NONE = np.zeros(0, np.int32), np.zeros(0, np.float32)
 
 
@@ -24,7 +26,7 @@ def pack_tokens(ids: tp.Iterable[int], vocab: int) -> np.ndarray:
     bits = np.zeros((vocab + 31) // 32 * 32, np.uint8)
     at = np.fromiter(ids, np.int64)
     if at.size and not (0 <= at.min() and at.max() < vocab):
-        raise ValueError(f"token ids from {at.min()} to {at.max()} for a vocabulary of {vocab}")
+        raise InvalidRequest(f"token ids from {at.min()} to {at.max()} for a vocabulary of {vocab}")
     bits[at] = 1
     return np.packbits(bits, bitorder="little").view(np.int32)
 
@@ -42,13 +44,13 @@ class TokenRules:
         self.vocab, self.grammar, self.min_tokens = vocab, sp.guided_decoding if callable(sp.guided_decoding) else None, sp.min_tokens
         bias = {int(t): float(v) for t, v in (sp.logit_bias or {}).items()}
         if any(not 0 <= t < vocab or v != v for t, v in bias.items()):
-            raise ValueError(f"logit_bias names a token outside the vocabulary of {vocab}, or is not a number")
+            raise InvalidRequest(f"logit_bias names a token outside the vocabulary of {vocab}, or is not a number")
         self.bias = _entries(bias) if bias else _NONE
         ends = {int(t): -np.inf for t in end_tokens if 0 <= t < vocab} if sp.min_tokens else {}
         self.bias_short = _entries({**bias, **ends}) if ends else self.bias      # while there are fewer than min_tokens
         self.allowed = None if sp.allowed_token_ids is None else pack_tokens(sp.allowed_token_ids, vocab)
         if self.allowed is not None and not self.allowed.any():
-            raise ValueError("allowed_token_ids is empty")
+            raise InvalidRequest("allowed_token_ids is empty")
         self._tokens = pack_tokens(range(vocab), vocab) if self.grammar is not None else None      # the last word's other bits name none
         self.error: Exception | None = None      # of the grammar
 
