@@ -112,6 +112,39 @@ _COMPILE_ONLY_OPTIONS = frozenset({
     "resolution_buckets", "vision_cache_capacity_mb"})
 
 
+class OutputStream:
+    """Outputs of a queued request, as they come. The request ends with its stream: one that is closed or dropped aborts what is left of it, also
+    before the first output was asked for."""
+
+    def __init__(self, engine: "eSurge", request_id: str):
+        self.request_id = request_id
+        self._engine, self._tracked = engine, engine._tracked[request_id]
+        self._it = engine._outputs(self._tracked)
+
+    def __iter__(self) -> "OutputStream":
+        return self
+
+    def __next__(self) -> RequestOutput:
+        try:
+            return next(self._it)
+        except BaseException:      # the end among them
+            self.close()
+            raise
+
+    def close(self) -> None:
+        if self._engine is None:
+            return
+        engine, self._engine = self._engine, None
+        self._it.close()
+        if not self._tracked.finished:
+            engine.abort_request(self.request_id)
+        engine._tracked.pop(self.request_id, None)
+
+    def __del__(self):
+        if getattr(self, "_engine", None) is not None:
+            self.close()
+
+
 class eSurge:
     def __init__(self, model, tokenizer=None, processor=None, max_model_len: int = 8192, max_num_seqs: int = 256,
                  max_num_batched_tokens: int | None = None, hbm_utilization: float = 0.85, page_size: int = PAGE_SIZE,
@@ -621,27 +654,23 @@ class eSurge:
                 break
 
     def stream(self, prompt, sampling_params: SamplingParams | None = None, request_id: str | None = None,
-               images: list | None = None, videos: list | None = None, adapter: str | None = None) -> tp.Iterator[RequestOutput]:
-        """Yields a ``RequestOutput`` whenever new tokens arrive (``delta_text`` holds the increment)."""
-        rid = self.add_request(prompt, sampling_params, request_id, images=images, videos=videos, adapter=adapter)
-        tr = self._tracked[rid]
+               images: list | None = None, videos: list | None = None, adapter: str | None = None) -> "OutputStream":
+        """Queues the request and gives a ``RequestOutput`` whenever new tokens arrive (``delta_text`` holds the increment)."""
+        return OutputStream(self, self.add_request(prompt, sampling_params, request_id, images=images, videos=videos, adapter=adapter))
+
+    def _outputs(self, tr: _Tracked) -> tp.Iterator[RequestOutput]:
         background = self._thread is not None and self._thread.is_alive()
-        try:
-            while True:
-                if not background:
-                    self.step()
-                else:
-                    tr.event.wait(timeout=1.0)
-                tr.event.clear()
-                fin = tr.finished
-                if tr.pending_ids or fin:
-                    yield self._snapshot(tr, fin)
-                if fin:
-                    break
-        finally:
-            if not tr.finished:
-                self.abort_request(rid)
-            self._tracked.pop(rid, None)
+        while True:
+            if not background:
+                self.step()
+            else:
+                tr.event.wait(timeout=1.0)
+            tr.event.clear()
+            fin = tr.finished
+            if tr.pending_ids or fin:
+                yield self._snapshot(tr, fin)
+            if fin:
+                break
 
     def chat(self, messages: list[dict], sampling_params: SamplingParams | None = None, tools: list | None = None,
              stream: bool = False, chat_template: str | None = None, adapter: str | None = None, **template_kwargs):

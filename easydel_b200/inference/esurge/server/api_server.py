@@ -149,6 +149,10 @@ class eSurgeApiServer:
                 if close:
                     await loop.run_in_executor(None, close)
 
+        async def opened(engine, prompt, sp, name):
+            """The engine's iterator over a queued request: what it refuses is an answer of its own, not a stream that breaks off."""
+            return await asyncio.get_running_loop().run_in_executor(None, functools.partial(engine.stream, prompt, sp, **server._adapter(name)))
+
         @app.get("/health")
         async def health():
             return {"status": "ok", "uptime_s": time.time() - server.started,
@@ -204,6 +208,8 @@ class eSurgeApiServer:
                 return ChatCompletionResponse(model=name, usage=_usage(out), choices=[
                     ChatCompletionResponseChoice(message=msg, finish_reason=_finish_reason(out, bool(calls)))])
 
+            outputs = await opened(engine, prompt, sp, name)
+
             async def gen():
                 rid = None
                 first = ChatCompletionStreamResponse(model=name, choices=[
@@ -211,7 +217,7 @@ class eSurgeApiServer:
                 rid = first.id
                 yield sse(first)
                 last, text, any_tools = None, "", False
-                async for out in pump(request, engine, engine.stream(prompt, sp, **server._adapter(name))):
+                async for out in pump(request, engine, outputs):
                     last = out
                     text += out.delta_text
                     d = parser.parse_streaming(text, final=out.finished)
@@ -257,10 +263,12 @@ class eSurgeApiServer:
                 server.auth.record_usage(rec, usage.prompt_tokens, usage.completion_tokens)
                 return CompletionResponse(model=name, choices=choices, usage=usage)
 
+            outputs = await opened(engine, prompts[0], sp, name)
+
             async def gen():
                 last = None
                 cid = None
-                async for out in pump(request, engine, engine.stream(prompts[0], sp, **server._adapter(name))):
+                async for out in pump(request, engine, outputs):
                     last = out
                     chunk = CompletionResponse(model=name, choices=[CompletionResponseChoice(
                         text=out.delta_text, finish_reason=_finish_reason(out, False) if out.finished else None)],
@@ -305,11 +313,13 @@ class eSurgeApiServer:
                 parser = server._parser(engine, bool(req.tools))
                 builder = ResponsesStreamBuilder(model=name, previous_response_id=req.previous_response_id)
 
+                outputs = await opened(engine, prompt, sp, name)
+
                 async def gen():
                     for ev, payload in builder.start():
                         yield sse_frame(ev, payload)
                     last, text = None, ""
-                    async for out in pump(request, engine, engine.stream(prompt, sp, **server._adapter(name))):
+                    async for out in pump(request, engine, outputs):
                         last = out
                         text += out.delta_text
                         d = parser.parse_streaming(text, final=out.finished)
