@@ -639,8 +639,15 @@ class eSurge:
         ads = list(adapter) if isinstance(adapter, (list, tuple)) else [adapter] * len(plist)
         if len(ads) != len(plist):
             raise ValueError(f"{len(ads)} adapters for {len(plist)} prompts")
-        ids = [self.add_request(p, sp, rid, images=im, videos=vd, adapter=ad)
-               for p, sp, rid, im, vd, ad in zip(plist, sps, rids, imgs, vids, ads)]
+        ids: list[str] = []
+        try:
+            for p, sp, rid, im, vd, ad in zip(plist, sps, rids, imgs, vids, ads):
+                ids.append(self.add_request(p, sp, rid, images=im, videos=vd, adapter=ad))
+        except BaseException:      # nobody waits for those before the one that was refused
+            for rid in ids:
+                self.abort_request(rid)
+                self._tracked.pop(rid, None)
+            raise
         self._drive(lambda: all(self._tracked[i].finished for i in ids))
         outs = [self._snapshot(self._tracked.pop(i), True) for i in ids]
         return outs

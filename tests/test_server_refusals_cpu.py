@@ -81,3 +81,12 @@ def test_two_streams_at_once(engine):
     a, b = engine.stream([5, 6, 7], sp), engine.stream([9, 10], sp)
     got = [list(a)[-1], list(b)[-1]]
     assert [o.outputs[0].token_ids for o in got] == want and not engine._tracked
+
+
+def test_a_refused_request_of_a_batch_leaves_none_behind(engine):
+    ok, bad = SamplingParams(max_tokens=6, temperature=0.0, ignore_eos=True), SamplingParams(logit_bias={4000: 1.0})
+    for _ in range(2 * engine.runner.max_num_seqs):
+        with pytest.raises(InvalidRequest):
+            engine.generate([[5, 6], [7, 8], [9, 10]], [ok, ok, bad])
+    assert not engine.scheduler.has_unfinished() and not engine._tracked and len(engine._free_slots) == engine.runner.max_num_seqs
+    assert len(engine.generate([[5, 6], [7, 8]], ok)) == 2
