@@ -98,7 +98,7 @@ class AdapterSet:
                 if lin.adapters is not None:
                     raise RuntimeError(f"{name}.{leaf} has adapters of another engine: close that one first")
                 w = getattr(lin, "weight", None)
-                dtype, device = (w.dtype, w.device) if w is not None else (model.param_dtype, lin.codes.device)
+                dtype, device = (w.dtype, w.device) if w is not None else (model.dtype, lin.codes.device)      # that of the rows
                 self.banks[f"{name}.{leaf}"] = AdapterBank(self, lin, count, self.rank, dtype, device)
         if not self.banks:
             raise NotImplementedError(f"{type(model).__name__} has no attention or feed-forward projections that take adapters")
