@@ -257,8 +257,9 @@ class QuantizedLinear(nn.Module):
 
             y = quantized_matmul(x, self.tensor(), None)
             y = tp.all_reduce(y, tp_group)
-            return y if self.bias is None else y + self.bias
-        y = quantized_matmul(x, self.tensor(), self.bias)
+            y = y if self.bias is None else y + self.bias
+        else:
+            y = quantized_matmul(x, self.tensor(), self.bias)
         return y if self.adapters is None else self.adapters.add(y, x)
 
     def extra_repr(self) -> str:

@@ -50,3 +50,15 @@ def test_projections(fmt, dtype, param_dtype):
     run_projections(model, aset, 7, dtype)
     with torch.no_grad(), aset.rows(torch.zeros(8, dtype=torch.int32)):
         assert torch.isfinite(model(input_ids=torch.arange(8)[None], apply_lm_head=False).last_hidden_state).all()
+
+
+def test_a_row_parallel_projection_of_one_rank_has_its_adapter(monkeypatch):
+    from easydel_b200.parallel import tp
+
+    monkeypatch.setattr(tp, "all_reduce", lambda y, group: y)
+    model = quantized("int8", torch.float32)
+    aset = loaded(model)
+    for name in ("self_attn.o_proj", "mlp.down_proj"):
+        lin = model.get_submodule(f"model.layers.0.{name}")
+        lin.tp_group, lin.parallel_style = object(), "row"
+    run_projections(model, aset, 5, torch.float32)
