@@ -33,6 +33,7 @@ _lib.register("edl_lora_backward", i32, [vp, vp, vp, vp, vp, vp, vp, vp, f32, vp
 MAX_RANK = 512       # ranks of all parts together
 MAX_PARTS = 8
 MAX_TRAINED = 65535  # adapters of a call with gradients
+MAX_ROWS = 2 ** 31 - 1
 BLOCK = 256          # rows that are looked through for their adapters together
 
 
@@ -75,6 +76,8 @@ def _check(y, x, a, b, index, scale, parts, out):
         raise ValueError(f"{sa[1]} ranks over all parts; at most {MAX_RANK}")
     if not sx or sx[-1] != sa[2]:
         raise ValueError(f"rows of x have {sx[-1] if sx else 0} elements, the adapters take {sa[2]}")
+    if x.numel() // sx[-1] > MAX_ROWS:
+        raise ValueError(f"{x.numel() // sx[-1]} rows; at most {MAX_ROWS}")
     if sy[:-1] != sx[:-1] or len(sy) != len(sx) or sy[-1] != N:
         raise ValueError(f"y is {tuple(sy)}, x and the adapters ask for {(*sx[:-1], N)}")
     if dt not in (torch.bfloat16, torch.float32) or a.dtype != dt or b.dtype != dt:
