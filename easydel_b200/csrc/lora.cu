@@ -1435,7 +1435,7 @@ __device__ __forceinline__ void write_grad(cg::cluster_group& cluster, const Gra
 // out[rank, col] (+)= sum over the adapter's rows t of p[t, rank] z[t, col]: ranks x 256 columns per cluster, the rows cut over its CTAs.
 // This form takes rows of any alignment and fp32 ones: 16 ranks at a time, operands along their rows from global memory, turned in registers.
 // Warps 0-3 and 4-7 take every other 16 rows. 1000 rows, 1023 and 1021 columns, rank 5: 12 us; 4096 rows of fp32, 4096 and 4096 columns, rank 16:
-// 139 us, bound by its products of parts.
+// 89 us, 134 MB at 1.5 TB/s: elements are cut into parts in registers, between loads that wait for the products of the rows before.
 template <typename T, int S, bool WIDE>
 __global__ void __launch_bounds__(LORA_THREADS, 1) lora_grad_any_kernel(const __grid_constant__ GradArgs a) {
   constexpr int P = PARTS<T>;
